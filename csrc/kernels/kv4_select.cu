@@ -1,0 +1,318 @@
+// Choosing the pages that a query attends to, per token and K/V head.
+//
+// The score of a page is an upper bound on the logits of the head's query rows against the
+// page's keys, from the page bounds that kv4_cache.cu keeps (hi, lo in units e):
+//   score = max over the head's rows of f e sum_d (max(r_d, 0) hi_d + min(r_d, 0) lo_d),
+// r = round(q / f), f the smallest power of two with max |q| <= 127 f.  The sum is an integer
+// below 2^24 (D <= 256 products of 7-bit numbers), f and e are powers of two: the score is
+// exact in f32 whatever the order of the additions, so every rank and every replay of a step
+// makes the same choice.  Ties go to the lowest page.
+//
+// Two launches.  Scores: the sum over d is one int8 matrix product of depth 2 D, [r+ | r-] by
+// [hi | lo]; a warp holds 16 pages' bounds as A fragments (16-byte loads, straight from
+// memory: each byte is used by one block per token tile) and walks over the rows' B fragments
+// in shared memory.  Bound by the bounds' bytes (2 D per page and head) in a decode step, by
+// the int8 product in a prompt chunk.  Choice: a block per (token, head) finds the threshold
+// by four passes of a radix search over the ordered bits and writes the pages in order.
+#include "kv4.cuh"
+#include "torch_glue.h"
+
+namespace moet {
+namespace kv4 {
+
+struct SelectArgs {
+  const void* q; long long q_tok; int q_head;
+  const int *cu_q, *seq_lens, *table; int B, W, T, H, G;
+  int gp, tpc;                        // rows reserved per token (a power of two or a multiple of 8), tokens per block
+  int tiles, chunks;                  // token tiles per sequence, page chunks
+  const int8_t* bounds; const float* unit; int n_pages;
+  float* score; int first, last, budget;
+  int* pages;
+  int* status;
+};
+
+constexpr int kScoreWarps = 8, kScoreRows = 64;     // rows per block: 8 n-tiles
+
+MOET_DEVICE void mma_s8_16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// first row and row count of a sequence, the position of its first row
+MOET_DEVICE void seq_rows(const SelectArgs& a, int b, int& c0, int& nq, int& p0) {
+  c0 = max(0, min(a.cu_q[b], a.T));
+  nq = max(0, max(0, min(a.cu_q[b + 1], a.T)) - c0);
+  p0 = min(a.seq_lens[b], a.W * kPage) - nq;
+}
+// pages of a row at position p that compete for a place: [first, n - last), n = p / 64 + 1
+MOET_DEVICE int rivals_end(const SelectArgs& a, int p) { return p < 0 ? 0 : p / kPage + 1 - a.last; }
+
+template <int D, typename T16>
+__global__ void __launch_bounds__(kScoreWarps * 32) kv4_score_kernel(SelectArgs a) {
+  constexpr int KB = 2 * D, STRIDE = KB + 64;       // rows 64 bytes apart in the banks: 16-byte reads do not meet
+  constexpr int CH = KB / 64;                       // 16-byte pieces of a lane per page
+  __shared__ __align__(16) int8_t rows[kScoreRows * STRIDE];
+  __shared__ float unit_q[kScoreRows];
+  pdl_entry();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int h = blockIdx.y, chunk = blockIdx.x % a.chunks, bt = blockIdx.x / a.chunks;
+  const int b = bt / a.tiles, tile = bt % a.tiles;
+  int c0, nq, p0;
+  seq_rows(a, b, c0, nq, p0);
+  const int i0 = tile * a.tpc, ntok = min(a.tpc, nq - i0);
+  if (ntok <= 0) return;
+  const int end = rivals_end(a, p0 + i0 + ntok - 1);       // the last token's
+  const int page0 = chunk * (kScoreWarps * 16);
+  if (page0 >= end) return;
+  if (p0 + i0 + ntok - 1 < a.budget * kPage) return;       // every token takes all its pages
+
+  // ---- rows: r = round(q / f) as [max(r, 0) | min(r, 0)]
+  const int nrows = ntok * a.gp;
+  constexpr int E = D / 32;                                // values per lane
+  for (int r = warp; r < ((nrows + 7) & ~7); r += kScoreWarps) {
+    const int ti = r / a.gp, gi = r % a.gp;
+    const bool live = ti < ntok && gi < a.G;
+    float v[E], amax = 0.f;
+    if (live) {
+      const T16* p = (const T16*)a.q + (long long)(c0 + i0 + ti) * a.q_tok + (long long)(h * a.G + gi) * a.q_head + lane * E;
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        float x = to_f32(p[e]);
+        x = x != x ? 0.f : fminf(fmaxf(x, -3.4028235e38f), 3.4028235e38f);
+        v[e] = x;
+        amax = fmaxf(amax, fabsf(x));
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; e++) v[e] = 0.f;
+    }
+    amax = warp_max(amax);
+    const int ex = exp_for_127(amax);
+    const float inv = pow2f(-ex);
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      const int x = __float2int_rn(v[e] * inv);
+      rows[r * STRIDE + lane * E + e] = (int8_t)max(x, 0);
+      rows[r * STRIDE + D + lane * E + e] = (int8_t)min(x, 0);
+    }
+    if (lane == 0) unit_q[r] = live ? pow2f(ex) : 0.f;
+  }
+  __syncthreads();
+
+  // ---- 16 pages per warp
+  const int pg = page0 + warp * 16;
+  if (pg >= end) return;
+  uint4 x[2][CH];
+  float u[2];
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const int page = pg + g + 8 * i;
+    int phys = 0;
+    if (page < end) {                                      // end <= W
+      phys = a.table[(long long)b * a.W + page];
+      if (phys < 0 || phys >= a.n_pages) {
+        set_status(a.status, kBadIndex);
+        phys = 0;
+      }
+    }
+    const int8_t* p = a.bounds + ((long long)phys * a.H + h) * KB + t * 16;
+#pragma unroll
+    for (int c = 0; c < CH; c++) x[i][c] = *reinterpret_cast<const uint4*>(p + c * 64);
+    u[i] = a.unit[(long long)phys * a.H + h];
+  }
+  const int wide = (a.gp + 7) / 8;                         // n-tiles of one token
+  float best[2] = {-INFINITY, -INFINITY};
+  const int ntiles = (nrows + 7) / 8;
+  for (int n = 0; n < ntiles; n++) {
+    int d[4] = {0, 0, 0, 0};
+    const int8_t* rp = rows + (n * 8 + g) * STRIDE + t * 16;
+#pragma unroll
+    for (int c = 0; c < CH; c++) {
+      const uint4 y = *reinterpret_cast<const uint4*>(rp + c * 64);
+      mma_s8_16832(d, x[0][c].x, x[1][c].x, x[0][c].y, x[1][c].y, y.x, y.y);
+      mma_s8_16832(d, x[0][c].z, x[1][c].z, x[0][c].w, x[1][c].w, y.z, y.w);
+    }
+    const int r0 = n * 8 + 2 * t;
+    const float f0 = unit_q[r0], f1 = unit_q[r0 + 1];
+    float s[4];                                            // (page g, row 2t), (g, 2t+1), (g + 8, 2t), (g + 8, 2t + 1)
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const float f = (k & 1) ? f1 : f0;
+      s[k] = f > 0.f ? (float)d[k] * f * u[k >> 1] : -INFINITY;
+    }
+    float* out = a.score + ((long long)(c0 + i0) * a.H + h) * a.W;       // + token * H * W + page
+    const long long tstep = (long long)a.H * a.W;
+    if (a.gp == 1) {
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const int ti = r0 + (k & 1), page = pg + g + 8 * (k >> 1);
+        if (ti < ntok && page < end) out[ti * tstep + page] = s[k];
+      }
+      continue;
+    }
+    float m[2] = {fmaxf(s[0], s[1]), fmaxf(s[2], s[3])};
+    if (a.gp >= 4) {
+#pragma unroll
+      for (int i = 0; i < 2; i++) m[i] = fmaxf(m[i], __shfl_xor_sync(0xffffffffu, m[i], 1));
+    }
+    if (a.gp >= 8) {
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        m[i] = fmaxf(m[i], __shfl_xor_sync(0xffffffffu, m[i], 2));
+        best[i] = fmaxf(best[i], m[i]);
+        m[i] = best[i];
+      }
+      if (n % wide != wide - 1) continue;                  // the token goes on in the next tile
+      best[0] = best[1] = -INFINITY;
+    }
+    const int ti = r0 / a.gp;
+    if (r0 % a.gp == 0 || (a.gp > 8 && t == 0)) {
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const int page = pg + g + 8 * i;
+        if (ti < ntok && page < end) out[ti * tstep + page] = m[i];
+      }
+    }
+  }
+}
+
+MOET_DEVICE uint32_t order_bits(float f) {
+  const uint32_t u = __float_as_uint(f == 0.f ? 0.f : f);  // -0 and 0 are one score
+  return u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u);
+}
+
+constexpr int kPickThreads = 128;
+
+__global__ void __launch_bounds__(kPickThreads) kv4_pick_kernel(SelectArgs a) {
+  pdl_entry();
+  __shared__ uint32_t hist[256];
+  __shared__ int scan[kPickThreads / 32][2];
+  __shared__ uint32_t prefix_s;
+  __shared__ int remain_s;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tok = blockIdx.x / a.H, h = blockIdx.x % a.H;
+  int lo = 0, hi = a.B;                                    // the token's sequence
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (max(0, min(a.cu_q[mid], a.T)) <= tok) lo = mid; else hi = mid;
+  }
+  int c0, nq, p0;
+  seq_rows(a, lo, c0, nq, p0);
+  const int p = tok - c0 < nq ? p0 + tok - c0 : -1, n = p < 0 ? 0 : p / kPage + 1;
+  int* out = a.pages + ((long long)tok * a.H + h) * a.budget;
+  if (n <= a.budget) {
+    for (int i = tid; i < a.budget; i += kPickThreads) out[i] = i < n ? i : -1;
+    return;
+  }
+  const int end = n - a.last, want = a.budget - a.first - a.last;   // rivals: [first, end), more than `want`
+  for (int i = tid; i < a.first; i += kPickThreads) out[i] = i;
+  for (int i = tid; i < a.last; i += kPickThreads) out[a.budget - a.last + i] = end + i;
+  if (want == 0) return;
+  const float* row = a.score + ((long long)tok * a.H + h) * a.W;
+  uint32_t prefix = 0, mask = 0;
+  int remain = want;
+#pragma unroll 1
+  for (int shift = 24; shift >= 0; shift -= 8) {
+    for (int i = tid; i < 256; i += kPickThreads) hist[i] = 0;
+    __syncthreads();
+    for (int i = a.first + tid; i < end; i += kPickThreads) {
+      const uint32_t k = order_bits(row[i]);
+      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1u);
+    }
+    __syncthreads();
+    if (warp == 0) {       // the bin, from the top, in which the count reaches `remain`
+      uint32_t c[8], sum = 0;
+#pragma unroll
+      for (int i = 0; i < 8; i++) c[i] = hist[255 - (lane * 8 + i)], sum += c[i];
+      uint32_t before = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += y;
+      }
+      before -= sum;
+      if ((int)before < remain && (int)(before + sum) >= remain) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          if ((int)before < remain && (int)(before + c[i]) >= remain) {
+            prefix_s = prefix | (uint32_t)(255 - (lane * 8 + i)) << shift;
+            remain_s = remain - (int)before;
+          }
+          before += c[i];
+        }
+      }
+    }
+    __syncthreads();
+    prefix = prefix_s;
+    remain = remain_s;
+    mask |= 255u << shift;
+  }
+  // take what is above the threshold, and the first `remain` that equal it, in page order
+  int above = 0, equal = 0;                                // taken so far
+  for (int i0 = a.first; i0 < end; i0 += kPickThreads) {
+    const int i = i0 + tid;
+    const uint32_t k = i < end ? order_bits(row[i]) : 0;
+    const bool gt = i < end && k > prefix, eq = i < end && k == prefix;
+    const uint32_t bg = __ballot_sync(0xffffffffu, gt), be = __ballot_sync(0xffffffffu, eq);
+    if (lane == 0) scan[warp][0] = __popc(bg), scan[warp][1] = __popc(be);
+    __syncthreads();
+    int ng = above, ne = equal;
+    for (int w = 0; w < warp; w++) ng += scan[w][0], ne += scan[w][1];
+    for (int w = 0; w < kPickThreads / 32; w++) above += scan[w][0], equal += scan[w][1];
+    const uint32_t below = (1u << lane) - 1;
+    ng += __popc(bg & below), ne += __popc(be & below);
+    if (gt || (eq && ne < remain)) out[a.first + ng + min(ne, remain)] = i;
+    __syncthreads();
+  }
+}
+
+}  // namespace kv4
+}  // namespace moet
+
+using namespace moet;
+using namespace moet::kv4;
+
+void kv4_select(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_lens, torch::Tensor table, torch::Tensor bounds,
+                torch::Tensor unit, int64_t max_q, int64_t first, int64_t last, torch::Tensor score,
+                torch::Tensor pages, torch::Tensor status) {
+  SelectArgs a;
+  const int D = (int)q.size(2);
+  a.T = (int)q.size(0); a.H = (int)bounds.size(1); a.G = (int)(q.size(1) / a.H);
+  a.B = (int)seq_lens.size(0); a.W = (int)table.size(1);
+  a.q = q.data_ptr(); a.q_tok = q.stride(0); a.q_head = (int)q.stride(1);
+  a.cu_q = (const int*)cu_q.data_ptr(); a.seq_lens = (const int*)seq_lens.data_ptr();
+  a.table = (const int*)table.data_ptr();
+  a.bounds = (const int8_t*)bounds.data_ptr(); a.unit = (const float*)unit.data_ptr(); a.n_pages = (int)bounds.size(0);
+  a.score = (float*)score.data_ptr(); a.first = (int)first; a.last = (int)last; a.budget = (int)pages.size(2);
+  a.pages = (int*)pages.data_ptr();
+  a.status = (int*)status.data_ptr();
+  TORCH_CHECK(a.G <= kScoreRows, "kv4_select: at most ", kScoreRows, " query heads per K/V head, got ", a.G);
+  TORCH_CHECK(first >= 0 && last >= 1 && first + last <= a.budget, "kv4_select: first + last pages exceed the budget");
+  TORCH_CHECK((a.W <= a.budget || score.numel() >= (int64_t)a.T * a.H * a.W) && pages.numel() == (int64_t)a.T * a.H * a.budget,
+              "kv4_select: score / pages do not fit the batch");
+  if (a.T == 0 || a.B == 0) return;
+  a.gp = 1;
+  while (a.gp < a.G && a.gp < 8) a.gp *= 2;
+  if (a.G > 8) a.gp = (a.G + 7) / 8 * 8;
+  a.tpc = kScoreRows / a.gp;
+  a.tiles = (int)((std::min<int64_t>(max_q, a.T) + a.tpc - 1) / a.tpc);
+  a.chunks = (a.W + kScoreWarps * 16 - 1) / (kScoreWarps * 16);
+  const int64_t blocks = (int64_t)a.B * a.tiles * a.chunks;
+  TORCH_CHECK(blocks < (int64_t)1 << 31 && (int64_t)a.T * a.H < (int64_t)1 << 31, "kv4_select: too much work for one call");
+  auto stream = at::cuda::getCurrentCUDAStream();
+  const dim3 grid((unsigned)blocks, a.H), block(kScoreWarps * 32);
+  auto go = [&](auto dim) {
+    constexpr int DD = decltype(dim)::value;
+    if (q.scalar_type() == at::kHalf) launch_k(kv4_score_kernel<DD, __half>, grid, block, 0, stream, a);
+    else launch_k(kv4_score_kernel<DD, __nv_bfloat16>, grid, block, 0, stream, a);
+  };
+  if (a.W > a.budget) {               // else every token takes all its pages
+    if (D == 64) go(std::integral_constant<int, 64>{});
+    else if (D == 128) go(std::integral_constant<int, 128>{});
+    else go(std::integral_constant<int, 256>{});
+  }
+  launch_k(kv4_pick_kernel, dim3((unsigned)((int64_t)a.T * a.H)), dim3(kPickThreads), 0, stream, a);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
