@@ -116,12 +116,11 @@ void kv4_append(torch::Tensor k, torch::Tensor v, torch::Tensor slots, torch::Te
 void kv4_read(torch::Tensor slots, torch::Tensor pages, int64_t k_exp, int64_t v_exp, torch::Tensor k, torch::Tensor v,
               torch::Tensor status);
 // kv4_attend.cu
-std::tuple<int64_t, int64_t> kv4_attend_workspace(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t max_q,
-                                                  bool chosen);
+std::tuple<int64_t, int64_t> kv4_attend_workspace(int64_t G, int64_t D, int64_t max_q, bool chosen);
 void kv4_attend(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_lens, torch::Tensor table, torch::Tensor pages,
                 c10::optional<torch::Tensor> sel, double scale, int64_t max_q, int64_t window, int64_t k_exp,
                 int64_t v_exp, torch::Tensor out, c10::optional<torch::Tensor> lse, torch::Tensor part,
-                torch::Tensor counters, torch::Tensor status);
+                torch::Tensor split, torch::Tensor status);
 // kv4_select.cu
 void kv4_select(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_lens, torch::Tensor table, torch::Tensor bounds,
                 torch::Tensor unit, int64_t max_q, int64_t first, int64_t last, torch::Tensor score,

@@ -1,11 +1,11 @@
 // Layout of the 4-bit paged K/V cache and the conversions its kernels share.
 //
-// A page holds 64 positions of one K/V head as two sub-blocks of 32 positions; a sub-block
-// is 36 D contiguous bytes (D = 64, 128 or 256 values per row):
-//   [ 0 D, 16 D)  key codes     [slab][32 tokens][piece t < 4][SD / 8 bytes]
-//   [16 D, 18 D)  key scales    [32 tokens][D / 16]           e4m3
-//   [18 D, 34 D)  value codes   [slab][16 token pairs][g < 8][token of the pair][SD / 16 bytes]
-//   [34 D, 36 D)  value scales  [16 token pairs][D / 16][token of the pair]   e4m3
+// A page holds 64 positions of one K/V head in 72 D contiguous bytes (D = 64, 128 or 256
+// values per row), keys first, so that either half is one copy:
+//   [ 0 D, 32 D)  key codes     [slab][64 tokens][piece t < 4][SD / 8 bytes]
+//   [32 D, 36 D)  key scales    [64 tokens][D / 16]           e4m3
+//   [36 D, 68 D)  value codes   [slab][32 token pairs][g < 8][token of the pair][SD / 16 bytes]
+//   [68 D, 72 D)  value scales  [32 token pairs][D / 16][token of the pair]   e4m3
 // A slab is SD = min(D, 128) values.  The orders are those in which a warp's m16n8k16
 // fragments want them, so one wide shared-memory load per token gives a lane all that it
 // needs of a row and no two lanes meet in a bank:
@@ -24,14 +24,14 @@ namespace moet {
 namespace kv4 {
 
 constexpr int kPage = 64;   // positions per page
-constexpr int kSub = 32;    // positions per sub-block
 
 template <int D> struct Lay {
   static constexpr int SD = D < 128 ? D : 128;       // values per slab
   static constexpr int NS = D / SD;                  // slabs
   static constexpr int NB = D / 16;                  // scale blocks per row
-  static constexpr int KC = 0, KS = 16 * D, VC = 18 * D, VS = 34 * D, kSubBytes = 36 * D;
-  static constexpr int kPageBytes = 2 * kSubBytes;
+  static constexpr int KC = 0, KS = 32 * D, VC = 36 * D, VS = 68 * D;
+  static constexpr int kHalfBytes = 36 * D, kPageBytes = 72 * D;
+  static constexpr int kSlabBytes = kPage * SD / 2;  // codes of a slab
 };
 
 // four bytes of two e2m1 codes each -> four f16x2 (low code in the low half)

@@ -13,11 +13,13 @@
 // bits, three more than a bf16 output has); maxima, sums and outputs stay in 32 bits.
 //
 // What bounds it is the cache's bytes (a long context), so each warp streams its own units
-// (64 positions; 32 with D = 256) through a private ring of bulk copies, one contiguous copy
-// per unit, with no block-wide barrier inside a tile.  Work is split evenly: the units of all
-// (sequence, row tile, head) tiles lie on one line, each block takes an equal stretch of it,
-// and a tile that several blocks share is joined by the last of them to arrive, in block
-// order (the order of arrival changes nothing in the result).
+// (pages) through a private ring of bulk copies, one for a page's keys and one for its
+// values, with no block-wide barrier inside a tile.  Work is split evenly: the units of all
+// (sequence, row tile, head) tiles lie on one line and each block takes an equal stretch of
+// it.  A tile that lies within one block is finished there; of the others each block leaves
+// its part (maxima, sums, unnormalised outputs), and kv4_join_kernel adds the parts up in
+// block order.  A split tile is named by the block in which it begins, so the join needs no
+// counters and its grid is the first one's.
 #include "kv4.cuh"
 #include "tcgen05.cuh"
 #include "torch_glue.h"
@@ -37,25 +39,37 @@ struct AttendArgs {
   float scale_log2;                                     // scale * log2(e) * 2^k_exp
   float v_mul;                                          // 2^v_exp
   void* out; float* lse;                                // [T, H * G, D], [T, H * G] or null
-  float* part; int* counters;
+  float* part; int* split;                              // parts: two per block; split: kSplitInts per block
   int min_units;
   int* status;
 };
+// What a block notes of the tile that begins in it and goes on past it:
+// {parts (0: none), head, first row, rows, first token}
+constexpr int kSplitInts = 8;
 
 MOET_DEVICE void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 MOET_DEVICE uint32_t transpose_8x8(uint32_t x) {
   uint32_t d;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
   return d;
 }
 MOET_DEVICE uint32_t pack_f16x2(float a, float b) {
   __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<uint32_t*>(&h);
+}
+// two f32 operations in one instruction
+MOET_DEVICE void mul2(float& x, float& y, float a, float b) {
+  asm("{\n.reg .b64 u, v;\nmov.b64 u, {%0, %1};\nmov.b64 v, {%2, %3};\nmul.rn.ftz.f32x2 u, u, v;\nmov.b64 {%0, %1}, u;\n}\n"
+      : "+f"(x), "+f"(y) : "f"(a), "f"(b));
+}
+MOET_DEVICE void sub2(float& x, float& y, float a, float b) {
+  asm("{\n.reg .b64 u, v;\nmov.b64 u, {%0, %1};\nmov.b64 v, {%2, %3};\nadd.rn.ftz.f32x2 u, u, v;\nmov.b64 {%0, %1}, u;\n}\n"
+      : "+f"(x), "+f"(y) : "f"(-a), "f"(-b));
 }
 MOET_DEVICE float fast_exp2(float x) {
   float y;
@@ -76,34 +90,38 @@ template <typename T16> MOET_DEVICE uint32_t round2(float a, float b);
 template <> MOET_DEVICE uint32_t round2<__nv_bfloat16>(float a, float b) { return pack_bf16x2(a, b); }
 template <> MOET_DEVICE uint32_t round2<__half>(float a, float b) { return pack_f16x2(a, b); }
 
-// A unit of work: 64 (or 32) positions of one tile (sequence, row tile, head).
+// A unit of work: a page of one tile (sequence, row tile, head).
 struct Unit {
   int b, h, row0, rows, tok0, p0;   // tile: rows [row0, row0 + count) of the sequence's; first token, its position
-  int x, n;                         // unit index in the tile, units of the tile
-  int page, tile;                   // logical page (or entry of the choice), counter of the tile
+  int x, n;                         // unit index in the tile, units of the tile: kTileCost empty ones, then its pages
+  int page;                         // logical page (or entry of the choice)
 };
 
-template <int D> struct StepCfg {
-  static constexpr int UT = D == 256 ? 32 : 64;                      // positions of a unit
-  static constexpr int PU = kPage / UT;
-  static constexpr int kUnitBytes = UT / kSub * Lay<D>::kSubBytes;   // 4608, 9216, 9216
-  static constexpr int kStages = D == 64 ? 4 : 2;
+// A tile's queries, join and output take a block as long as about this many of its pages;
+// counted as empty units in front of them, so that many short tiles do not all fall to one block.
+constexpr int kTileCost = 4;
+
+// A unit is one page of a tile.  Its keys and its values are two copies, each into a slot of
+// its own; a warp takes TS tokens per softmax step.
+template <int D, int NT> struct StepCfg {
+  static constexpr int kSlots = NT == 1 ? 2 : 3;                                   // 2304, 4608 or 9216 bytes each
+  static constexpr int TS = NT == 1 ? 64 : 32;                       // as the registers allow
 };
 
-constexpr int kMaxBlocks = 3;       // blocks per SM, at most
+constexpr int kMaxBlocks = 4;       // blocks per SM, at most
+template <int D, int NT> constexpr int blocks_per_sm() { return D <= 128 && NT == 1 ? 4 : 2; }   // by registers
 
 template <int D, int NT> struct StepSmem {
-  using C = StepCfg<D>;
+  using C = StepCfg<D, NT>;
   static constexpr int RT = 8 * NT;
   static constexpr int kRedStride = D + 4;                           // rows 4 banks apart: stores of a quad do not meet
-  uint8_t ring[kWarps][C::kStages][C::kUnitBytes];
-  float red[RT * kRedStride];
+  uint8_t ring[kWarps][C::kSlots][Lay<D>::kHalfBytes];
+  float red[2][RT * kRedStride];                                     // warps 0 and 2, warps 1 and 3
   float wm[kWarps][RT], wl[kWarps][RT];
   float fm[RT], fl[RT];
-  uint64_t bar[kWarps][C::kStages];
-  int start[kWarps][C::kStages];
+  uint64_t bar[kWarps][C::kSlots];
+  int start[kWarps][C::kSlots];
   int scan[kWarps];
-  int last;
 };
 
 // start of sequence b's rows; an offset outside the rows is pulled back into them
@@ -116,19 +134,18 @@ MOET_DEVICE void seq_units(const AttendArgs& a, int b, int& tiles, int& n, int& 
   const int len = max(0, min(a.seq_lens[b], a.W * kPage));
   tiles = (nq * a.G + 8 * NT - 1) / (8 * NT);
   page0 = a.window > 0 ? max(0, len - nq - a.window + 1) / kPage : 0;
-  n = max(1, (len + kPage - 1) / kPage - page0) * StepCfg<D>::PU;    // an empty sequence's rows are still written
+  n = max(1, (len + kPage - 1) / kPage - page0) + kTileCost;      // an empty sequence's rows are still written
 }
 
 template <int D, int NT>
 MOET_DEVICE Unit find_unit(const AttendArgs& a, const int* pre, int u) {
-  constexpr int RT = 8 * NT, PU = StepCfg<D>::PU;
+  constexpr int RT = 8 * NT;
   Unit r;
   if (a.sel) {
     const int nc = (a.G + RT - 1) / RT;
-    r.n = a.budget * PU;
+    r.n = a.budget + kTileCost;
     const int th = u / r.n;
     r.x = u - th * r.n;
-    r.tile = th;
     const int chunk = th % nc;
     r.h = (th / nc) % a.H;
     r.tok0 = th / (nc * a.H);
@@ -141,7 +158,7 @@ MOET_DEVICE Unit find_unit(const AttendArgs& a, const int* pre, int u) {
     r.row0 = chunk * RT;
     r.rows = a.G;
     r.p0 = r.tok0 < pre[lo + 1] ? min(a.seq_lens[lo], a.W * kPage) - pre[lo + 1] + r.tok0 : -1;   // -1: no sequence's
-    r.page = r.x / PU;
+    r.page = r.x - kTileCost;
     return r;
   }
   int lo = 0, hi = a.B;
@@ -160,23 +177,43 @@ MOET_DEVICE Unit find_unit(const AttendArgs& a, const int* pre, int u) {
   r.rows = nq * a.G;
   r.tok0 = c0;
   r.p0 = min(a.seq_lens[lo], a.W * kPage) - nq;
-  r.page = page0 + r.x / PU;
-  r.tile = ((int)((long long)c0 * a.G / RT) + lo + tile) * a.H + r.h;
+  r.page = page0 + r.x - kTileCost;
   return r;
 }
 
+template <int D, int NT> constexpr int part_floats() { return 8 * NT * (D + 2); }
+
+MOET_DEVICE long long out_row(const AttendArgs& a, int h, int row, int tok0) {
+  const int tok = tok0 + (a.sel ? 0 : row / a.G), head = h * a.G + (a.sel ? row : row % a.G);
+  return (long long)tok * a.H * a.G + head;
+}
+// N neighbouring values x of an output row (unnormalised, with the row's sum)
+template <typename T16, int N>
+MOET_DEVICE void store_row(const AttendArgs& a, int h, int row, int tok0, int d, int D, const float (&x)[N], float sum) {
+  const float inv = sum > 0.f ? __fdividef(a.v_mul, sum) : sum;      // 0: nothing was seen; NaN stays
+  uint32_t w[N / 2];
+#pragma unroll
+  for (int k = 0; k < N / 2; k++) w[k] = round2<T16>(x[2 * k] * inv, x[2 * k + 1] * inv);
+  T16* p = (T16*)a.out + out_row(a, h, row, tok0) * D + d;
+  if constexpr (N == 8) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+}
+MOET_DEVICE void store_lse(const AttendArgs& a, int h, int row, int tok0, float m, float sum) {
+  if (a.lse) a.lse[out_row(a, h, row, tok0)] = sum == 0.f ? -INFINITY : (m + __log2f(sum)) * 0.6931471805599453f;
+}
+
 template <int D, int NT, typename T16>
-__global__ void __launch_bounds__(kWarps * 32, 2) kv4_attend_kernel(AttendArgs a) {
+__global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, NT>()) kv4_attend_kernel(AttendArgs a) {
   using L = Lay<D>;
-  using C = StepCfg<D>;
+  using C = StepCfg<D, NT>;
   using S = StepSmem<D, NT>;
-  constexpr int RT = S::RT, NSTG = C::kStages, KW = D / 32;
+  constexpr int RT = S::RT, NSLOT = C::kSlots, TS = C::TS, MT = TS / 16, KW = D / 32;
   extern __shared__ __align__(128) uint8_t smem_raw[];
   S& sm = *reinterpret_cast<S*>(smem_raw);
   int* pre = reinterpret_cast<int*>(smem_raw + sizeof(S));            // [B + 1]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   if (lane == 0) {
-    for (int i = 0; i < NSTG; i++) tc::mbar_init(&sm.bar[warp][i], 1);
+    for (int i = 0; i < NSLOT; i++) tc::mbar_init(&sm.bar[warp][i], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   pdl_entry();
@@ -185,7 +222,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attend_kernel(AttendArgs a
   int total;
   if (a.sel) {
     for (int i = tid; i <= a.B; i += kWarps * 32) pre[i] = row_start(a, i);
-    total = a.T * a.H * ((a.G + RT - 1) / RT) * a.budget * C::PU;
+    total = a.T * a.H * ((a.G + RT - 1) / RT) * (a.budget + kTileCost);
   } else {
     int run = 0;
     for (int b0 = 0; b0 < a.B; b0 += kWarps * 32) {
@@ -216,6 +253,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attend_kernel(AttendArgs a
   __syncthreads();
   const int per = max((int)(((long long)total + gridDim.x - 1) / gridDim.x), a.min_units);
   const int u0 = (int)min((long long)blockIdx.x * per, (long long)total), u1 = min(u0 + per, total);
+  int* split = a.split + blockIdx.x * kSplitInts;
+  if (tid == 0) split[0] = 0;
   if (u0 >= u1) return;
 
   // ---- this warp's units u0 + warp + 4 i through its ring
@@ -224,9 +263,11 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attend_kernel(AttendArgs a
   int my_start = -1;
   uint32_t phase = 0;
   bool dead = false;
-  auto issue = [&](int i) {
+  int next = 0, next_slot = 0;           // the half to be issued (keys of unit next / 2, or its values) and its slot
+  auto issue = [&]() {
+    const int i = next >> 1;
     if (i >= mine) return;
-    if ((i & 31) == 0) {                 // look up the next 32 units, one per lane
+    if ((next & 63) == 0) {              // look up the next 32 units, one per lane
       my_start = -1;
       if (i + lane < mine) {
         const Unit r = find_unit<D, NT>(a, pre, u0 + warp + kWarps * (i + lane));
@@ -234,35 +275,49 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attend_kernel(AttendArgs a
         bool bad = false;
         const int row_last = min(r.row0 + RT, r.rows) - 1;
         const int p_last = r.p0 + (a.sel ? 0 : row_last / a.G);        // the tile's last position
-        if (a.sel) page = a.sel[((long long)r.tok0 * a.H + r.h) * a.budget + page];
-        const int st = page * kPage + (r.x % C::PU) * C::UT;
-        if (page >= 0 && page < a.W && st <= p_last) {
+        const bool real = r.x >= kTileCost;
+        if (a.sel && real) page = a.sel[((long long)r.tok0 * a.H + r.h) * a.budget + page];
+        if (real && page >= 0 && page < a.W && page * kPage <= p_last) {
           const int phys = a.table[(long long)r.b * a.W + page];
           bad = phys < 0 || phys >= a.n_pages;
           if (!bad) {
-            my_start = st;
-            my_src = a.pages + ((long long)phys * a.H + r.h) * L::kPageBytes + (r.x % C::PU) * C::kUnitBytes;
+            my_start = page * kPage;
+            my_src = a.pages + ((long long)phys * a.H + r.h) * L::kPageBytes;
           }
         } else {
-          bad = page >= a.W;
+          bad = real && page >= a.W;
         }
         if (bad) set_status(a.status, kBadIndex);
       }
     }
-    const int st = i % NSTG;
     if (lane == (i & 31)) {
-      sm.start[warp][st] = dead ? -1 : my_start;
-      if (my_start >= 0 && !dead) bulk_load(sm.ring[warp][st], my_src, C::kUnitBytes, &sm.bar[warp][st]);
+      sm.start[warp][next_slot] = dead ? -1 : my_start;
+      if (my_start >= 0 && !dead)
+        bulk_load(sm.ring[warp][next_slot], my_src + (next & 1) * L::kHalfBytes, L::kHalfBytes, &sm.bar[warp][next_slot]);
     }
+    next++;
+    next_slot = next_slot + 1 == NSLOT ? 0 : next_slot + 1;
     __syncwarp();
   };
 #pragma unroll 1
-  for (int i = 0; i < NSTG; i++) issue(i);
+  for (int k = 0; k < NSLOT; k++) issue();
+  int slot = 0;                          // the half that comes next
+  auto arrived = [&](int k) {            // wait for slot k; false: the copy did not come in time
+    if (dead) return;
+    if (!tc::mbar_wait(&sm.bar[warp][k], (phase >> k) & 1)) {
+      set_status(a.status, kTimeout);
+      dead = true;
+    }
+    phase ^= 1u << k;
+  };
 
   int i = 0;                             // next own unit
   for (int cur = u0; cur < u1;) {
     const Unit tl = find_unit<D, NT>(a, pre, cur);
-    const int first = cur - tl.x, seg_end = min(u1, first + tl.n);     // tile = [first, first + n)
+    const int first = cur - tl.x + kTileCost, end = cur - tl.x + tl.n, seg_end = min(u1, end);   // pages: [first, end)
+    if (seg_end <= first) {                                            // the tile begins in the next block
+      break;
+    }
 
     // ---- queries: B fragments of rows n * 8 + g, positions of accumulator columns n * 8 + 2 t, + 1
     uint32_t qf[NT][KW][2][2];
@@ -321,32 +376,27 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attend_kernel(AttendArgs a
     }
 
     for (; u0 + warp + kWarps * i < seg_end; i++) {
-      const int st = i % NSTG, start = sm.start[warp][st];
-      if (start >= 0 && !dead) {
-        if (!tc::mbar_wait(&sm.bar[warp][st], (phase >> st) & 1)) {
-          set_status(a.status, kTimeout);
-          dead = true;
-        }
-        phase ^= 1u << st;
-      }
-      if (start >= 0 && !dead) {
+      const int ks = slot, vs_ = ks + 1 == NSLOT ? 0 : ks + 1, start = sm.start[warp][ks];
+      slot = vs_ + 1 == NSLOT ? 0 : vs_ + 1;
+      if (start >= 0) arrived(ks);
+      const uint8_t *keys = sm.ring[warp][ks], *values = sm.ring[warp][vs_];
 #pragma unroll 1
-        for (int sb = 0; sb < C::UT / kSub; sb++) {
-          const uint8_t* sub = sm.ring[warp][st] + sb * L::kSubBytes;
-          const int s0 = start + sb * kSub;
-          // S^T: two tiles of 16 tokens
-          float s[2][NT][4];
+      for (int st = 0; st < kPage / TS; st++) {
+        const int s0 = start + st * TS;
+        if (start >= 0 && !dead) {
+          // S^T: tiles of 16 tokens
+          float s[MT][NT][4];
 #pragma unroll
-          for (int mt = 0; mt < 2; mt++) {
+          for (int mt = 0; mt < MT; mt++) {
 #pragma unroll
             for (int n = 0; n < NT; n++) s[mt][n][0] = s[mt][n][1] = s[mt][n][2] = s[mt][n][3] = 0.f;
-            const int j0 = mt * 16 + g, j1 = j0 + 8;
+            const int j0 = st * TS + mt * 16 + g, j1 = j0 + 8;
 #pragma unroll
             for (int sl = 0; sl < L::NS; sl++) {
               constexpr int W = L::SD / 32;
               uint32_t c0[W], c1[W], f0[W], f1[W];
-              const uint8_t* kc = sub + L::KC + sl * (kSub * L::SD / 2) + t * (L::SD / 8);
-              const uint8_t* ks = sub + L::KS + sl * (L::SD / 16);
+              const uint8_t* kc = keys + L::KC + sl * L::kSlabBytes + t * (L::SD / 8);
+              const uint8_t* ks = keys + L::KS + sl * (L::SD / 16);
               if (W == 4) {
                 const uint4 x = *reinterpret_cast<const uint4*>(kc + j0 * (L::SD / 2));
                 const uint4 y = *reinterpret_cast<const uint4*>(kc + j1 * (L::SD / 2));
@@ -381,24 +431,30 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attend_kernel(AttendArgs a
               }
             }
           }
-          // online softmax over the 32 tokens, in powers of two
-          const bool edge = s0 + kSub - 1 > p_first || (a.window > 0 && s0 <= p_last - a.window);
-          uint32_t pf[2][NT][2];
+          // online softmax over the step's tokens, in powers of two
+          const bool edge = s0 + TS - 1 > p_first || (a.window > 0 && s0 <= p_last - a.window);
+          uint32_t pf[MT][NT][2];
 #pragma unroll
           for (int n = 0; n < NT; n++) {
             float mx[2] = {m[n][0], m[n][1]};
 #pragma unroll
-            for (int mt = 0; mt < 2; mt++)
+            for (int mt = 0; mt < MT; mt++) {
+              mul2(s[mt][n][0], s[mt][n][1], cs[n][0], cs[n][1]);
+              mul2(s[mt][n][2], s[mt][n][3], cs[n][0], cs[n][1]);
+            }
+            if (edge) {
 #pragma unroll
-              for (int k = 0; k < 4; k++) {
-                float x = s[mt][n][k] * cs[n][k & 1];
-                if (edge) {
+              for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
                   const int j = s0 + mt * 16 + g + (k >> 1) * 8, p = pc[n][k & 1];
-                  if (j > p || (a.window > 0 && j <= p - a.window)) x = -INFINITY;
+                  if (j > p || (a.window > 0 && j <= p - a.window)) s[mt][n][k] = -INFINITY;
                 }
-                s[mt][n][k] = x;
-                mx[k & 1] = fmaxf(mx[k & 1], x);
-              }
+            }
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+              for (int k = 0; k < 4; k++) mx[k & 1] = fmaxf(mx[k & 1], s[mt][n][k]);
 #pragma unroll
             for (int c = 0; c < 2; c++) {
 #pragma unroll
@@ -409,34 +465,41 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attend_kernel(AttendArgs a
               const float a0 = fast_exp2(m[n][0] - ref0), a1 = fast_exp2(m[n][1] - ref1);
               l[n][0] *= a0, l[n][1] *= a1;
 #pragma unroll
-              for (int d = 0; d < D / 16; d++) o[d][n][0] *= a0, o[d][n][1] *= a1, o[d][n][2] *= a0, o[d][n][3] *= a1;
+              for (int d = 0; d < D / 16; d++) mul2(o[d][n][0], o[d][n][1], a0, a1), mul2(o[d][n][2], o[d][n][3], a0, a1);
               m[n][0] = mx[0], m[n][1] = mx[1];
             }
 #pragma unroll
-            for (int mt = 0; mt < 2; mt++) {
-              float p[4];
+            for (int mt = 0; mt < MT; mt++) {
+              float (&p)[4] = s[mt][n];
+              sub2(p[0], p[1], ref0, ref1);
+              sub2(p[2], p[3], ref0, ref1);
 #pragma unroll
-              for (int k = 0; k < 4; k++) p[k] = fast_exp2(s[mt][n][k] - ((k & 1) ? ref1 : ref0));
+              for (int k = 0; k < 4; k++) p[k] = fast_exp2(p[k]);
               l[n][0] += p[0] + p[2], l[n][1] += p[1] + p[3];
               pf[mt][n][0] = transpose_8x8(pack_f16x2(p[0], p[1]));
               pf[mt][n][1] = transpose_8x8(pack_f16x2(p[2], p[3]));
             }
           }
+          if (st == kPage / TS - 1) {
+            __syncwarp();           // every lane has read the keys
+            issue();
+          }
+          if (st == 0) arrived(vs_);
           // O^T += V^T P^T
 #pragma unroll
-          for (int mt = 0; mt < 2; mt++) {
-            const int pa = mt * 8 + t, pb = pa + 4;                 // token pairs 2 pa, 2 pa + 1 and 2 pb, 2 pb + 1
+          for (int mt = 0; mt < MT; mt++) {
+            const int pa = st * (TS / 2) + mt * 8 + t, pb = pa + 4;                 // token pairs 2 pa, 2 pa + 1 and 2 pb, 2 pb + 1
             uint32_t keep_a = 0xFFFFFFFFu, keep_b = 0xFFFFFFFFu;
             if (edge) {      // what lies past the rows may be anything: its scales (NaN, maybe) are put to 0
-              keep_a = (s0 + 2 * pa <= p_last ? 0xFFFFu : 0u) | (s0 + 2 * pa + 1 <= p_last ? 0xFFFF0000u : 0u);
-              keep_b = (s0 + 2 * pb <= p_last ? 0xFFFFu : 0u) | (s0 + 2 * pb + 1 <= p_last ? 0xFFFF0000u : 0u);
+              keep_a = (start + 2 * pa <= p_last ? 0xFFFFu : 0u) | (start + 2 * pa + 1 <= p_last ? 0xFFFF0000u : 0u);
+              keep_b = (start + 2 * pb <= p_last ? 0xFFFFu : 0u) | (start + 2 * pb + 1 <= p_last ? 0xFFFF0000u : 0u);
             }
 #pragma unroll
             for (int sl = 0; sl < L::NS; sl++) {
               constexpr int PB = L::SD / 16, W = PB / 4;            // words per token and piece
               uint32_t xa[2][W], xb[2][W], sa[PB], sb2[PB];
-              const uint8_t* vc = sub + L::VC + sl * (kSub * L::SD / 2) + g * (2 * PB);
-              const uint8_t* vs = sub + L::VS + sl * (2 * PB);
+              const uint8_t* vc = values + sl * L::kSlabBytes + g * (2 * PB);
+              const uint8_t* vs = values + (L::VS - L::VC) + sl * (2 * PB);
               if (W == 2) {
                 const uint4 x = *reinterpret_cast<const uint4*>(vc + pa * (16 * PB));
                 const uint4 y = *reinterpret_cast<const uint4*>(vc + pb * (16 * PB));
@@ -479,6 +542,11 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attend_kernel(AttendArgs a
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                   const int blk = 4 * w + k;
+                  if constexpr (NT == 1) {      // the scales go to the smaller side
+                    mma_f16_16816(o[sl * PB + blk][0], va[k], va8[k], vb[k], vb8[k], mul_f16x2(pf[mt][0][0], sa[blk]),
+                                  mul_f16x2(pf[mt][0][1], sb2[blk]));
+                    continue;
+                  }
                   const uint32_t f0 = mul_f16x2(va[k], sa[blk]), f1 = mul_f16x2(va8[k], sa[blk]);
                   const uint32_t f2 = mul_f16x2(vb[k], sb2[blk]), f3 = mul_f16x2(vb8[k], sb2[blk]);
 #pragma unroll
@@ -488,10 +556,12 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attend_kernel(AttendArgs a
               }
             }
           }
+        } else if (st == kPage / TS - 1) {
+          issue();
         }
       }
-      __syncwarp();                 // every lane has read the stage
-      issue(i + NSTG);
+      __syncwarp();                 // every lane has read the values
+      issue();
     }
 
     // ---- join the four warps, in warp order
@@ -520,98 +590,107 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attend_kernel(AttendArgs a
         f[n][c] = fast_exp2(m[n][c] - ref);
         if (warp == 0 && g == 0) sm.fm[r] = M, sm.fl[r] = sum;
       }
-    for (int w = 0; w < kWarps; w++) {
-      if (warp == w) {
+#pragma unroll
+    for (int round = 0; round < 2; round++) {
+      if (warp >> 1 == round) {
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
           for (int d = 0; d < D / 16; d++)
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-              float* p = &sm.red[(n * 8 + 2 * t + (k & 1)) * S::kRedStride + d * 16 + g + (k >> 1) * 8];
+              float* p = &sm.red[warp & 1][(n * 8 + 2 * t + (k & 1)) * S::kRedStride + d * 16 + g + (k >> 1) * 8];
               const float x = o[d][n][k] * f[n][k & 1];
-              *p = w ? *p + x : x;
+              *p = round ? *p + x : x;
             }
       }
       __syncthreads();
     }
 
-    // ---- a whole tile is finished here; a shared one by the last block that arrives
-    bool final = seg_end - cur == tl.n;
-    constexpr int kPart = RT * (D + 2);
-    if (!final) {
-      float* pt = a.part + ((long long)blockIdx.x * 2 + (first >= u0 ? 1 : 0)) * kPart;
+    // ---- a whole tile is finished here; of a shared one the block leaves its part
+    if (first >= u0 && seg_end == end) {
+      for (int e = tid; e < RT * D / 8; e += kWarps * 32) {
+        const int r = e / (D / 8), d = e % (D / 8) * 8;
+        float x[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) x[k] = sm.red[0][r * S::kRedStride + d + k] + sm.red[1][r * S::kRedStride + d + k];
+        if (tl.row0 + r < tl.rows) store_row<T16, 8>(a, tl.h, tl.row0 + r, tl.tok0, d, D, x, sm.fl[r]);
+      }
+      if (tid < RT && tl.row0 + tid < tl.rows) store_lse(a, tl.h, tl.row0 + tid, tl.tok0, sm.fm[tid], sm.fl[tid]);
+    } else {
+      float* pt = a.part + ((long long)blockIdx.x * 2 + (first >= u0 ? 1 : 0)) * part_floats<D, NT>();
       for (int e = tid; e < RT * D / 4; e += kWarps * 32) {
         const int r = e / (D / 4), d = e % (D / 4) * 4;
-        __stcg(reinterpret_cast<float4*>(pt + r * D + d), *reinterpret_cast<const float4*>(&sm.red[r * S::kRedStride + d]));
+        const float4 x = *reinterpret_cast<const float4*>(&sm.red[0][r * S::kRedStride + d]);
+        const float4 y = *reinterpret_cast<const float4*>(&sm.red[1][r * S::kRedStride + d]);
+        *reinterpret_cast<float4*>(pt + r * D + d) = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
       }
       if (tid < RT) {
-        __stcg(pt + RT * D + tid, sm.fm[tid]);
-        __stcg(pt + RT * D + RT + tid, sm.fl[tid]);
+        pt[RT * D + tid] = sm.fm[tid];
+        pt[RT * D + RT + tid] = sm.fl[tid];
       }
-      __threadfence();
-      __syncthreads();
-      const int c0 = first / per, c1 = (first + tl.n - 1) / per;
-      if (tid == 0) {
-        const int was = atomicAdd(&a.counters[tl.tile], 1);
-        sm.last = was == c1 - c0;
-        if (sm.last) a.counters[tl.tile] = 0;
-      }
-      __syncthreads();
-      if (sm.last) {
-        __threadfence();
-        auto at = [&](int c) { return a.part + ((long long)c * 2 + (first >= c * per ? 1 : 0)) * kPart; };
-        if (tid < RT) {
-          float M = -INFINITY, sum = 0.f;
-          for (int c = c0; c <= c1; c++) M = fmaxf(M, __ldcg(at(c) + RT * D + tid));
-          const float ref = M == -INFINITY ? 0.f : M;
-          for (int c = c0; c <= c1; c++)
-            sum += __ldcg(at(c) + RT * D + RT + tid) * fast_exp2(__ldcg(at(c) + RT * D + tid) - ref);
-          sm.fm[tid] = M;
-          sm.fl[tid] = sum;
-        }
-        __syncthreads();
-        for (int e = tid; e < RT * D / 4; e += kWarps * 32) {
-          const int r = e / (D / 4), d = e % (D / 4) * 4;
-          const float ref = sm.fm[r] == -INFINITY ? 0.f : sm.fm[r];
-          float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (int c = c0; c <= c1; c++) {
-            const float* p = at(c);
-            const float w = fast_exp2(__ldcg(p + RT * D + r) - ref);
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(p + r * D + d));
-            sum.x += w * x.x, sum.y += w * x.y, sum.z += w * x.z, sum.w += w * x.w;
-          }
-          *reinterpret_cast<float4*>(&sm.red[r * S::kRedStride + d]) = sum;
-        }
-        __syncthreads();
-        final = true;
-      }
-    }
-    if (final) {
-      for (int e = tid; e < RT * D / 8; e += kWarps * 32) {
-        const int r = e / (D / 8), d = e % (D / 8) * 8, row = tl.row0 + r;
-        if (row < tl.rows) {
-          const int tok = tl.tok0 + (a.sel ? 0 : row / a.G), head = tl.h * a.G + (a.sel ? row : row % a.G);
-          const float inv = sm.fl[r] > 0.f ? __fdividef(a.v_mul, sm.fl[r]) : (sm.fl[r] == 0.f ? 0.f : sm.fl[r]);
-          const float* x = &sm.red[r * S::kRedStride + d];
-          *reinterpret_cast<uint4*>((T16*)a.out + ((long long)tok * a.H * a.G + head) * D + d) =
-              make_uint4(round2<T16>(x[0] * inv, x[1] * inv), round2<T16>(x[2] * inv, x[3] * inv),
-                         round2<T16>(x[4] * inv, x[5] * inv), round2<T16>(x[6] * inv, x[7] * inv));
-        }
-      }
-      if (a.lse && tid < RT && tl.row0 + tid < tl.rows) {
-        const int row = tl.row0 + tid;
-        const int tok = tl.tok0 + (a.sel ? 0 : row / a.G), head = tl.h * a.G + (a.sel ? row : row % a.G);
-        a.lse[(long long)tok * a.H * a.G + head] =
-            sm.fl[tid] == 0.f ? -INFINITY : (sm.fm[tid] + __log2f(sm.fl[tid])) * 0.6931471805599453f;
+      if (tid == 0 && first >= u0) {          // it begins here: the join of block blockIdx.x
+        split[0] = (end - 1) / per - (int)blockIdx.x + 1;
+        split[1] = tl.h, split[2] = tl.row0, split[3] = tl.rows, split[4] = tl.tok0;
       }
     }
     __syncthreads();
     cur = seg_end;
   }
   if (dead) {        // copies that are still in flight must not outlive the block's shared memory
-    for (int k = 0; k < NSTG; k++) tc::mbar_wait(&sm.bar[warp][k], (phase >> k) & 1);
+    for (int k = 0; k < NSLOT; k++) tc::mbar_wait(&sm.bar[warp][k], (phase >> k) & 1);
   }
+}
+
+// Joins the tile that begins in block blockIdx.x and goes on: 32 columns per block, the parts
+// shared out over groups of threads.
+template <int D, int NT, typename T16>
+__global__ void __launch_bounds__(256) kv4_join_kernel(AttendArgs a) {
+  constexpr int RT = 8 * NT, ITEMS = RT * 8, GROUPS = 256 / ITEMS, PF = part_floats<D, NT>();
+  __shared__ float fm[RT], fl[RT];
+  __shared__ float4 sum[GROUPS][ITEMS];
+  pdl_entry();
+  const int c0 = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int* split = a.split + c0 * kSplitInts;
+  const int parts = split[0];
+  if (parts == 0) return;
+  const int h = split[1], row0 = split[2], rows = split[3], tok0 = split[4];
+  // part p: the tail of block c0's stretch, then the head of each next block's
+  auto at = [&](int p) { return a.part + ((long long)(c0 + p) * 2 + (p == 0 ? 1 : 0)) * PF; };
+  for (int r = warp; r < RT; r += 8) {
+    float M = -INFINITY, l = 0.f;
+    for (int p = lane; p < parts; p += 32) {
+      const float* x = at(p) + RT * D + r;
+      const float m = __ldcg(x), s = __ldcg(x + RT), hi = fmaxf(M, m);
+      if (hi != -INFINITY) l = l * fast_exp2(M - hi) + s * fast_exp2(m - hi);
+      else l += s;                              // 0, or NaN from a row that has one
+      M = hi;
+    }
+    const float top = warp_max(M);
+    l = warp_sum(l * (top == -INFINITY ? 1.f : fast_exp2(M - top)));
+    if (lane == 0) fm[r] = top, fl[r] = l;
+  }
+  __syncthreads();
+  const int it = tid % ITEMS, grp = tid / ITEMS, r = it / 8, d = blockIdx.y * 32 + it % 8 * 4;
+  const float ref = fm[r] == -INFINITY ? 0.f : fm[r];
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int p = grp; p < parts; p += GROUPS) {
+    const float w = fast_exp2(__ldcg(at(p) + RT * D + r) - ref);
+    const float4 y = __ldcg(reinterpret_cast<const float4*>(at(p) + r * D + d));
+    x.x += w * y.x, x.y += w * y.y, x.z += w * y.z, x.w += w * y.w;
+  }
+  sum[grp][it] = x;
+  __syncthreads();
+  if (grp || row0 + r >= rows) return;
+#pragma unroll
+  for (int k = 1; k < GROUPS; k++) {
+    const float4 y = sum[k][it];
+    x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+  }
+  const float v[4] = {x.x, x.y, x.z, x.w};
+  store_row<T16, 4>(a, h, row0 + r, tok0, d, D, v, fl[r]);
+  if (blockIdx.y == 0 && it % 8 == 0) store_lse(a, h, row0 + r, tok0, fm[r], fl[r]);
 }
 
 static int sm_count() {
@@ -633,19 +712,16 @@ static int row_tiles(int64_t rows, int D) { return rows <= 8 ? 1 : (rows <= 16 |
 using namespace moet;
 using namespace moet::kv4;
 
-// (floats of `part`, ints of `counters`) that kv4_attend needs; counters start as zeros and are
-// left as zeros.
-std::tuple<int64_t, int64_t> kv4_attend_workspace(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t max_q,
-                                                  bool chosen) {
-  const int64_t rt = 8 * row_tiles(chosen ? G : max_q * G, (int)D);
-  const int64_t tiles = chosen ? T * H * ((G + rt - 1) / rt) : (T * G / rt + B + 1) * H;
-  return {(int64_t)sm_count() * kMaxBlocks * 2 * rt * (D + 2), tiles};
+// floats of `part` and ints of `split` that kv4_attend needs (their contents do not matter)
+std::tuple<int64_t, int64_t> kv4_attend_workspace(int64_t G, int64_t D, int64_t max_q, bool chosen) {
+  const int64_t rt = 8 * row_tiles(chosen ? G : max_q * G, (int)D), blocks = (int64_t)sm_count() * kMaxBlocks;
+  return {blocks * 2 * rt * (D + 2), blocks * kSplitInts};
 }
 
 void kv4_attend(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_lens, torch::Tensor table, torch::Tensor pages,
                 c10::optional<torch::Tensor> sel, double scale, int64_t max_q, int64_t window, int64_t k_exp,
                 int64_t v_exp, torch::Tensor out, c10::optional<torch::Tensor> lse, torch::Tensor part,
-                torch::Tensor counters, torch::Tensor status) {
+                torch::Tensor split, torch::Tensor status) {
   const int T = (int)q.size(0), H = (int)pages.size(1), D = (int)(pages.size(2) / 72), G = (int)(q.size(1) / H);
   const int B = (int)seq_lens.size(0), W = (int)table.size(1);
   const bool chosen = sel.has_value() && sel->defined();
@@ -662,22 +738,23 @@ void kv4_attend(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_lens, tor
   a.scale_log2 = (float)(scale * 1.4426950408889634 * std::ldexp(1.0, (int)k_exp));
   a.v_mul = std::ldexp(1.f, (int)v_exp);
   a.out = out.data_ptr(); a.lse = (float*)opt_ptr(lse);
-  a.part = (float*)part.data_ptr(); a.counters = (int*)counters.data_ptr();
-  a.min_units = kWarps;
+  a.part = (float*)part.data_ptr(); a.split = (int*)split.data_ptr();
+  a.min_units = kWarps + kTileCost;
   a.status = (int*)status.data_ptr();
   if (T == 0 || B == 0) return;
   // the unit line is counted in 32 bits
-  const int64_t line = chosen ? (int64_t)T * H * ((G + 8 * nt - 1) / (8 * nt)) * a.budget * 2
-                              : ((int64_t)T * G / (8 * nt) + B) * H * W * 2;
+  const int64_t line = chosen ? (int64_t)T * H * ((G + 8 * nt - 1) / (8 * nt)) * (a.budget + kTileCost)
+                              : ((int64_t)T * G / (8 * nt) + B) * H * (W + kTileCost);
   TORCH_CHECK(line < (int64_t)1 << 31, "kv4_attend: too much work for one call (", line, " units)");
   auto stream = at::cuda::getCurrentCUDAStream();
   auto go = [&](auto dim, auto n, auto t) {
     constexpr int DD = decltype(dim)::value, NT = decltype(n)::value;
     using T16 = decltype(t);
     const size_t smem = sizeof(StepSmem<DD, NT>) + (B + 1) * sizeof(int);
-    const int blocks = std::max(1, std::min(2, (int)(227 * 1024 / (smem + 1024))));
+    const int blocks = std::max(1, std::min(blocks_per_sm<DD, NT>(), (int)(227 * 1024 / (smem + 1024))));
     moet_allow_max_smem(kv4_attend_kernel<DD, NT, T16>);
     launch_k(kv4_attend_kernel<DD, NT, T16>, dim3(sm_count() * blocks), dim3(kWarps * 32), smem, stream, a);
+    launch_k(kv4_join_kernel<DD, NT, T16>, dim3(sm_count() * blocks, DD / 32), dim3(256), 0, stream, a);
   };
   auto by_type = [&](auto dim, auto n) {
     if (q.scalar_type() == at::kHalf) go(dim, n, __half{});

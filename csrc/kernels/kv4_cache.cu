@@ -108,8 +108,7 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(AppendArgs a) {
   if (slot >= a.n_slots) set_status(a.status, kBadIndex);
   live = slot >= 0 && slot < a.n_slots;
   const int j = (int)(slot % kPage);                                   // position in its page
-  uint8_t* sub = a.pages + ((slot / kPage) * a.H + h) * (long long)L::kPageBytes + (j / kSub) * L::kSubBytes;
-  const int js = j % kSub;
+  uint8_t* page = a.pages + ((slot / kPage) * a.H + h) * (long long)L::kPageBytes;
   float x[16], s;
 #pragma unroll
   for (int i = 0; i < 16; i++) x[i] = 0.f;
@@ -125,11 +124,11 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(AppendArgs a) {
     other[t] = __shfl_xor_sync(0xffffffffu, word[t], 1);
   }
   if (live) {
-    uint8_t* kc = sub + L::KC + slab * (kSub * L::SD / 2) + js * (L::SD / 2) + (bs >> 1) * 4;
+    uint8_t* kc = page + L::KC + slab * L::kSlabBytes + j * (L::SD / 2) + (bs >> 1) * 4;
     const int t0 = (b & 1) * 2;
     *reinterpret_cast<uint32_t*>(kc + t0 * (L::SD / 8)) = (b & 1) ? other[2] | word[2] << 4 : word[0] | other[0] << 4;
     *reinterpret_cast<uint32_t*>(kc + (t0 + 1) * (L::SD / 8)) = (b & 1) ? other[3] | word[3] << 4 : word[1] | other[1] << 4;
-    sub[L::KS + js * L::NB + b] = (uint8_t)s8;
+    page[L::KS + j * L::NB + b] = (uint8_t)s8;
     // values: byte (g, block) holds values g and g + 8; staged so that a store takes a lane's whole piece
     load16<T16, VEC>((const T16*)a.v.p + tok * a.v.tok + h * a.v.head + b * 16, x);
   }
@@ -141,16 +140,16 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(AppendArgs a) {
   if (live) {
     // this lane's eight bytes of its own row: pieces g of SD / 16 bytes, 8 / (SD / 16) of them
     constexpr int PB = L::SD / 16, PN = 8 / PB;
-    uint8_t* vc = sub + L::VC + (js >> 1) * (PB * 16) + (js & 1) * PB;
+    uint8_t* vc = page + L::VC + (j >> 1) * (PB * 16) + (j & 1) * PB;
 #pragma unroll
     for (int i = 0; i < PN; i++) {
       const int piece = b * PN + i, sl = piece / 8, g = piece % 8;      // of the row's 8 * slabs pieces
       const uint8_t* src = &stage[warp][(lane / L::NB) * (D / 2) + piece * PB];
-      uint8_t* dst = vc + sl * (kSub * L::SD / 2) + g * (2 * PB);
+      uint8_t* dst = vc + sl * L::kSlabBytes + g * (2 * PB);
       if (PB == 8) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(src);
       else *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(src);
     }
-    sub[L::VS + (js >> 1) * (2 * L::NB) + 2 * b + (js & 1)] = (uint8_t)s8;
+    page[L::VS + (j >> 1) * (2 * L::NB) + 2 * b + (j & 1)] = (uint8_t)s8;
   }
   if (bad && live) set_status(a.status, kBadValue);
 }
@@ -189,13 +188,11 @@ __global__ void __launch_bounds__(256) kv4_bounds_kernel(BoundsArgs a) {
     for (int i = 0; i < L::NS * W * 4; i++) (&hi[0][0][0])[i] = ninf, (&lo[0][0][0])[i] = pinf;
 #pragma unroll
     for (int j = lane >> 2; j < kPage; j += 8) {
-      const uint8_t* sub = base + (j / kSub) * L::kSubBytes;
-      const int js = j % kSub;
 #pragma unroll
       for (int sl = 0; sl < L::NS; sl++) {
         uint32_t c[W], s[W];
-        const uint8_t* kc = sub + L::KC + sl * (kSub * L::SD / 2) + js * (L::SD / 2) + t * (L::SD / 8);
-        const uint8_t* ks = sub + L::KS + js * L::NB + sl * (L::SD / 16);
+        const uint8_t* kc = base + L::KC + sl * L::kSlabBytes + j * (L::SD / 2) + t * (L::SD / 8);
+        const uint8_t* ks = base + L::KS + j * L::NB + sl * (L::SD / 16);
         if (W == 4) {
           const uint4 v = *reinterpret_cast<const uint4*>(kc);
           c[0] = v.x, c[1] = v.y, c[W - 2] = v.z, c[W - 1] = v.w;
@@ -285,11 +282,11 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(ReadArgs a) {
 #pragma unroll
   for (int i = 0; i < 16; i++) x[i] = y[i] = 0.f;
   if (live) {
-    const int j = (int)(slot % kPage), js = j % kSub;
-    const uint8_t* sub = a.pages + ((slot / kPage) * a.H + h) * (long long)L::kPageBytes + (j / kSub) * L::kSubBytes;
-    const float ks = e4m3_to_f32(sub[L::KS + js * L::NB + b]) * a.k_mul;
-    const float vs = e4m3_to_f32(sub[L::VS + (js >> 1) * (2 * L::NB) + 2 * b + (js & 1)]) * a.v_mul;
-    const uint8_t* kc = sub + L::KC + slab * (kSub * L::SD / 2) + js * (L::SD / 2) + (bs >> 1) * 4;
+    const int j = (int)(slot % kPage);
+    const uint8_t* page = a.pages + ((slot / kPage) * a.H + h) * (long long)L::kPageBytes;
+    const float ks = e4m3_to_f32(page[L::KS + j * L::NB + b]) * a.k_mul;
+    const float vs = e4m3_to_f32(page[L::VS + (j >> 1) * (2 * L::NB) + 2 * b + (j & 1)]) * a.v_mul;
+    const uint8_t* kc = page + L::KC + slab * L::kSlabBytes + j * (L::SD / 2) + (bs >> 1) * 4;
 #pragma unroll
     for (int t = 0; t < 4; t++) {
       uint32_t r[4];
@@ -301,7 +298,7 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(ReadArgs a) {
       }
     }
     constexpr int PB = L::SD / 16;
-    const uint8_t* vc = sub + L::VC + slab * (kSub * L::SD / 2) + (js >> 1) * (PB * 16) + (js & 1) * PB + bs;
+    const uint8_t* vc = page + L::VC + slab * L::kSlabBytes + (j >> 1) * (PB * 16) + (j & 1) * PB + bs;
 #pragma unroll
     for (int g = 0; g < 8; g += 4) {
       uint32_t r[4];

@@ -34,22 +34,19 @@ HEAD_DIMS = (64, 128, 256)
 _STATUS = {1: "a slot or page out of range", 2: "a wait on the device ran out", 3: "bad size",
            4: "a key or value that is not finite (NaN is held as 0, infinities as the largest value)"}
 
-# part / counters of kv4_attend, by stream: calls on one stream run one after the other
+# parts of split tiles (kv4_attend), by stream: calls on one stream run one after the other
 _workspaces: dict = {}
 
 
 def _workspace(device: torch.device, floats: int, ints: int) -> Tuple[torch.Tensor, torch.Tensor]:
-    if torch.cuda.is_current_stream_capturing():      # a captured graph owns its workspace
-        return (torch.empty(floats, dtype=torch.float32, device=device),
-                torch.zeros(ints, dtype=torch.int32, device=device))
     key = (device.index, torch.cuda.current_stream(device).cuda_stream)
-    part, counters = _workspaces.get(key, (None, None))
+    part, split = _workspaces.get(key, (None, None))
     if part is None or part.numel() < floats:
         part = torch.empty(floats, dtype=torch.float32, device=device)
-    if counters is None or counters.numel() < ints:
-        counters = torch.zeros(max(ints, 4096), dtype=torch.int32, device=device)
-    _workspaces[key] = (part, counters)
-    return part, counters
+        split = torch.empty(ints, dtype=torch.int32, device=device)
+        if not torch.cuda.is_current_stream_capturing():      # a captured graph owns its workspace
+            _workspaces[key] = (part, split)
+    return part, split
 
 
 class KV4Cache:
@@ -179,9 +176,8 @@ class KV4Cache:
         out = torch.empty(T, Hq, self.head_dim, dtype=q.dtype, device=self.device)
         lse = torch.empty(T, Hq, dtype=torch.float32, device=self.device) if return_lse else None
         if T:
-            part, counters = _workspace(self.device, *self._C.kv4_attend_workspace(
-                T, seq_lens.shape[0], self.num_kv_heads, Hq // self.num_kv_heads, self.head_dim, max_q,
-                pages is not None))
+            part, split = _workspace(self.device, *self._C.kv4_attend_workspace(
+                Hq // self.num_kv_heads, self.head_dim, max_q, pages is not None))
             self._C.kv4_attend(q, cu_q, seq_lens, block_table, self.pages, pages, scale, max_q, window, self.k_exp,
-                               self.v_exp, out, lse, part, counters, self.status)
+                               self.v_exp, out, lse, part, split, self.status)
         return (out, lse) if return_lse else out
