@@ -4,16 +4,18 @@
 // values per row), keys first, so that either half is one copy:
 //   [ 0 D, 32 D)  key codes     [slab][64 tokens][piece t < 4][SD / 8 bytes]
 //   [32 D, 36 D)  key scales    [64 tokens][D / 16]           e4m3
-//   [36 D, 68 D)  value codes   [slab][32 token pairs][g < 8][token of the pair][SD / 16 bytes]
+//   [36 D, 68 D)  value codes   [slab][32 token pairs][piece g < 8][token of the pair][SD / 16 bytes]
 //   [68 D, 72 D)  value scales  [32 token pairs][D / 16][token of the pair]   e4m3
-// A slab is SD = min(D, 128) values.  The orders are those in which a warp's m16n8k16
-// fragments want them, so one wide shared-memory load per token gives a lane all that it
-// needs of a row and no two lanes meet in a bank:
-//   key byte (t, 4 w + i)  = value 32 w + 4 t + i (low half), value 32 w + 16 + 4 t + i (high half):
-//       the two halves of a converted f16x2 carry two scales that are neighbours in memory;
-//   value byte (g, block b) = value 16 b + g (low half), value 16 b + 8 + g (high half):
-//       a row's bytes are its own (two tokens never share a byte, so rows can be written in
-//       any order); a lane joins the two tokens of a pair with two ALU operations per word.
+// A slab is SD = min(D, 128) values.  A piece is what one lane of a warp needs of a row in the
+// m16n8k16 fragments (the order of the values within a product's depth, or of its rows, is
+// free), chosen so that it takes few scales:
+//   key piece t:   SD = 128: byte i = value 32 t + i (low half), 32 t + 16 + i (high half): two
+//                  blocks, whose scales are the two halves of one f16x2;
+//                  SD = 64:  byte i = value 16 t + i, 16 t + 8 + i: one block;
+//   value piece g: byte i = value E g + i, E g + E / 2 + i, E = SD / 8 (one block, or half of
+//                  one); a row's bytes are its own (two tokens never share a byte, so rows can be
+//                  written in any order), and a lane joins the two tokens of a pair with two ALU
+//                  operations per word; their scales are one f16x2.
 // An element is e2m1 * scale * 2^exp (exp per cache, for K and V).  e2m1 times e4m3 has at
 // most six significant bits, at most 2688 and is a multiple of 2^-10: exact in f16.
 #pragma once
@@ -41,11 +43,21 @@ MOET_DEVICE void e2m1x8_to_f16(uint32_t w, uint32_t (&r)[4]) {
       "cvt.rn.f16x2.e2m1x2 %2, b2;\ncvt.rn.f16x2.e2m1x2 %3, b3;\n}\n"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(w));
 }
-// four e4m3 bytes -> two f16x2
-MOET_DEVICE void e4m3x4_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  asm("{\n.reg .b16 h0, h1;\nmov.b32 {h0, h1}, %2;\n"
-      "cvt.rn.f16x2.e4m3x2 %0, h0;\ncvt.rn.f16x2.e4m3x2 %1, h1;\n}\n"
-      : "=r"(lo), "=r"(hi) : "r"(w));
+// two e4m3 bytes (the low half of w) -> f16x2
+MOET_DEVICE uint32_t e4m3x2_to_f16(uint16_t w) {
+  uint32_t d;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(d) : "h"(w));
+  return d;
+}
+// 2 or 4 words, from 8- or 16-byte aligned memory
+template <int W> MOET_DEVICE void load_words(const uint8_t* p, uint32_t (&c)[W]) {
+  if constexpr (W == 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    c[0] = v.x, c[1] = v.y, c[2] = v.z, c[3] = v.w;
+  } else {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    c[0] = v.x, c[1] = v.y;
+  }
 }
 // products of f16 pairs keep their subnormals (no .ftz)
 MOET_DEVICE uint32_t mul_f16x2(uint32_t a, uint32_t b) {
@@ -62,6 +74,18 @@ MOET_DEVICE void join_pair(uint32_t a, uint32_t b, uint32_t& g0, uint32_t& g8) {
 template <typename T16> MOET_DEVICE float to_f32(T16 x);
 template <> MOET_DEVICE float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
 template <> MOET_DEVICE float to_f32(__half x) { return __half2float(x); }
+
+// the f16x2 that scales a lane's key codes: `row` = the token's scales, sl the slab, t the piece
+template <int D> MOET_DEVICE uint32_t key_scales(const uint8_t* row, int sl, int t) {
+  if constexpr (Lay<D>::SD == 128) return e4m3x2_to_f16(*reinterpret_cast<const uint16_t*>(row + sl * 8 + 2 * t));
+  const uint32_t b = row[t];
+  return e4m3x2_to_f16((uint16_t)(b | b << 8));
+}
+// the f16x2 (one scale per token of the pair) of a lane's value codes: `row` = the pair's scales
+template <int D> MOET_DEVICE uint32_t value_scales(const uint8_t* row, int sl, int g) {
+  const int b = Lay<D>::SD == 128 ? sl * 8 + g : g >> 1;
+  return e4m3x2_to_f16(*reinterpret_cast<const uint16_t*>(row + 2 * b));
+}
 
 MOET_DEVICE float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }   // -126 <= e <= 127
 

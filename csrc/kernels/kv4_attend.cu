@@ -104,12 +104,12 @@ constexpr int kTileCost = 4;
 // A unit is one page of a tile.  Its keys and its values are two copies, each into a slot of
 // its own; a warp takes TS tokens per softmax step.
 template <int D, int NT> struct StepCfg {
-  static constexpr int kSlots = NT == 1 ? 2 : 3;                                   // 2304, 4608 or 9216 bytes each
+  static constexpr int kSlots = 3;                                   // 2304, 4608 or 9216 bytes each
   static constexpr int TS = NT == 1 ? 64 : 32;                       // as the registers allow
 };
 
 constexpr int kMaxBlocks = 4;       // blocks per SM, at most
-template <int D, int NT> constexpr int blocks_per_sm() { return D <= 128 && NT == 1 ? 4 : 2; }   // by registers
+template <int D, int NT> constexpr int blocks_per_sm() { return D <= 128 && NT == 1 ? 3 : 2; }   // by registers
 
 template <int D, int NT> struct StepSmem {
   using C = StepCfg<D, NT>;
@@ -179,6 +179,13 @@ MOET_DEVICE Unit find_unit(const AttendArgs& a, const int* pre, int u) {
   r.p0 = min(a.seq_lens[lo], a.W * kPage) - nq;
   r.page = page0 + r.x - kTileCost;
   return r;
+}
+
+// where value d of a row lies in the accumulators' order [M tile][half][g]
+template <int D> MOET_DEVICE int column(int d) {
+  constexpr int SD = Lay<D>::SD, E = SD / 8;
+  const int sl = d / SD, g = d % SD / E, half = d % E / (E / 2), i = d % (E / 2);
+  return (sl * (E / 2) + i) * 16 + half * 8 + g;
 }
 
 template <int D, int NT> constexpr int part_floats() { return 8 * NT * (D + 2); }
@@ -329,18 +336,18 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, NT>()) kv4_atten
       const bool live = r < tl.rows;
       const int tok = tl.tok0 + (a.sel ? 0 : r / a.G), head = tl.h * a.G + (a.sel ? r : r % a.G);
       const T16* qp = (const T16*)a.q + (long long)(live ? tok : 0) * a.q_tok + (long long)(live ? head : 0) * a.q_head;
-      float v[KW][8];
+      float v[D / 4];                     // of each slab, piece t's values
       float amax = 0.f;
 #pragma unroll
-      for (int w = 0; w < KW; w++) {
+      for (int x = 0; x < D / 16; x++) {
         // 8-byte loads: the host checks that rows start on 8 bytes
-        const uint2 lo = live ? *reinterpret_cast<const uint2*>(qp + 32 * w + 4 * t) : make_uint2(0, 0);
-        const uint2 hi = live ? *reinterpret_cast<const uint2*>(qp + 32 * w + 16 + 4 * t) : make_uint2(0, 0);
-        const float2 a0 = unpack2<T16>(lo.x), a1 = unpack2<T16>(lo.y), b0 = unpack2<T16>(hi.x), b1 = unpack2<T16>(hi.y);
-        v[w][0] = a0.x, v[w][1] = a0.y, v[w][2] = a1.x, v[w][3] = a1.y;
-        v[w][4] = b0.x, v[w][5] = b0.y, v[w][6] = b1.x, v[w][7] = b1.y;
+        constexpr int PER = L::SD / 16;   // loads per slab
+        const int d = x / PER * L::SD + t * (L::SD / 4) + x % PER * 4;
+        const uint2 y = live ? *reinterpret_cast<const uint2*>(qp + d) : make_uint2(0, 0);
+        const float2 a0 = unpack2<T16>(y.x), a1 = unpack2<T16>(y.y);
+        v[4 * x] = a0.x, v[4 * x + 1] = a0.y, v[4 * x + 2] = a1.x, v[4 * x + 3] = a1.y;
 #pragma unroll
-        for (int k = 0; k < 8; k++) amax = fmaxf(amax, fabsf(v[w][k]));
+        for (int k = 0; k < 4; k++) amax = fmaxf(amax, fabsf(v[4 * x + k]));
       }
       float mul = 1.f, back = 1.f;
       if (sizeof(T16) == 2 && !std::is_same<T16, __half>::value) {
@@ -350,12 +357,13 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, NT>()) kv4_atten
         mul = pow2f(-e), back = pow2f(e);
       }
 #pragma unroll
-      for (int w = 0; w < KW; w++) {
-        qf[n][w][0][0] = pack_f16x2(v[w][0] * mul, v[w][4] * mul);
-        qf[n][w][0][1] = pack_f16x2(v[w][1] * mul, v[w][5] * mul);
-        qf[n][w][1][0] = pack_f16x2(v[w][2] * mul, v[w][6] * mul);
-        qf[n][w][1][1] = pack_f16x2(v[w][3] * mul, v[w][7] * mul);
-      }
+      for (int w = 0; w < KW; w++)
+#pragma unroll
+        for (int k = 0; k < 4; k++) {      // byte k of word w: a code in its low half, one in its high half
+          constexpr int WS = L::SD / 32, HALF = L::SD / 8;
+          const int lo = w / WS * (L::SD / 4) + w % WS * 4 + k;
+          qf[n][w][k >> 1][k & 1] = pack_f16x2(v[lo] * mul, v[lo + HALF] * mul);
+        }
 #pragma unroll
       for (int c = 0; c < 2; c++) {
         cs[n][c] = __shfl_sync(0xffffffffu, back, (2 * t + c) * 4) * a.scale_log2;
@@ -394,34 +402,19 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, NT>()) kv4_atten
 #pragma unroll
             for (int sl = 0; sl < L::NS; sl++) {
               constexpr int W = L::SD / 32;
-              uint32_t c0[W], c1[W], f0[W], f1[W];
+              uint32_t c0[W], c1[W];
               const uint8_t* kc = keys + L::KC + sl * L::kSlabBytes + t * (L::SD / 8);
-              const uint8_t* ks = keys + L::KS + sl * (L::SD / 16);
-              if (W == 4) {
-                const uint4 x = *reinterpret_cast<const uint4*>(kc + j0 * (L::SD / 2));
-                const uint4 y = *reinterpret_cast<const uint4*>(kc + j1 * (L::SD / 2));
-                c0[0] = x.x, c0[1] = x.y, c0[W - 2] = x.z, c0[W - 1] = x.w;
-                c1[0] = y.x, c1[1] = y.y, c1[W - 2] = y.z, c1[W - 1] = y.w;
-                const uint2 p = *reinterpret_cast<const uint2*>(ks + j0 * L::NB);
-                const uint2 q = *reinterpret_cast<const uint2*>(ks + j1 * L::NB);
-                e4m3x4_to_f16(p.x, f0[0], f0[1]);
-                e4m3x4_to_f16(p.y, f0[W - 2], f0[W - 1]);
-                e4m3x4_to_f16(q.x, f1[0], f1[1]);
-                e4m3x4_to_f16(q.y, f1[W - 2], f1[W - 1]);
-              } else {
-                const uint2 x = *reinterpret_cast<const uint2*>(kc + j0 * (L::SD / 2));
-                const uint2 y = *reinterpret_cast<const uint2*>(kc + j1 * (L::SD / 2));
-                c0[0] = x.x, c0[1] = x.y, c1[0] = y.x, c1[1] = y.y;
-                e4m3x4_to_f16(*reinterpret_cast<const uint32_t*>(ks + j0 * L::NB), f0[0], f0[1]);
-                e4m3x4_to_f16(*reinterpret_cast<const uint32_t*>(ks + j1 * L::NB), f1[0], f1[1]);
-              }
+              load_words<W>(kc + j0 * (L::SD / 2), c0);
+              load_words<W>(kc + j1 * (L::SD / 2), c1);
+              const uint32_t f0 = key_scales<D>(keys + L::KS + j0 * L::NB, sl, t);
+              const uint32_t f1 = key_scales<D>(keys + L::KS + j1 * L::NB, sl, t);
 #pragma unroll
               for (int w = 0; w < W; w++) {
                 uint32_t x[4], y[4];
                 e2m1x8_to_f16(c0[w], x);
                 e2m1x8_to_f16(c1[w], y);
 #pragma unroll
-                for (int k = 0; k < 4; k++) x[k] = mul_f16x2(x[k], f0[w]), y[k] = mul_f16x2(y[k], f1[w]);
+                for (int k = 0; k < 4; k++) x[k] = mul_f16x2(x[k], f0), y[k] = mul_f16x2(y[k], f1);
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
                   const uint32_t(&q)[2][2] = qf[n][sl * W + w];
@@ -496,62 +489,30 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, NT>()) kv4_atten
             }
 #pragma unroll
             for (int sl = 0; sl < L::NS; sl++) {
-              constexpr int PB = L::SD / 16, W = PB / 4;            // words per token and piece
-              uint32_t xa[2][W], xb[2][W], sa[PB], sb2[PB];
+              constexpr int PB = L::SD / 16, W = PB / 4;            // bytes and words per token and piece
+              uint32_t xa[2 * W], xb[2 * W];                        // the pair's first token, then its second
               const uint8_t* vc = values + sl * L::kSlabBytes + g * (2 * PB);
-              const uint8_t* vs = values + (L::VS - L::VC) + sl * (2 * PB);
-              if (W == 2) {
-                const uint4 x = *reinterpret_cast<const uint4*>(vc + pa * (16 * PB));
-                const uint4 y = *reinterpret_cast<const uint4*>(vc + pb * (16 * PB));
-                xa[0][0] = x.x, xa[0][W - 1] = x.y, xa[1][0] = x.z, xa[1][W - 1] = x.w;
-                xb[0][0] = y.x, xb[0][W - 1] = y.y, xb[1][0] = y.z, xb[1][W - 1] = y.w;
-                const uint4 p = *reinterpret_cast<const uint4*>(vs + pa * (2 * L::NB));
-                const uint4 q = *reinterpret_cast<const uint4*>(vs + pb * (2 * L::NB));
-                e4m3x4_to_f16(p.x, sa[0], sa[1]);
-                e4m3x4_to_f16(p.y, sa[2], sa[3]);
-                e4m3x4_to_f16(p.z, sa[PB - 4], sa[PB - 3]);
-                e4m3x4_to_f16(p.w, sa[PB - 2], sa[PB - 1]);
-                e4m3x4_to_f16(q.x, sb2[0], sb2[1]);
-                e4m3x4_to_f16(q.y, sb2[2], sb2[3]);
-                e4m3x4_to_f16(q.z, sb2[PB - 4], sb2[PB - 3]);
-                e4m3x4_to_f16(q.w, sb2[PB - 2], sb2[PB - 1]);
-              } else {
-                const uint2 x = *reinterpret_cast<const uint2*>(vc + pa * (16 * PB));
-                const uint2 y = *reinterpret_cast<const uint2*>(vc + pb * (16 * PB));
-                xa[0][0] = x.x, xa[1][0] = x.y, xb[0][0] = y.x, xb[1][0] = y.y;
-                const uint2 p = *reinterpret_cast<const uint2*>(vs + pa * (2 * L::NB));
-                const uint2 q = *reinterpret_cast<const uint2*>(vs + pb * (2 * L::NB));
-                e4m3x4_to_f16(p.x, sa[0], sa[1]);
-                e4m3x4_to_f16(p.y, sa[2], sa[3]);
-                e4m3x4_to_f16(q.x, sb2[0], sb2[1]);
-                e4m3x4_to_f16(q.y, sb2[2], sb2[3]);
-              }
-              if (edge) {
-#pragma unroll
-                for (int k = 0; k < PB; k++) sa[k] &= keep_a, sb2[k] &= keep_b;
-              }
+              load_words<2 * W>(vc + pa * (16 * PB), xa);
+              load_words<2 * W>(vc + pb * (16 * PB), xb);
+              const uint8_t* vs = values + (L::VS - L::VC);
+              const uint32_t fa = value_scales<D>(vs + pa * (2 * L::NB), sl, g) & keep_a;
+              const uint32_t fb = value_scales<D>(vs + pb * (2 * L::NB), sl, g) & keep_b;
 #pragma unroll
               for (int w = 0; w < W; w++) {
                 uint32_t ca, ca8, cb, cb8, va[4], va8[4], vb[4], vb8[4];
-                join_pair(xa[0][w], xa[1][w], ca, ca8);
-                join_pair(xb[0][w], xb[1][w], cb, cb8);
+                join_pair(xa[w], xa[W + w], ca, ca8);
+                join_pair(xb[w], xb[W + w], cb, cb8);
                 e2m1x8_to_f16(ca, va);
                 e2m1x8_to_f16(ca8, va8);
                 e2m1x8_to_f16(cb, vb);
                 e2m1x8_to_f16(cb8, vb8);
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                  const int blk = 4 * w + k;
-                  if constexpr (NT == 1) {      // the scales go to the smaller side
-                    mma_f16_16816(o[sl * PB + blk][0], va[k], va8[k], vb[k], vb8[k], mul_f16x2(pf[mt][0][0], sa[blk]),
-                                  mul_f16x2(pf[mt][0][1], sb2[blk]));
-                    continue;
-                  }
-                  const uint32_t f0 = mul_f16x2(va[k], sa[blk]), f1 = mul_f16x2(va8[k], sa[blk]);
-                  const uint32_t f2 = mul_f16x2(vb[k], sb2[blk]), f3 = mul_f16x2(vb8[k], sb2[blk]);
+                  const uint32_t f0 = mul_f16x2(va[k], fa), f1 = mul_f16x2(va8[k], fa);
+                  const uint32_t f2 = mul_f16x2(vb[k], fb), f3 = mul_f16x2(vb8[k], fb);
 #pragma unroll
                   for (int n = 0; n < NT; n++)
-                    mma_f16_16816(o[sl * PB + blk][n], f0, f1, f2, f3, pf[mt][n][0], pf[mt][n][1]);
+                    mma_f16_16816(o[sl * PB + 4 * w + k][n], f0, f1, f2, f3, pf[mt][n][0], pf[mt][n][1]);
                 }
               }
             }
@@ -599,7 +560,7 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, NT>()) kv4_atten
           for (int d = 0; d < D / 16; d++)
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-              float* p = &sm.red[warp & 1][(n * 8 + 2 * t + (k & 1)) * S::kRedStride + d * 16 + g + (k >> 1) * 8];
+              float* p = &sm.red[warp & 1][(n * 8 + 2 * t + (k & 1)) * S::kRedStride + d * 16 + (k >> 1) * 8 + g];
               const float x = o[d][n][k] * f[n][k & 1];
               *p = round ? *p + x : x;
             }
@@ -613,7 +574,10 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, NT>()) kv4_atten
         const int r = e / (D / 8), d = e % (D / 8) * 8;
         float x[8];
 #pragma unroll
-        for (int k = 0; k < 8; k++) x[k] = sm.red[0][r * S::kRedStride + d + k] + sm.red[1][r * S::kRedStride + d + k];
+        for (int k = 0; k < 8; k++) {
+          const int c = column<D>(d + k);
+          x[k] = sm.red[0][r * S::kRedStride + c] + sm.red[1][r * S::kRedStride + c];
+        }
         if (tl.row0 + r < tl.rows) store_row<T16, 8>(a, tl.h, tl.row0 + r, tl.tok0, d, D, x, sm.fl[r]);
       }
       if (tid < RT && tl.row0 + tid < tl.rows) store_lse(a, tl.h, tl.row0 + tid, tl.tok0, sm.fm[tid], sm.fl[tid]);
@@ -621,9 +585,13 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, NT>()) kv4_atten
       float* pt = a.part + ((long long)blockIdx.x * 2 + (first >= u0 ? 1 : 0)) * part_floats<D, NT>();
       for (int e = tid; e < RT * D / 4; e += kWarps * 32) {
         const int r = e / (D / 4), d = e % (D / 4) * 4;
-        const float4 x = *reinterpret_cast<const float4*>(&sm.red[0][r * S::kRedStride + d]);
-        const float4 y = *reinterpret_cast<const float4*>(&sm.red[1][r * S::kRedStride + d]);
-        *reinterpret_cast<float4*>(pt + r * D + d) = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
+        float x[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const int c = column<D>(d + k);
+          x[k] = sm.red[0][r * S::kRedStride + c] + sm.red[1][r * S::kRedStride + c];
+        }
+        *reinterpret_cast<float4*>(pt + r * D + d) = make_float4(x[0], x[1], x[2], x[3]);
       }
       if (tid < RT) {
         pt[RT * D + tid] = sm.fm[tid];

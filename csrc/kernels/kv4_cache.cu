@@ -48,8 +48,7 @@ MOET_DEVICE void load16(const T16* p, float (&x)[16]) {
   for (int i = 0; i < 16; i++) x[i] = to_f32(h[i]);
 }
 
-// e2m1 codes of 16 values; codes of (values[a], values[b]) are taken as the low and the high
-// half of a byte by pack(); returns the scale byte.
+// The block's scale byte, and its values over the scale (what a code is rounded from) in x.
 MOET_DEVICE uint32_t scale_of(float (&x)[16], float inv_exp, bool& bad, float& s) {
   float amax = 0.f;
   bool odd = false;
@@ -84,10 +83,14 @@ MOET_DEVICE uint32_t scale_of(float (&x)[16], float inv_exp, bool& bad, float& s
   }
   return s8;
 }
-MOET_DEVICE uint32_t code_byte(float lo, float hi) {
+// codes of values a[0..3] in the low halves of a word's bytes, of b[0..3] in the high halves
+MOET_DEVICE uint32_t codes4(const float* a, const float* b) {
   uint32_t r;
-  asm("{\n.reg .b8 b;\n.reg .b8 z;\ncvt.rn.satfinite.e2m1x2.f32 b, %2, %1;\nmov.b32 %0, {b, 0, 0, 0};\n}\n"
-      : "=r"(r) : "f"(lo), "f"(hi));
+  asm("{\n.reg .b8 b0, b1, b2, b3;\n"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %5, %1;\ncvt.rn.satfinite.e2m1x2.f32 b1, %6, %2;\n"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %7, %3;\ncvt.rn.satfinite.e2m1x2.f32 b3, %8, %4;\n"
+      "mov.b32 %0, {b0, b1, b2, b3};\n}\n"
+      : "=r"(r) : "f"(a[0]), "f"(a[1]), "f"(a[2]), "f"(a[3]), "f"(b[0]), "f"(b[1]), "f"(b[2]), "f"(b[3]));
   return r;
 }
 
@@ -97,8 +100,6 @@ template <int D, typename T16, bool VEC>
 __global__ void __launch_bounds__(256) kv4_append_kernel(AppendArgs a) {
   using L = Lay<D>;
   pdl_entry();
-  __shared__ __align__(16) uint8_t stage[8][256];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long idx = (long long)blockIdx.x * 256 + threadIdx.x;
   const long long row = idx / L::NB;
   const int b = (int)(idx % L::NB), bs = b % (L::SD / 16), slab = b / (L::SD / 16);
@@ -109,49 +110,41 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(AppendArgs a) {
   live = slot >= 0 && slot < a.n_slots;
   const int j = (int)(slot % kPage);                                   // position in its page
   uint8_t* page = a.pages + ((slot / kPage) * a.H + h) * (long long)L::kPageBytes;
-  float x[16], s;
+  float x[16], y[16], s;
 #pragma unroll
-  for (int i = 0; i < 16; i++) x[i] = 0.f;
-  // keys: byte (t, 4 w + i) pairs value 4 t + i of blocks 2 w and 2 w + 1, held by neighbours
-  if (live) load16<T16, VEC>((const T16*)a.k.p + tok * a.k.tok + h * a.k.head + b * 16, x);
-  uint32_t s8 = scale_of(x, a.k_inv, bad, s);
-  uint32_t word[4], other[4];
-#pragma unroll
-  for (int t = 0; t < 4; t++) {
-    // the upper code is 0 here: the neighbour's goes there
-    word[t] = code_byte(x[4 * t], 0.f) | code_byte(x[4 * t + 1], 0.f) << 8 | code_byte(x[4 * t + 2], 0.f) << 16 |
-              code_byte(x[4 * t + 3], 0.f) << 24;
-    other[t] = __shfl_xor_sync(0xffffffffu, word[t], 1);
-  }
+  for (int i = 0; i < 16; i++) x[i] = y[i] = 0.f;
   if (live) {
-    uint8_t* kc = page + L::KC + slab * L::kSlabBytes + j * (L::SD / 2) + (bs >> 1) * 4;
-    const int t0 = (b & 1) * 2;
-    *reinterpret_cast<uint32_t*>(kc + t0 * (L::SD / 8)) = (b & 1) ? other[2] | word[2] << 4 : word[0] | other[0] << 4;
-    *reinterpret_cast<uint32_t*>(kc + (t0 + 1) * (L::SD / 8)) = (b & 1) ? other[3] | word[3] << 4 : word[1] | other[1] << 4;
-    page[L::KS + j * L::NB + b] = (uint8_t)s8;
-    // values: byte (g, block) holds values g and g + 8; staged so that a store takes a lane's whole piece
-    load16<T16, VEC>((const T16*)a.v.p + tok * a.v.tok + h * a.v.head + b * 16, x);
+    load16<T16, VEC>((const T16*)a.k.p + tok * a.k.tok + h * a.k.head + b * 16, x);
+    load16<T16, VEC>((const T16*)a.v.p + tok * a.v.tok + h * a.v.head + b * 16, y);
   }
-  s8 = scale_of(x, a.v_inv, bad, s);
-  const int base = (lane / L::NB) * (D / 2) + slab * (L::SD / 2) + bs;
+  const uint32_t k8 = scale_of(x, a.k_inv, bad, s), v8 = scale_of(y, a.v_inv, bad, s);
+  uint8_t* kc = page + L::KC + slab * L::kSlabBytes + j * (L::SD / 2);
+  uint8_t* vc = page + L::VC + slab * L::kSlabBytes + (j >> 1) * L::SD + (j & 1) * (L::SD / 16);
+  if constexpr (L::SD == 128) {
+    // key piece: this block's codes and its neighbour's; each of the two lanes stores one half
+    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+    uint32_t w[4], o[4];
 #pragma unroll
-  for (int g = 0; g < 8; g++) stage[warp][base + g * (L::SD / 16)] = (uint8_t)code_byte(x[g], x[g + 8]);
-  __syncwarp();
-  if (live) {
-    // this lane's eight bytes of its own row: pieces g of SD / 16 bytes, 8 / (SD / 16) of them
-    constexpr int PB = L::SD / 16, PN = 8 / PB;
-    uint8_t* vc = page + L::VC + (j >> 1) * (PB * 16) + (j & 1) * PB;
-#pragma unroll
-    for (int i = 0; i < PN; i++) {
-      const int piece = b * PN + i, sl = piece / 8, g = piece % 8;      // of the row's 8 * slabs pieces
-      const uint8_t* src = &stage[warp][(lane / L::NB) * (D / 2) + piece * PB];
-      uint8_t* dst = vc + sl * L::kSlabBytes + g * (2 * PB);
-      if (PB == 8) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(src);
-      else *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(src);
+    for (int i = 0; i < 4; i++) {
+      w[i] = codes4(x + 4 * i, zero);
+      o[i] = __shfl_xor_sync(0xffffffffu, w[i], 1);
     }
-    page[L::VS + (j >> 1) * (2 * L::NB) + 2 * b + (j & 1)] = (uint8_t)s8;
+    if (live) {
+      const bool odd = b & 1;
+      *reinterpret_cast<uint2*>(kc + bs * 8) = odd ? make_uint2(o[2] | w[2] << 4, o[3] | w[3] << 4)
+                                                   : make_uint2(w[0] | o[0] << 4, w[1] | o[1] << 4);
+      *reinterpret_cast<uint2*>(vc + bs * 16) = make_uint2(codes4(y, y + 8), codes4(y + 4, y + 12));
+    }
+  } else if (live) {
+    *reinterpret_cast<uint2*>(kc + bs * 8) = make_uint2(codes4(x, x + 8), codes4(x + 4, x + 12));
+    *reinterpret_cast<uint32_t*>(vc + (2 * bs) * 8) = codes4(y, y + 4);
+    *reinterpret_cast<uint32_t*>(vc + (2 * bs + 1) * 8) = codes4(y + 8, y + 12);
   }
-  if (bad && live) set_status(a.status, kBadValue);
+  if (live) {
+    page[L::KS + j * L::NB + b] = (uint8_t)k8;
+    page[L::VS + (j >> 1) * (2 * L::NB) + 2 * b + (j & 1)] = (uint8_t)v8;
+    if (bad) set_status(a.status, kBadValue);
+  }
 }
 
 struct BoundsArgs {
@@ -190,27 +183,16 @@ __global__ void __launch_bounds__(256) kv4_bounds_kernel(BoundsArgs a) {
     for (int j = lane >> 2; j < kPage; j += 8) {
 #pragma unroll
       for (int sl = 0; sl < L::NS; sl++) {
-        uint32_t c[W], s[W];
-        const uint8_t* kc = base + L::KC + sl * L::kSlabBytes + j * (L::SD / 2) + t * (L::SD / 8);
-        const uint8_t* ks = base + L::KS + j * L::NB + sl * (L::SD / 16);
-        if (W == 4) {
-          const uint4 v = *reinterpret_cast<const uint4*>(kc);
-          c[0] = v.x, c[1] = v.y, c[W - 2] = v.z, c[W - 1] = v.w;
-          const uint2 q = *reinterpret_cast<const uint2*>(ks);
-          e4m3x4_to_f16(q.x, s[0], s[1]);
-          e4m3x4_to_f16(q.y, s[W - 2], s[W - 1]);
-        } else {
-          const uint2 v = *reinterpret_cast<const uint2*>(kc);
-          c[0] = v.x, c[1] = v.y;
-          e4m3x4_to_f16(*reinterpret_cast<const uint32_t*>(ks), s[0], s[1]);
-        }
+        uint32_t c[W];
+        load_words<W>(base + L::KC + sl * L::kSlabBytes + j * (L::SD / 2) + t * (L::SD / 8), c);
+        const uint32_t s = key_scales<D>(base + L::KS + j * L::NB, sl, t);
 #pragma unroll
         for (int w = 0; w < W; w++) {
           uint32_t r[4];
           e2m1x8_to_f16(c[w], r);
 #pragma unroll
           for (int i = 0; i < 4; i++) {
-            const uint32_t m = mul_f16x2(r[i], s[w]);
+            const uint32_t m = mul_f16x2(r[i], s);
             const __half2 x = *reinterpret_cast<const __half2*>(&m);
             hi[sl][w][i] = __hmax2(hi[sl][w][i], x);
             lo[sl][w][i] = __hmin2(lo[sl][w][i], x);
@@ -249,12 +231,23 @@ __global__ void __launch_bounds__(256) kv4_bounds_kernel(BoundsArgs a) {
               ph |= (uint32_t)(uint8_t)(int8_t)(int)ceilf(x * inv) << (8 * i);
               pl |= (uint32_t)(uint8_t)(int8_t)(int)floorf(y * inv) << (8 * i);
             }
-            const int d = sl * L::SD + 32 * w + 16 * half + 4 * t;
+            const int d = sl * L::SD + (L::SD / 4) * t + (L::SD / 8) * half + 4 * w;
             *reinterpret_cast<uint32_t*>(out + d) = ph;
             *reinterpret_cast<uint32_t*>(out + D + d) = pl;
           }
       if (lane == 0) a.unit[page * a.H + h] = amax > 0.f ? pow2f(ex) * a.k_mul : 1.f;
     }
+  }
+}
+
+// four bytes' low codes and high codes
+MOET_DEVICE void values4(uint32_t w, float* lo, float* hi) {
+  uint32_t r[4];
+  e2m1x8_to_f16(w, r);
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r[i]));
+    lo[i] = f.x, hi[i] = f.y;
   }
 }
 
@@ -286,31 +279,33 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(ReadArgs a) {
     const uint8_t* page = a.pages + ((slot / kPage) * a.H + h) * (long long)L::kPageBytes;
     const float ks = e4m3_to_f32(page[L::KS + j * L::NB + b]) * a.k_mul;
     const float vs = e4m3_to_f32(page[L::VS + (j >> 1) * (2 * L::NB) + 2 * b + (j & 1)]) * a.v_mul;
-    const uint8_t* kc = page + L::KC + slab * L::kSlabBytes + j * (L::SD / 2) + (bs >> 1) * 4;
+    const uint8_t* kc = page + L::KC + slab * L::kSlabBytes + j * (L::SD / 2);
+    const uint8_t* vc = page + L::VC + slab * L::kSlabBytes + (j >> 1) * L::SD + (j & 1) * (L::SD / 16);
+    if constexpr (L::SD == 128) {
+      uint32_t c[4];
+      load_words<4>(kc + (bs >> 1) * 16, c);
 #pragma unroll
-    for (int t = 0; t < 4; t++) {
-      uint32_t r[4];
-      e2m1x8_to_f16(*reinterpret_cast<const uint32_t*>(kc + t * (L::SD / 8)), r);
+      for (int w = 0; w < 4; w++) {      // this block's codes are the low or the high halves
+        float lo[4], hi[4];
+        values4(c[w], lo, hi);
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const __half2 p = *reinterpret_cast<const __half2*>(&r[i]);
-        x[4 * t + i] = ((b & 1) ? __high2float(p) : __low2float(p)) * ks;
+        for (int i = 0; i < 4; i++) x[4 * w + i] = ((b & 1) ? hi[i] : lo[i]) * ks;
       }
-    }
-    constexpr int PB = L::SD / 16;
-    const uint8_t* vc = page + L::VC + slab * L::kSlabBytes + (j >> 1) * (PB * 16) + (j & 1) * PB + bs;
+      load_words<2>(vc + bs * 16, *reinterpret_cast<uint32_t(*)[2]>(c));
+      values4(c[0], y, y + 8);
+      values4(c[1], y + 4, y + 12);
+    } else {
+      uint32_t c[2];
+      load_words<2>(kc + bs * 8, c);
+      values4(c[0], x, x + 8);
+      values4(c[1], x + 4, x + 12);
+      values4(*reinterpret_cast<const uint32_t*>(vc + (2 * bs) * 8), y, y + 4);
+      values4(*reinterpret_cast<const uint32_t*>(vc + (2 * bs + 1) * 8), y + 8, y + 12);
 #pragma unroll
-    for (int g = 0; g < 8; g += 4) {
-      uint32_t r[4];
-      e2m1x8_to_f16(vc[g * 2 * PB] | vc[(g + 1) * 2 * PB] << 8 | vc[(g + 2) * 2 * PB] << 16 |
-                        (uint32_t)vc[(g + 3) * 2 * PB] << 24, r);
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const __half2 p = *reinterpret_cast<const __half2*>(&r[i]);
-        y[g + i] = __low2float(p) * vs;
-        y[g + i + 8] = __high2float(p) * vs;
-      }
+      for (int i = 0; i < 16; i++) x[i] *= ks;
     }
+#pragma unroll
+    for (int i = 0; i < 16; i++) y[i] *= vs;
   }
   uint32_t o[8];
 #pragma unroll
