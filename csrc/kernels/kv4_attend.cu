@@ -99,12 +99,13 @@ struct Unit {
 
 // A tile's queries, join and output take a block as long as about this many of its pages;
 // counted as empty units in front of them, so that many short tiles do not all fall to one block.
-constexpr int kTileCost = 4;
+constexpr int kTileCost = 8;
 
 // A unit is one page of a tile.  Its keys and its values are two copies, each into a slot of
 // its own; a warp takes TS tokens per softmax step.
 template <int D, int NT> struct StepCfg {
-  static constexpr int kSlots = 3;                                   // 2304, 4608 or 9216 bytes each
+  static constexpr int kSlots = D == 256 ? 2 : 3;                    // 2304, 4608 or 9216 bytes each
+  static constexpr int kRed = D == 256 ? 1 : 2;                      // buffers in which the warps are joined
   static constexpr int TS = NT == 1 ? 64 : 32;                       // as the registers allow
 };
 
@@ -116,7 +117,9 @@ template <int D, int NT> struct StepSmem {
   static constexpr int RT = 8 * NT;
   static constexpr int kRedStride = D + 4;                           // rows 4 banks apart: stores of a quad do not meet
   uint8_t ring[kWarps][C::kSlots][Lay<D>::kHalfBytes];
-  float red[2][RT * kRedStride];                                     // warps 0 and 2, warps 1 and 3
+  static constexpr int kQStride = D + 8;
+  __align__(16) uint16_t q[RT * kQStride];                           // the next tile's queries
+  float red[C::kRed][RT * kRedStride];
   float wm[kWarps][RT], wl[kWarps][RT];
   float fm[RT], fl[RT];
   uint64_t bar[kWarps][C::kSlots];
@@ -223,6 +226,8 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, NT>()) kv4_atten
     for (int i = 0; i < NSLOT; i++) tc::mbar_init(&sm.bar[warp][i], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  // what is read first is fetched into L2 while the kernel before still runs (a prefetch uses no value)
+  if (tid == 0) prefetch_l2(a.q), prefetch_l2(a.seq_lens), prefetch_l2(a.cu_q), prefetch_l2(a.table);
   pdl_entry();
 
   // the line of units: prefix sums over the sequences (all pages), or over nothing (chosen pages)
@@ -263,6 +268,20 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, NT>()) kv4_atten
   int* split = a.split + blockIdx.x * kSplitInts;
   if (tid == 0) split[0] = 0;
   if (u0 >= u1) return;
+
+  // ---- queries come by way of shared memory, a tile ahead
+  auto stage_q = [&](const Unit& tl) {
+    for (int e = tid; e < RT * D / 8; e += kWarps * 32) {
+      const int r = e / (D / 8), d = e % (D / 8) * 8, row = tl.row0 + r;
+      const bool live = row < tl.rows;
+      const int tok = tl.tok0 + (a.sel || !live ? 0 : row / a.G), head = tl.h * a.G + (!live ? 0 : a.sel ? row : row % a.G);
+      const T16* src = (const T16*)a.q + (long long)tok * a.q_tok + (long long)head * a.q_head + d;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"      // rows past the tile's: zeros
+                   ::"r"(tc::smem_addr(&sm.q[r * S::kQStride + d])), "l"(src), "r"(live ? 16 : 0) : "memory");
+    }
+  };
+  Unit tl = find_unit<D, NT>(a, pre, u0);
+  stage_q(tl);
 
   // ---- this warp's units u0 + warp + 4 i through its ring
   const int mine = (u1 - u0 - warp + kWarps - 1) / kWarps;
@@ -320,34 +339,33 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, NT>()) kv4_atten
 
   int i = 0;                             // next own unit
   for (int cur = u0; cur < u1;) {
-    const Unit tl = find_unit<D, NT>(a, pre, cur);
     const int first = cur - tl.x + kTileCost, end = cur - tl.x + tl.n, seg_end = min(u1, end);   // pages: [first, end)
-    if (seg_end <= first) {                                            // the tile begins in the next block
-      break;
-    }
+    if (seg_end <= first) break;                                       // the tile begins in the next block
+    Unit after = tl;
+    if (seg_end < u1) after = find_unit<D, NT>(a, pre, seg_end);
 
     // ---- queries: B fragments of rows n * 8 + g, positions of accumulator columns n * 8 + 2 t, + 1
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
     uint32_t qf[NT][KW][2][2];
     float cs[NT][2];
     int pc[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; n++) {
-      const int r = tl.row0 + n * 8 + g;
-      const bool live = r < tl.rows;
-      const int tok = tl.tok0 + (a.sel ? 0 : r / a.G), head = tl.h * a.G + (a.sel ? r : r % a.G);
-      const T16* qp = (const T16*)a.q + (long long)(live ? tok : 0) * a.q_tok + (long long)(live ? head : 0) * a.q_head;
       float v[D / 4];                     // of each slab, piece t's values
       float amax = 0.f;
 #pragma unroll
-      for (int x = 0; x < D / 16; x++) {
-        // 8-byte loads: the host checks that rows start on 8 bytes
-        constexpr int PER = L::SD / 16;   // loads per slab
-        const int d = x / PER * L::SD + t * (L::SD / 4) + x % PER * 4;
-        const uint2 y = live ? *reinterpret_cast<const uint2*>(qp + d) : make_uint2(0, 0);
-        const float2 a0 = unpack2<T16>(y.x), a1 = unpack2<T16>(y.y);
-        v[4 * x] = a0.x, v[4 * x + 1] = a0.y, v[4 * x + 2] = a1.x, v[4 * x + 3] = a1.y;
+      for (int x = 0; x < D / 32; x++) {
+        constexpr int PER = L::SD / 32;   // 16-byte loads per slab
+        const int d = x / PER * L::SD + t * (L::SD / 4) + x % PER * 8;
+        const uint4 y = *reinterpret_cast<const uint4*>(&sm.q[(n * 8 + g) * S::kQStride + d]);
+        const uint32_t w[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-        for (int k = 0; k < 4; k++) amax = fmaxf(amax, fabsf(v[4 * x + k]));
+        for (int k = 0; k < 4; k++) {
+          const float2 f = unpack2<T16>(w[k]);
+          v[8 * x + 2 * k] = f.x, v[8 * x + 2 * k + 1] = f.y;
+          amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+        }
       }
       float mul = 1.f, back = 1.f;
       if (sizeof(T16) == 2 && !std::is_same<T16, __half>::value) {
@@ -371,6 +389,8 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, NT>()) kv4_atten
         pc[n][c] = tl.p0 + (a.sel ? 0 : rc / a.G);
       }
     }
+    __syncthreads();
+    if (seg_end < u1) stage_q(after);
     const int row_last = min(tl.row0 + RT, tl.rows) - 1;
     const int p_first = tl.p0 + (a.sel ? 0 : tl.row0 / a.G), p_last = tl.p0 + (a.sel ? 0 : row_last / a.G);
 
@@ -552,15 +572,15 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, NT>()) kv4_atten
         if (warp == 0 && g == 0) sm.fm[r] = M, sm.fl[r] = sum;
       }
 #pragma unroll
-    for (int round = 0; round < 2; round++) {
-      if (warp >> 1 == round) {
+    for (int round = 0; round < kWarps / C::kRed; round++) {
+      if (warp / C::kRed == round) {
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
           for (int d = 0; d < D / 16; d++)
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-              float* p = &sm.red[warp & 1][(n * 8 + 2 * t + (k & 1)) * S::kRedStride + d * 16 + (k >> 1) * 8 + g];
+              float* p = &sm.red[warp % C::kRed][(n * 8 + 2 * t + (k & 1)) * S::kRedStride + d * 16 + (k >> 1) * 8 + g];
               const float x = o[d][n][k] * f[n][k & 1];
               *p = round ? *p + x : x;
             }
@@ -576,7 +596,8 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, NT>()) kv4_atten
 #pragma unroll
         for (int k = 0; k < 8; k++) {
           const int c = column<D>(d + k);
-          x[k] = sm.red[0][r * S::kRedStride + c] + sm.red[1][r * S::kRedStride + c];
+          x[k] = sm.red[0][r * S::kRedStride + c];
+          if (C::kRed == 2) x[k] += sm.red[C::kRed - 1][r * S::kRedStride + c];
         }
         if (tl.row0 + r < tl.rows) store_row<T16, 8>(a, tl.h, tl.row0 + r, tl.tok0, d, D, x, sm.fl[r]);
       }
@@ -589,7 +610,8 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, NT>()) kv4_atten
 #pragma unroll
         for (int k = 0; k < 4; k++) {
           const int c = column<D>(d + k);
-          x[k] = sm.red[0][r * S::kRedStride + c] + sm.red[1][r * S::kRedStride + c];
+          x[k] = sm.red[0][r * S::kRedStride + c];
+          if (C::kRed == 2) x[k] += sm.red[C::kRed - 1][r * S::kRedStride + c];
         }
         *reinterpret_cast<float4*>(pt + r * D + d) = make_float4(x[0], x[1], x[2], x[3]);
       }
@@ -604,7 +626,9 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, NT>()) kv4_atten
     }
     __syncthreads();
     cur = seg_end;
+    tl = after;
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
   if (dead) {        // copies that are still in flight must not outlive the block's shared memory
     for (int k = 0; k < NSLOT; k++) tc::mbar_wait(&sm.bar[warp][k], (phase >> k) & 1);
   }
@@ -707,7 +731,7 @@ void kv4_attend(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_lens, tor
   a.v_mul = std::ldexp(1.f, (int)v_exp);
   a.out = out.data_ptr(); a.lse = (float*)opt_ptr(lse);
   a.part = (float*)part.data_ptr(); a.split = (int*)split.data_ptr();
-  a.min_units = kWarps + kTileCost;
+  a.min_units = kWarps;
   a.status = (int*)status.data_ptr();
   if (T == 0 || B == 0) return;
   // the unit line is counted in 32 bits

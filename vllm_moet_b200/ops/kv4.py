@@ -101,8 +101,6 @@ class KV4Cache:
         self._need(q.device == self.device and q.dtype in (torch.bfloat16, torch.float16) and q.dim() == 3
                    and q.shape[2] == D and q.stride(2) == 1, f"q must be bf16 or f16 [rows, heads, {D}], inner stride 1")
         self._need(q.shape[1] >= H and q.shape[1] % H == 0, f"q's heads must be a multiple of the {H} K/V heads")
-        self._need(q.stride(0) % 4 == 0 and q.stride(1) % 4 == 0 and q.data_ptr() % 8 == 0,
-                   "q's rows must start on 8 bytes")
         for name, x, n in (("cu_q", cu_q, seq_lens.shape[0] + 1), ("seq_lens", seq_lens, seq_lens.shape[0])):
             self._need(x.device == self.device and x.dtype == torch.int32 and x.dim() == 1 and x.is_contiguous()
                        and x.shape[0] == n, f"{name} must be a contiguous int32 tensor [{n}]")
@@ -173,6 +171,8 @@ class KV4Cache:
             self._need(pages.device == self.device and pages.dtype == torch.int32 and pages.is_contiguous()
                        and pages.dim() == 3 and pages.shape[:2] == (T, self.num_kv_heads) and pages.shape[2] >= 1,
                        f"pages must be a contiguous int32 tensor [{T}, {self.num_kv_heads}, n >= 1]")
+        if q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:      # the kernel copies rows 16 bytes at a time
+            q = q.clone(memory_format=torch.contiguous_format)
         out = torch.empty(T, Hq, self.head_dim, dtype=q.dtype, device=self.device)
         lse = torch.empty(T, Hq, dtype=torch.float32, device=self.device) if return_lse else None
         if T:
