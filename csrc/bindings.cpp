@@ -125,6 +125,10 @@ void kv4_attend(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_lens, tor
 void kv4_select(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_lens, torch::Tensor table, torch::Tensor bounds,
                 torch::Tensor unit, int64_t max_q, int64_t first, int64_t last, torch::Tensor score,
                 torch::Tensor pages, torch::Tensor status);
+// kv4_prompt.cu
+void kv4_prompt(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_lens, torch::Tensor table, torch::Tensor pages,
+                double scale, int64_t max_q, int64_t window, int64_t k_exp, int64_t v_exp, torch::Tensor out,
+                c10::optional<torch::Tensor> lse, torch::Tensor status);
 // hyper_conn.cu
 void hc_mix(torch::Tensor xs, c10::optional<torch::Tensor> upd, c10::optional<torch::Tensor> post,
             c10::optional<torch::Tensor> comb, c10::optional<torch::Tensor> fn, c10::optional<torch::Tensor> part);
@@ -238,6 +242,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("kv4_select", &kv4_select);
   m.def("kv4_attend_workspace", &kv4_attend_workspace);
   m.def("kv4_attend", &kv4_attend);
+  m.def("kv4_prompt", &kv4_prompt);
   m.def("hc_mix", &hc_mix, py::arg("xs"), py::arg("upd") = py::none(), py::arg("post") = py::none(),
         py::arg("comb") = py::none(), py::arg("fn") = py::none(), py::arg("part") = py::none());
   m.def("hc_apply", &hc_apply, py::arg("xs"), py::arg("part"), py::arg("base"), py::arg("scale"), py::arg("eps"),

@@ -1,0 +1,508 @@
+// Attention of many query rows per sequence (prompt chunks) over the 4-bit paged K/V cache, on
+// the tcgen05 tensor cores.  The mathematics and the layout of a batch are kv4_attend.cu's.
+//
+// A block takes two tiles of 128 rows ((token, head of the group) pairs of one K/V head; one
+// tile with D = 256) and walks over blocks of 128 (64) keys.  Per key block and tile
+//   S = Q K^T   f16 x f16 -> f32 in tensor memory,
+//   P = exp2(S c - m), written back over S as f16 (the A operand of the second product),
+//   O += P V    f32 in tensor memory.
+// Roles: four warps convert keys and values from 4 bits into f16 operands in shared memory
+// (exact, kv4.cuh), once for both tiles; four warps per tile hold a row per thread and do the
+// softmax; one thread issues the products, in the order S0 S1 | PV0 S0' | PV1 S1' | ..., so one
+// tile's products run under the other's softmax.
+//
+// The running maximum is only moved when a row's scores exceed it by 2^8 (P <= 256 in f16, sums
+// in f32): O is rescaled a few times per row, not per block.  Operands are
+// in the no-swizzle core-matrix order; the orders of values (depth of S, columns of O) are the
+// ones the cache's pieces give, so every 16-byte store of the conversion is one core-matrix row
+// and a warp's stores fill whole matrices without bank conflicts.
+#include "kv4.cuh"
+#include "tcgen05.cuh"
+#include "torch_glue.h"
+
+namespace moet {
+namespace kv4 {
+
+struct PromptArgs {
+  const void* q; long long q_tok; int q_head;
+  const int *cu_q, *seq_lens, *table; int B, W, T, H, G, window;
+  const uint8_t* pages; int n_pages;
+  float scale_log2, v_mul;
+  void* out; float* lse;
+  int* status;
+};
+
+template <int D> struct PromptCfg {
+  static constexpr int BK = D == 256 ? 64 : 128;            // keys per block
+  static constexpr int TILES = D == 256 ? 1 : 2;            // row tiles per block
+  static constexpr int kSoftWarps = 4 * TILES, kWarps = kSoftWarps + 5;
+  static constexpr int kQBytes = 128 * D * 2, kKBytes = BK * D * 2;   // one operand tile; V's is K's size
+  static constexpr int kOCol = 256;                         // tensor memory: S (and P) of tile t at t * 128, O after them
+};
+
+template <int D> struct PromptSmem {
+  using C = PromptCfg<D>;
+  uint8_t q[C::TILES][C::kQBytes];
+  uint8_t k[2][C::kKBytes];
+  uint8_t v[2][C::kKBytes];
+  float row_scale[C::TILES * 128];
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full;
+  uint32_t tmem;
+};
+
+namespace pr {
+MOET_DEVICE uint32_t idesc_f16(int M, int N) { return 1u << 4 | (uint32_t)(N >> 3) << 17 | (uint32_t)(M >> 4) << 24; }
+MOET_DEVICE void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+MOET_DEVICE void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
+               ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+#define KV4_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
+#define KV4_W8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
+MOET_DEVICE void ld32(uint32_t addr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : KV4_R8(r, 0), KV4_R8(r, 8), KV4_R8(r, 16), KV4_R8(r, 24) : "r"(addr));
+}
+MOET_DEVICE void st32(uint32_t addr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
+      ::KV4_W8(r, 0), KV4_W8(r, 8), KV4_W8(r, 16), KV4_W8(r, 24), "r"(addr) : "memory");
+}
+MOET_DEVICE void st16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
+      ::KV4_W8(r, 0), KV4_W8(r, 8), "r"(addr) : "memory");
+}
+MOET_DEVICE void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+MOET_DEVICE void arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc::smem_addr(bar)) : "memory");
+}
+MOET_DEVICE float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// x * c + b on a pair
+MOET_DEVICE void fma2(float& x, float& y, float c, float b) {
+  asm("{\n.reg .b64 u, v, w;\nmov.b64 u, {%0, %1};\nmov.b64 v, {%2, %2};\nmov.b64 w, {%3, %3};\n"
+      "fma.rn.ftz.f32x2 u, u, v, w;\nmov.b64 {%0, %1}, u;\n}\n" : "+f"(x), "+f"(y) : "f"(c), "f"(b));
+}
+MOET_DEVICE float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+template <typename T16> MOET_DEVICE float2 up2(uint32_t v);
+template <> MOET_DEVICE float2 up2<__half>(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
+template <> MOET_DEVICE float2 up2<__nv_bfloat16>(uint32_t v) {
+  return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u));
+}
+MOET_DEVICE uint32_t f16x2(float a, float b) {
+  __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+template <typename T16> MOET_DEVICE uint32_t down2(float a, float b);
+template <> MOET_DEVICE uint32_t down2<__half>(float a, float b) { return f16x2(a, b); }
+template <> MOET_DEVICE uint32_t down2<__nv_bfloat16>(float a, float b) { return pack_bf16x2(a, b); }
+}  // namespace pr
+
+// scores of keys j0 .. that the row at position p does not see -> -inf
+template <int N> MOET_DEVICE void hide(uint32_t (&u)[N], int j0, int p, int window) {
+#pragma unroll
+  for (int k = 0; k < N; k++)
+    if (j0 + k > p || (window > 0 && j0 + k <= p - window)) u[k] = 0xFF800000u;
+}
+
+template <int D, typename T16>
+__global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kernel(PromptArgs a) {
+  using L = Lay<D>;
+  using C = PromptCfg<D>;
+  constexpr int BK = C::BK, TILES = C::TILES, E2 = L::SD / 8;      // E2: f16 pairs of a key piece
+  constexpr uint32_t kQSbo = 16 * D, kKSbo = 16 * D, kVSbo = 16 * BK;   // bytes from 8 rows to the next 8
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  PromptSmem<D>& sm = *reinterpret_cast<PromptSmem<D>*>(smem_raw);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  pdl_entry();
+
+  const int b = blockIdx.z, h = blockIdx.y;
+  const int c0 = max(0, min(a.cu_q[b], a.T)), nq = max(0, max(0, min(a.cu_q[b + 1], a.T)) - c0);
+  const int rows = nq * a.G, p0 = min(a.seq_lens[b], a.W * kPage) - nq;
+  const int ntiles_seq = (rows + TILES * 128 - 1) / (TILES * 128);
+  const int tile = ntiles_seq - 1 - (int)blockIdx.x;               // the longest stretches of keys first
+  if (tile < 0) return;
+  const int row0 = tile * TILES * 128, live = min(rows - row0, TILES * 128);
+  const int p_first = p0 + row0 / a.G, p_last = p0 + (row0 + live - 1) / a.G;
+  const int ntile = (live + 127) / 128;
+  const int kb0 = a.window > 0 ? max(0, p_first - a.window + 1) / BK : 0;
+  const int kb1 = p_last < 0 ? kb0 : p_last / BK + 1;              // key blocks [kb0, kb1)
+  const int nkb = kb1 - kb0;
+
+  // ---- queries as f16 operands (bf16 rows scaled to at most 512), barriers, tensor memory
+  if (warp == 0) tc::tmem_alloc(&sm.tmem, 512);
+  if (tid == 0) {
+    for (int i = 0; i < 2; i++) {
+      tc::mbar_init(&sm.k_full[i], 128);
+      tc::mbar_init(&sm.v_full[i], 128);
+      tc::mbar_init(&sm.k_empty[i], 1);
+      tc::mbar_init(&sm.v_empty[i], 1);
+      tc::mbar_init(&sm.s_full[i], 1);
+      tc::mbar_init(&sm.p_full[i], 128);
+    }
+    tc::mbar_init(&sm.o_full, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  for (int it = tid; it < TILES * 128 * 4; it += C::kWarps * 32) {   // kWarps * 32 is a multiple of 4: lanes stay together
+    const int r = it >> 2, t = it & 3, row = row0 + r;
+    const bool on = r < live;
+    const T16* src = (const T16*)a.q + (long long)(c0 + (on ? row / a.G : 0)) * a.q_tok +
+                     (long long)(h * a.G + (on ? row % a.G : 0)) * a.q_head;
+    float v[L::NS][2 * E2], amax = 0.f;
+#pragma unroll
+    for (int sl = 0; sl < L::NS; sl++)
+#pragma unroll
+      for (int x = 0; x < 2 * E2 / 8; x++) {
+        const uint4 y = on ? *reinterpret_cast<const uint4*>(src + sl * L::SD + t * 2 * E2 + x * 8) : make_uint4(0, 0, 0, 0);
+        const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const float2 f = pr::up2<T16>(w[k]);
+          v[sl][8 * x + 2 * k] = f.x, v[sl][8 * x + 2 * k + 1] = f.y;
+          amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+        }
+      }
+    float mul = 1.f, back = 1.f;
+    if (!std::is_same<T16, __half>::value) {
+      const uint32_t quad = 0xFu << (lane & 28);
+      amax = fmaxf(amax, __shfl_xor_sync(quad, amax, 1));
+      amax = fmaxf(amax, __shfl_xor_sync(quad, amax, 2));
+      const int e = amax > 0.f ? max(-110, min(110, (int)(__float_as_uint(amax) >> 23) - 127 - 8)) : 0;
+      mul = pow2f(-e), back = pow2f(e);
+    }
+    if (t == 0) sm.row_scale[r] = back * fabsf(a.scale_log2);     // the scale's sign goes to the row: scores only grow
+    mul = copysignf(mul, a.scale_log2);
+    uint8_t* dst = sm.q[r >> 7] + ((r & 127) >> 3) * kQSbo + (r & 7) * 16;
+#pragma unroll
+    for (int sl = 0; sl < L::NS; sl++)
+#pragma unroll
+      for (int c = 0; c < E2 / 4; c++) {
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) w[k] = pr::f16x2(v[sl][4 * c + k] * mul, v[sl][E2 + 4 * c + k] * mul);
+        *reinterpret_cast<uint4*>(dst + (sl * (L::SD / 8) + t * (E2 / 4) + c) * 128) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+  }
+  tc::fence_proxy_async_smem();
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = sm.tmem;
+  bool ok = true;
+
+  if (warp < C::kSoftWarps) {
+    // ---- softmax: thread = row
+    const int t = warp >> 2, r = t * 128 + (warp & 3) * 32 + lane;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_at = tmem + lanes + t * 128, o_at = tmem + lanes + C::kOCol + t * D;
+    const int row = row0 + r, p = p0 + min(row, rows - 1) / a.G;
+    const int pt_first = p0 + (row0 + t * 128) / a.G, pt_last = p0 + min(row0 + t * 128 + 127, rows - 1) / a.G;
+    const float cs = sm.row_scale[r];
+    float m = -INFINITY, l = 0.f;
+    if (t < ntile) {
+      for (int i = 0; i < nkb && ok; i++) {
+        const int j0 = (kb0 + i) * BK;
+        const bool edge = j0 + BK - 1 > pt_first || (a.window > 0 && j0 <= pt_last - a.window);
+        ok = tc::mbar_wait(&sm.s_full[t], i & 1);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        tc::fence_after();
+        // the row's largest score; where it exceeds the reference by 2^8 (or there is none yet) the reference moves
+        float top = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < BK / 32; c++) {
+          uint32_t u[32];
+          pr::ld32(s_at + c * 32, u);
+          tc::tmem_wait_ld();
+          if (edge) hide<32>(u, j0 + c * 32, p, a.window);
+#pragma unroll
+          for (int k = 0; k < 32; k += 2) top = pr::max3(top, __uint_as_float(u[k]), __uint_as_float(u[k + 1]));
+        }
+        top *= cs;                           // cs >= 0; -inf stays (0 * -inf: NaN, which moves nothing)
+        const bool move = m == -INFINITY ? top > -INFINITY : top > m + 8.f;
+        if (__any_sync(0xffffffffu, move)) {
+          const float f = !move ? 1.f : m == -INFINITY ? 0.f : pr::exp2_fast(m - top);
+          if (move) m = top;
+          l *= f;
+          if (i > 0) {                       // S is complete, so the product before it, into O, is too
+#pragma unroll 1
+            for (int c = 0; c < D / 32; c++) {
+              uint32_t u[32];
+              pr::ld32(o_at + c * 32, u);
+              tc::tmem_wait_ld();
+#pragma unroll
+              for (int k = 0; k < 32; k++) u[k] = __float_as_uint(__uint_as_float(u[k]) * f);
+              pr::st32(o_at + c * 32, u);
+            }
+          }
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+        float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+        for (int c = 0; c < BK / 32; c++) {  // P of these 32 keys takes columns that have been read
+          uint32_t u[32], pk[16];
+          pr::ld32(s_at + c * 32, u);
+          tc::tmem_wait_ld();
+          if (edge) hide<32>(u, j0 + c * 32, p, a.window);
+#pragma unroll
+          for (int k = 0; k < 32; k += 2) {
+            float x = __uint_as_float(u[k]), y = __uint_as_float(u[k + 1]);
+            pr::fma2(x, y, cs, -ref);
+            x = pr::exp2_fast(x), y = pr::exp2_fast(y);
+            s0 += x, s1 += y;
+            pk[k / 2] = pr::f16x2(x, y);
+          }
+          pr::st16(s_at + c * 16, pk);
+        }
+        l += s0 + s1;
+        pr::wait_st();
+        tc::fence_before();
+        pr::arrive(&sm.p_full[t]);
+      }
+      // ---- output
+      if (nkb > 0 && ok) {
+        ok = tc::mbar_wait(&sm.o_full, 0);
+        if (!__all_sync(0xffffffffu, ok)) ok = false;
+      }
+      if (ok) {
+        tc::fence_after();
+        const float inv = l > 0.f ? __fdividef(a.v_mul, l) : l;
+        const long long at = (long long)(c0 + row / a.G) * a.H * a.G + h * a.G + row % a.G;
+        const bool on = r < live;
+        constexpr int E = L::SD / 8;         // values of a lane's piece; column (i, g) of a slab = value E g + i
+#pragma unroll
+        for (int sl = 0; sl < L::NS; sl++)
+#pragma unroll
+          for (int part = 0; part < E / 8; part++) {      // 64 columns: values i = 8 part .. + 7 of all pieces
+            uint32_t u[2][32];
+            if (nkb > 0) {
+              pr::ld32(o_at + sl * L::SD + part * 64, u[0]);
+              pr::ld32(o_at + sl * L::SD + part * 64 + 32, u[1]);
+              tc::tmem_wait_ld();
+            } else {
+#pragma unroll
+              for (int k = 0; k < 64; k++) u[k >> 5][k & 31] = 0;
+            }
+            if (on) {
+#pragma unroll
+              for (int g = 0; g < 8; g++) {
+                float x[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++) x[k] = __uint_as_float(u[(k * 8 + g) >> 5][(k * 8 + g) & 31]) * inv;
+                *reinterpret_cast<uint4*>((T16*)a.out + at * D + sl * L::SD + E * g + part * 8) =
+                    make_uint4(pr::down2<T16>(x[0], x[1]), pr::down2<T16>(x[2], x[3]), pr::down2<T16>(x[4], x[5]),
+                               pr::down2<T16>(x[6], x[7]));
+              }
+            }
+          }
+        if (on && a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.6931471805599453f;
+      }
+    }
+  } else if (warp < C::kSoftWarps + 4) {
+    // ---- keys and values from 4 bits to f16 operands; codes are fetched a block ahead
+    const int dt = tid - C::kSoftWarps * 32;
+    constexpr int KI = BK * 4 * L::NS / 128;                 // key pieces per thread: 4
+    constexpr int W = L::SD / 32;                            // 32-bit words of a key piece
+    const int kt = (dt >> 3) & 3, kj = (dt & 7) | (dt >> 5) << 3;   // piece, token (of 32): 8 neighbours store one core matrix
+    constexpr int OCT = BK / 8;                              // octets of tokens
+    const int vg = dt & 7, vo = (dt >> 3) % OCT, vsl = (dt >> 3) / OCT;
+    uint32_t kc[KI][W], vc[4][W], ks[KI], vs[4];
+    auto page_at = [&](int kb, int i) -> const uint8_t* {    // page i of the key block; null: none, or a bad one
+      const int page = kb * (BK / kPage) + i;
+      if (kb >= kb1 || page >= a.W || page * kPage > p_last) return nullptr;
+      const int phys = a.table[(long long)b * a.W + page];
+      if (phys < 0 || phys >= a.n_pages) {
+        set_status(a.status, kBadIndex);
+        return nullptr;
+      }
+      return a.pages + ((long long)phys * a.H + h) * L::kPageBytes;
+    };
+    auto fetch_k = [&](int kb) {
+#pragma unroll
+      for (int i = 0; i < KI; i++) {
+        const int sl = i * 32 / BK, j = i * 32 % BK + kj;    // BK = 64: two tokens per slab
+        const uint8_t* pg = page_at(kb, j / kPage);
+        const int jj = j % kPage;
+        ks[i] = 0;
+        if (pg && kb * BK + j <= p_last) {
+          load_words<W>(pg + L::KC + sl * L::kSlabBytes + jj * (L::SD / 2) + kt * (L::SD / 8), kc[i]);
+          ks[i] = key_scales<D>(pg + L::KS + jj * L::NB, sl, kt);
+        } else {
+#pragma unroll
+          for (int w = 0; w < W; w++) kc[i][w] = 0;
+        }
+      }
+    };
+    auto fetch_v = [&](int kb) {
+      const uint8_t* pg = page_at(kb, vo / 8);
+      const int pair0 = vo % 8 * 4;
+#pragma unroll
+      for (int x = 0; x < 4; x++) {
+        vs[x] = 0;
+        const int j = kb * BK + vo * 8 + 2 * x;
+        if (pg && j <= p_last) {
+          load_words<W>(pg + L::VC + vsl * L::kSlabBytes + (pair0 + x) * L::SD + vg * (L::SD / 8), vc[x]);
+          vs[x] = value_scales<D>(pg + L::VS + (pair0 + x) * (2 * L::NB), vsl, vg);
+          if (j == p_last) vs[x] &= 0xFFFFu;                 // the pair's second token is past the rows
+        } else {
+#pragma unroll
+          for (int w = 0; w < W; w++) vc[x][w] = 0;
+        }
+      }
+    };
+    fetch_k(kb0);
+    fetch_v(kb0);
+    for (int i = 0; i < nkb && ok; i++) {
+      const int st = i & 1;
+      if (i >= 2) ok = tc::mbar_wait(&sm.k_empty[st], ((i >> 1) - 1) & 1);
+      if (!ok) break;
+#pragma unroll
+      for (int x = 0; x < KI; x++) {
+        const int sl = x * 32 / BK, j = x * 32 % BK + kj;
+        uint8_t* dst = sm.k[st] + (j >> 3) * kKSbo + (j & 7) * 16 + (sl * (L::SD / 8) + kt * (E2 / 4)) * 128;
+#pragma unroll
+        for (int w = 0; w < W; w++) {
+          uint32_t f[4];
+          e2m1x8_to_f16(kc[x][w], f);
+          *reinterpret_cast<uint4*>(dst + w * 128) = make_uint4(mul_f16x2(f[0], ks[x]), mul_f16x2(f[1], ks[x]),
+                                                               mul_f16x2(f[2], ks[x]), mul_f16x2(f[3], ks[x]));
+        }
+      }
+      tc::fence_proxy_async_smem();
+      pr::arrive(&sm.k_full[st]);
+      fetch_k(kb0 + i + 1);
+      if (i >= 2) ok = tc::mbar_wait(&sm.v_empty[st], ((i >> 1) - 1) & 1);
+      if (!ok) break;
+      // values: a thread has 8 tokens of its piece: per value one 16-byte row of a core matrix
+      uint8_t* dst = sm.v[st] + vsl * (L::SD / 8) * kVSbo + vo * 128 + vg * 16;
+      constexpr int WV = W / 2;                              // words per token
+#pragma unroll
+      for (int w = 0; w < WV; w++) {
+        uint32_t lo[4][4], hi[4][4];                         // [pair][value]
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+          uint32_t c0w, c8w;
+          join_pair(vc[x][w], vc[x][WV + w], c0w, c8w);
+          e2m1x8_to_f16(c0w, lo[x]);
+          e2m1x8_to_f16(c8w, hi[x]);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const int n = 4 * w + k;
+          *reinterpret_cast<uint4*>(dst + n * kVSbo) = make_uint4(mul_f16x2(lo[0][k], vs[0]), mul_f16x2(lo[1][k], vs[1]),
+                                                                 mul_f16x2(lo[2][k], vs[2]), mul_f16x2(lo[3][k], vs[3]));
+          *reinterpret_cast<uint4*>(dst + (E2 / 2 + n) * kVSbo) = make_uint4(
+              mul_f16x2(hi[0][k], vs[0]), mul_f16x2(hi[1][k], vs[1]), mul_f16x2(hi[2][k], vs[2]), mul_f16x2(hi[3][k], vs[3]));
+        }
+      }
+      tc::fence_proxy_async_smem();
+      pr::arrive(&sm.v_full[st]);
+      fetch_v(kb0 + i + 1);
+    }
+  } else if (lane == 0) {
+    // ---- products
+    const uint32_t id_s = pr::idesc_f16(128, BK), id_o = pr::idesc_f16(128, D);
+    auto scores = [&](int t, int st) {
+      const uint32_t qa = tc::smem_addr(sm.q[t]), ka = tc::smem_addr(sm.k[st]);
+#pragma unroll
+      for (int k = 0; k < D / 16; k++)
+        pr::mma_ss(tmem + t * 128, tc::smem_desc(qa + k * 256, 128, kQSbo), tc::smem_desc(ka + k * 256, 128, kKSbo), id_s, k > 0);
+      tc::commit(&sm.s_full[t]);
+    };
+    auto outputs = [&](int t, int st, bool first) {
+      const uint32_t va = tc::smem_addr(sm.v[st]);
+#pragma unroll
+      for (int k = 0; k < BK / 16; k++)
+        pr::mma_ts(tmem + C::kOCol + t * D, tmem + t * 128 + k * 8, tc::smem_desc(va + k * 256, 128, kVSbo), id_o, !first || k > 0);
+    };
+    if (nkb > 0) {
+      ok = tc::mbar_wait(&sm.k_full[0], 0);
+      tc::fence_after();
+      if (ok) {
+        for (int t = 0; t < ntile; t++) scores(t, 0);
+        tc::commit(&sm.k_empty[0]);
+      }
+    }
+    for (int i = 0; i < nkb && ok; i++) {
+      const int st = i & 1, nx = st ^ 1;
+      ok = tc::mbar_wait(&sm.v_full[st], (i >> 1) & 1);
+      if (ok && i + 1 < nkb) ok = tc::mbar_wait(&sm.k_full[nx], ((i + 1) >> 1) & 1);
+      for (int t = 0; t < ntile && ok; t++) {
+        ok = tc::mbar_wait(&sm.p_full[t], i & 1);
+        if (!ok) break;
+        tc::fence_after();
+        outputs(t, st, i == 0);
+        if (i + 1 < nkb) scores(t, nx);        // runs after the product that reads P, in the order of issue
+      }
+      if (!ok) break;
+      tc::commit(&sm.v_empty[st]);
+      if (i + 1 < nkb) tc::commit(&sm.k_empty[nx]);
+    }
+    if (nkb > 0) tc::commit(&sm.o_full);
+  }
+  __syncwarp();
+  if (!ok) set_status(a.status, kTimeout);
+  tc::fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc::fence_after();
+    tc::tmem_relinquish();
+    tc::tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace kv4
+}  // namespace moet
+
+using namespace moet;
+using namespace moet::kv4;
+
+void kv4_prompt(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_lens, torch::Tensor table, torch::Tensor pages,
+                double scale, int64_t max_q, int64_t window, int64_t k_exp, int64_t v_exp, torch::Tensor out,
+                c10::optional<torch::Tensor> lse, torch::Tensor status) {
+  PromptArgs a;
+  const int D = (int)(pages.size(2) / 72);
+  a.T = (int)q.size(0); a.H = (int)pages.size(1); a.G = (int)(q.size(1) / a.H);
+  a.B = (int)seq_lens.size(0); a.W = (int)table.size(1);
+  a.q = q.data_ptr(); a.q_tok = q.stride(0); a.q_head = (int)q.stride(1);
+  a.cu_q = (const int*)cu_q.data_ptr(); a.seq_lens = (const int*)seq_lens.data_ptr();
+  a.table = (const int*)table.data_ptr(); a.window = (int)window;
+  a.pages = (const uint8_t*)pages.data_ptr(); a.n_pages = (int)pages.size(0);
+  a.scale_log2 = (float)(scale * 1.4426950408889634 * std::ldexp(1.0, (int)k_exp));
+  a.v_mul = std::ldexp(1.f, (int)v_exp);
+  a.out = out.data_ptr(); a.lse = (float*)opt_ptr(lse);
+  a.status = (int*)status.data_ptr();
+  if (a.T == 0 || a.B == 0) return;
+  TORCH_CHECK(a.B <= 65535 && a.H <= 65535, "kv4_prompt: too many sequences or heads");
+  auto stream = at::cuda::getCurrentCUDAStream();
+  auto go = [&](auto dim, auto t) {
+    constexpr int DD = decltype(dim)::value;
+    using T16 = decltype(t);
+    using C = PromptCfg<DD>;
+    const int64_t rows = std::min<int64_t>(max_q, a.T) * a.G;
+    const dim3 grid((unsigned)((rows + C::TILES * 128 - 1) / (C::TILES * 128)), a.H, a.B);
+    moet_allow_max_smem(kv4_prompt_kernel<DD, T16>);
+    launch_k(kv4_prompt_kernel<DD, T16>, grid, dim3(C::kWarps * 32), sizeof(PromptSmem<DD>), stream, a);
+  };
+  auto by_type = [&](auto dim) {
+    if (q.scalar_type() == at::kHalf) go(dim, __half{});
+    else go(dim, __nv_bfloat16{});
+  };
+  if (D == 64) by_type(std::integral_constant<int, 64>{});
+  else if (D == 128) by_type(std::integral_constant<int, 128>{});
+  else by_type(std::integral_constant<int, 256>{});
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}

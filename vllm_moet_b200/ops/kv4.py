@@ -31,6 +31,8 @@ from . import native
 
 PAGE = 64
 HEAD_DIMS = (64, 128, 256)
+# query rows of one sequence and K/V head above which attention runs on the tcgen05 kernel
+PROMPT_ROWS = 64
 _STATUS = {1: "a slot or page out of range", 2: "a wait on the device ran out", 3: "bad size",
            4: "a key or value that is not finite (NaN is held as 0, infinities as the largest value)"}
 
@@ -175,7 +177,10 @@ class KV4Cache:
             q = q.clone(memory_format=torch.contiguous_format)
         out = torch.empty(T, Hq, self.head_dim, dtype=q.dtype, device=self.device)
         lse = torch.empty(T, Hq, dtype=torch.float32, device=self.device) if return_lse else None
-        if T:
+        if T and pages is None and max_q * (Hq // self.num_kv_heads) > PROMPT_ROWS:
+            self._C.kv4_prompt(q, cu_q, seq_lens, block_table, self.pages, scale, max_q, window, self.k_exp, self.v_exp,
+                               out, lse, self.status)
+        elif T:
             part, split = _workspace(self.device, *self._C.kv4_attend_workspace(
                 Hq // self.num_kv_heads, self.head_dim, max_q, pages is not None))
             self._C.kv4_attend(q, cu_q, seq_lens, block_table, self.pages, pages, scale, max_q, window, self.k_exp,
