@@ -75,16 +75,21 @@ template <typename T16> MOET_DEVICE float to_f32(T16 x);
 template <> MOET_DEVICE float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
 template <> MOET_DEVICE float to_f32(__half x) { return __half2float(x); }
 
-// the f16x2 that scales a lane's key codes: `row` = the token's scales, sl the slab, t the piece
-template <int D> MOET_DEVICE uint32_t key_scales(const uint8_t* row, int sl, int t) {
-  if constexpr (Lay<D>::SD == 128) return e4m3x2_to_f16(*reinterpret_cast<const uint16_t*>(row + sl * 8 + 2 * t));
+// the two scale bytes of a lane's key codes: `row` = the token's scales, sl the slab, t the piece
+template <int D> MOET_DEVICE uint16_t raw_key_scales(const uint8_t* row, int sl, int t) {
+  if constexpr (Lay<D>::SD == 128) return *reinterpret_cast<const uint16_t*>(row + sl * 8 + 2 * t);
   const uint32_t b = row[t];
-  return e4m3x2_to_f16((uint16_t)(b | b << 8));
+  return (uint16_t)(b | b << 8);
 }
-// the f16x2 (one scale per token of the pair) of a lane's value codes: `row` = the pair's scales
+// of a lane's value codes, one per token of the pair: `row` = the pair's scales, g the piece
+template <int D> MOET_DEVICE uint16_t raw_value_scales(const uint8_t* row, int sl, int g) {
+  return *reinterpret_cast<const uint16_t*>(row + 2 * (Lay<D>::SD == 128 ? sl * 8 + g : g >> 1));
+}
+template <int D> MOET_DEVICE uint32_t key_scales(const uint8_t* row, int sl, int t) {
+  return e4m3x2_to_f16(raw_key_scales<D>(row, sl, t));
+}
 template <int D> MOET_DEVICE uint32_t value_scales(const uint8_t* row, int sl, int g) {
-  const int b = Lay<D>::SD == 128 ? sl * 8 + g : g >> 1;
-  return e4m3x2_to_f16(*reinterpret_cast<const uint16_t*>(row + 2 * b));
+  return e4m3x2_to_f16(raw_value_scales<D>(row, sl, g));
 }
 
 MOET_DEVICE float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }   // -126 <= e <= 127

@@ -35,7 +35,7 @@ struct PromptArgs {
 template <int D> struct PromptCfg {
   static constexpr int BK = D == 256 ? 64 : 128;            // keys per block
   static constexpr int TILES = D == 256 ? 1 : 2;            // row tiles per block
-  static constexpr int kSoftWarps = 4 * TILES, kWarps = kSoftWarps + 5;
+  static constexpr int kSoftWarps = 4 * TILES, kWarps = kSoftWarps + 8;   // + conversion, + products (one of four)
   static constexpr int kQBytes = 128 * D * 2, kKBytes = BK * D * 2;   // one operand tile; V's is K's size
   static constexpr int kOCol = 256;                         // tensor memory: S (and P) of tile t at t * 128, O after them
 };
@@ -92,6 +92,10 @@ MOET_DEVICE float exp2_fast(float x) {
 MOET_DEVICE void fma2(float& x, float& y, float c, float b) {
   asm("{\n.reg .b64 u, v, w;\nmov.b64 u, {%0, %1};\nmov.b64 v, {%2, %2};\nmov.b64 w, {%3, %3};\n"
       "fma.rn.ftz.f32x2 u, u, v, w;\nmov.b64 {%0, %1}, u;\n}\n" : "+f"(x), "+f"(y) : "f"(c), "f"(b));
+}
+MOET_DEVICE void add2(float& x, float& y, float a, float b) {
+  asm("{\n.reg .b64 u, v;\nmov.b64 u, {%0, %1};\nmov.b64 v, {%2, %3};\nadd.rn.ftz.f32x2 u, u, v;\nmov.b64 {%0, %1}, u;\n}\n"
+      : "+f"(x), "+f"(y) : "f"(a), "f"(b));
 }
 MOET_DEVICE float max3(float a, float b, float c) {
   float d;
@@ -204,8 +208,11 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
   const uint32_t tmem = sm.tmem;
   bool ok = true;
 
+  // Registers go where they are needed: the block starts with 128 a thread (512 threads) and ends with
+  // 256 x 168 + 128 x 104 + 128 x 72, the same sum.  (One tile: 384 threads start with 168.)
   if (warp < C::kSoftWarps) {
-    // ---- softmax: thread = row
+    // ---- softmax: thread = row; its scores of a block all in registers
+    if constexpr (TILES == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
     const int t = warp >> 2, r = t * 128 + (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + lanes + t * 128, o_at = tmem + lanes + C::kOCol + t * D;
@@ -220,17 +227,22 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
         ok = tc::mbar_wait(&sm.s_full[t], i & 1);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         tc::fence_after();
+        uint32_t u[BK / 32][32];
+#pragma unroll
+        for (int c = 0; c < BK / 32; c++) pr::ld32(s_at + c * 32, u[c]);
+        tc::tmem_wait_ld();
         // the row's largest score; where it exceeds the reference by 2^8 (or there is none yet) the reference moves
-        float top = -INFINITY;
+        float top = -INFINITY, top1 = -INFINITY;
 #pragma unroll
         for (int c = 0; c < BK / 32; c++) {
-          uint32_t u[32];
-          pr::ld32(s_at + c * 32, u);
-          tc::tmem_wait_ld();
-          if (edge) hide<32>(u, j0 + c * 32, p, a.window);
+          if (edge) hide<32>(u[c], j0 + c * 32, p, a.window);
 #pragma unroll
-          for (int k = 0; k < 32; k += 2) top = pr::max3(top, __uint_as_float(u[k]), __uint_as_float(u[k + 1]));
+          for (int k = 0; k < 32; k += 4) {
+            top = pr::max3(top, __uint_as_float(u[c][k]), __uint_as_float(u[c][k + 1]));
+            top1 = pr::max3(top1, __uint_as_float(u[c][k + 2]), __uint_as_float(u[c][k + 3]));
+          }
         }
+        top = fmaxf(top, top1);
         top *= cs;                           // cs >= 0; -inf stays (0 * -inf: NaN, which moves nothing)
         const bool move = m == -INFINITY ? top > -INFINITY : top > m + 8.f;
         if (__any_sync(0xffffffffu, move)) {
@@ -252,17 +264,14 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
         const float ref = m == -INFINITY ? 0.f : m;
         float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-        for (int c = 0; c < BK / 32; c++) {  // P of these 32 keys takes columns that have been read
-          uint32_t u[32], pk[16];
-          pr::ld32(s_at + c * 32, u);
-          tc::tmem_wait_ld();
-          if (edge) hide<32>(u, j0 + c * 32, p, a.window);
+        for (int c = 0; c < BK / 32; c++) {
+          uint32_t pk[16];
 #pragma unroll
           for (int k = 0; k < 32; k += 2) {
-            float x = __uint_as_float(u[k]), y = __uint_as_float(u[k + 1]);
+            float x = __uint_as_float(u[c][k]), y = __uint_as_float(u[c][k + 1]);
             pr::fma2(x, y, cs, -ref);
             x = pr::exp2_fast(x), y = pr::exp2_fast(y);
-            s0 += x, s1 += y;
+            pr::add2(s0, s1, x, y);
             pk[k / 2] = pr::f16x2(x, y);
           }
           pr::st16(s_at + c * 16, pk);
@@ -313,33 +322,39 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
     }
   } else if (warp < C::kSoftWarps + 4) {
     // ---- keys and values from 4 bits to f16 operands; codes are fetched a block ahead
+    if constexpr (TILES == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     const int dt = tid - C::kSoftWarps * 32;
     constexpr int KI = BK * 4 * L::NS / 128;                 // key pieces per thread: 4
     constexpr int W = L::SD / 32;                            // 32-bit words of a key piece
     const int kt = (dt >> 3) & 3, kj = (dt & 7) | (dt >> 5) << 3;   // piece, token (of 32): 8 neighbours store one core matrix
     constexpr int OCT = BK / 8;                              // octets of tokens
     const int vg = dt & 7, vo = (dt >> 3) % OCT, vsl = (dt >> 3) / OCT;
-    uint32_t kc[KI][W], vc[4][W], ks[KI], vs[4];
-    auto page_at = [&](int kb, int i) -> const uint8_t* {    // page i of the key block; null: none, or a bad one
-      const int page = kb * (BK / kPage) + i;
-      if (kb >= kb1 || page >= a.W || page * kPage > p_last) return nullptr;
-      const int phys = a.table[(long long)b * a.W + page];
-      if (phys < 0 || phys >= a.n_pages) {
-        set_status(a.status, kBadIndex);
-        return nullptr;
+    uint32_t kc[KI][W], vc[4][W];
+    uint16_t ks[KI], vs[4];                                  // scales as they are held: converting waits for the load
+    // pages of a key block, looked up two blocks ahead (the look-up is a load of its own): -1 for none
+    constexpr int KP = BK / kPage;
+    int ahead[KP], page[KP];                                 // of the block after the next one, of the next one
+    auto look_up = [&](int kb, int (&to)[KP]) {
+#pragma unroll
+      for (int i = 0; i < KP; i++) {
+        const int x = kb * KP + i;
+        to[i] = kb < kb1 && x < a.W && x * kPage <= p_last ? a.table[(long long)b * a.W + x] : -1;
       }
-      return a.pages + ((long long)phys * a.H + h) * L::kPageBytes;
+    };
+    auto at = [&](int phys) -> const uint8_t* {
+      if (phys >= a.n_pages || phys < -1) set_status(a.status, kBadIndex);
+      return phys < 0 || phys >= a.n_pages ? nullptr : a.pages + ((long long)phys * a.H + h) * L::kPageBytes;
     };
     auto fetch_k = [&](int kb) {
 #pragma unroll
       for (int i = 0; i < KI; i++) {
         const int sl = i * 32 / BK, j = i * 32 % BK + kj;    // BK = 64: two tokens per slab
-        const uint8_t* pg = page_at(kb, j / kPage);
+        const uint8_t* pg = at(page[i * 32 % BK / kPage]);
         const int jj = j % kPage;
         ks[i] = 0;
         if (pg && kb * BK + j <= p_last) {
           load_words<W>(pg + L::KC + sl * L::kSlabBytes + jj * (L::SD / 2) + kt * (L::SD / 8), kc[i]);
-          ks[i] = key_scales<D>(pg + L::KS + jj * L::NB, sl, kt);
+          ks[i] = raw_key_scales<D>(pg + L::KS + jj * L::NB, sl, kt);
         } else {
 #pragma unroll
           for (int w = 0; w < W; w++) kc[i][w] = 0;
@@ -347,7 +362,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
       }
     };
     auto fetch_v = [&](int kb) {
-      const uint8_t* pg = page_at(kb, vo / 8);
+      const uint8_t* pg = at(vo / 8 ? page[KP - 1] : page[0]);
       const int pair0 = vo % 8 * 4;
 #pragma unroll
       for (int x = 0; x < 4; x++) {
@@ -355,14 +370,16 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
         const int j = kb * BK + vo * 8 + 2 * x;
         if (pg && j <= p_last) {
           load_words<W>(pg + L::VC + vsl * L::kSlabBytes + (pair0 + x) * L::SD + vg * (L::SD / 8), vc[x]);
-          vs[x] = value_scales<D>(pg + L::VS + (pair0 + x) * (2 * L::NB), vsl, vg);
-          if (j == p_last) vs[x] &= 0xFFFFu;                 // the pair's second token is past the rows
+          vs[x] = raw_value_scales<D>(pg + L::VS + (pair0 + x) * (2 * L::NB), vsl, vg);
+          if (j == p_last) vs[x] &= 0xFFu;                   // the pair's second token is past the rows
         } else {
 #pragma unroll
           for (int w = 0; w < W; w++) vc[x][w] = 0;
         }
       }
     };
+    look_up(kb0, page);
+    look_up(kb0 + 1, ahead);
     fetch_k(kb0);
     fetch_v(kb0);
     for (int i = 0; i < nkb && ok; i++) {
@@ -372,23 +389,30 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
 #pragma unroll
       for (int x = 0; x < KI; x++) {
         const int sl = x * 32 / BK, j = x * 32 % BK + kj;
+        const uint32_t f16s = e4m3x2_to_f16(ks[x]);
         uint8_t* dst = sm.k[st] + (j >> 3) * kKSbo + (j & 7) * 16 + (sl * (L::SD / 8) + kt * (E2 / 4)) * 128;
 #pragma unroll
         for (int w = 0; w < W; w++) {
           uint32_t f[4];
           e2m1x8_to_f16(kc[x][w], f);
-          *reinterpret_cast<uint4*>(dst + w * 128) = make_uint4(mul_f16x2(f[0], ks[x]), mul_f16x2(f[1], ks[x]),
-                                                               mul_f16x2(f[2], ks[x]), mul_f16x2(f[3], ks[x]));
+          *reinterpret_cast<uint4*>(dst + w * 128) = make_uint4(mul_f16x2(f[0], f16s), mul_f16x2(f[1], f16s),
+                                                               mul_f16x2(f[2], f16s), mul_f16x2(f[3], f16s));
         }
       }
       tc::fence_proxy_async_smem();
       pr::arrive(&sm.k_full[st]);
+#pragma unroll
+      for (int x = 0; x < KP; x++) page[x] = ahead[x];
       fetch_k(kb0 + i + 1);
+      look_up(kb0 + i + 2, ahead);
       if (i >= 2) ok = tc::mbar_wait(&sm.v_empty[st], ((i >> 1) - 1) & 1);
       if (!ok) break;
       // values: a thread has 8 tokens of its piece: per value one 16-byte row of a core matrix
       uint8_t* dst = sm.v[st] + vsl * (L::SD / 8) * kVSbo + vo * 128 + vg * 16;
       constexpr int WV = W / 2;                              // words per token
+      uint32_t fs[4];
+#pragma unroll
+      for (int x = 0; x < 4; x++) fs[x] = e4m3x2_to_f16(vs[x]);
 #pragma unroll
       for (int w = 0; w < WV; w++) {
         uint32_t lo[4][4], hi[4][4];                         // [pair][value]
@@ -402,17 +426,19 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
 #pragma unroll
         for (int k = 0; k < 4; k++) {
           const int n = 4 * w + k;
-          *reinterpret_cast<uint4*>(dst + n * kVSbo) = make_uint4(mul_f16x2(lo[0][k], vs[0]), mul_f16x2(lo[1][k], vs[1]),
-                                                                 mul_f16x2(lo[2][k], vs[2]), mul_f16x2(lo[3][k], vs[3]));
+          *reinterpret_cast<uint4*>(dst + n * kVSbo) = make_uint4(mul_f16x2(lo[0][k], fs[0]), mul_f16x2(lo[1][k], fs[1]),
+                                                                 mul_f16x2(lo[2][k], fs[2]), mul_f16x2(lo[3][k], fs[3]));
           *reinterpret_cast<uint4*>(dst + (E2 / 2 + n) * kVSbo) = make_uint4(
-              mul_f16x2(hi[0][k], vs[0]), mul_f16x2(hi[1][k], vs[1]), mul_f16x2(hi[2][k], vs[2]), mul_f16x2(hi[3][k], vs[3]));
+              mul_f16x2(hi[0][k], fs[0]), mul_f16x2(hi[1][k], fs[1]), mul_f16x2(hi[2][k], fs[2]), mul_f16x2(hi[3][k], fs[3]));
         }
       }
       tc::fence_proxy_async_smem();
       pr::arrive(&sm.v_full[st]);
       fetch_v(kb0 + i + 1);
     }
-  } else if (lane == 0) {
+  } else {
+    if constexpr (TILES == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == C::kSoftWarps + 4 && lane == 0) {
     // ---- products
     const uint32_t id_s = pr::idesc_f16(128, BK), id_o = pr::idesc_f16(128, D);
     auto scores = [&](int t, int st) {
@@ -452,6 +478,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
       if (i + 1 < nkb) tc::commit(&sm.k_empty[nx]);
     }
     if (nkb > 0) tc::commit(&sm.o_full);
+    }
   }
   __syncwarp();
   if (!ok) set_status(a.status, kTimeout);
