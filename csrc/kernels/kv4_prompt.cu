@@ -4,12 +4,13 @@
 // A block takes two tiles of 128 rows ((token, head of the group) pairs of one K/V head; one
 // tile with D = 256) and walks over blocks of 128 (64) keys.  Per key block and tile
 //   S = Q K^T   f16 x f16 -> f32 in tensor memory,
-//   P = exp2(S c - m), written back over S as f16 (the A operand of the second product),
+//   P = exp2(S c - m) as f16 in tensor memory (the A operand of the second product),
 //   O += P V    f32 in tensor memory.
 // Roles: four warps convert keys and values from 4 bits into f16 operands in shared memory
 // (exact, kv4.cuh), once for both tiles; four warps per tile hold a row per thread and do the
-// softmax; one thread issues the products, in the order S0 S1 | PV0 S0' | PV1 S1' | ..., so one
-// tile's products run under the other's softmax.
+// softmax; one thread issues the products.  A row's scores go to registers at once, so the two
+// tiles share one S buffer and a tile's next scores are computed under its softmax; the order
+// of issue is S0' PV0 S1' PV1 (' = next key block).
 //
 // The running maximum is only moved when a row's scores exceed it by 2^8 (P <= 256 in f16, sums
 // in f32): O is rescaled a few times per row, not per block.  Operands are
@@ -37,7 +38,7 @@ template <int D> struct PromptCfg {
   static constexpr int TILES = D == 256 ? 1 : 2;            // row tiles per block
   static constexpr int kSoftWarps = 4 * TILES, kWarps = kSoftWarps + 8;   // + conversion, + products (one of four)
   static constexpr int kQBytes = 128 * D * 2, kKBytes = BK * D * 2;   // one operand tile; V's is K's size
-  static constexpr int kOCol = 256;                         // tensor memory: S (and P) of tile t at t * 128, O after them
+  static constexpr int kPCol = 128, kOCol = 256;            // tensor memory: S at 0, P of tile t at 128 + 64 t, O at 256 + D t
 };
 
 template <int D> struct PromptSmem {
@@ -46,19 +47,33 @@ template <int D> struct PromptSmem {
   uint8_t k[2][C::kKBytes];
   uint8_t v[2][C::kKBytes];
   float row_scale[C::TILES * 128];
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full;
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], s_free, p_full[2], pv_done[2];
   uint32_t tmem;
 };
 
 namespace pr {
 MOET_DEVICE uint32_t idesc_f16(int M, int N) { return 1u << 4 | (uint32_t)(N >> 3) << 17 | (uint32_t)(M >> 4) << 24; }
-MOET_DEVICE void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
-               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+// One product, issued by the warp's elected lane (`lead`); the operands are the same in every lane,
+// so that they stay in uniform registers.
+MOET_DEVICE void mma_ss(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile("{\n.reg .pred p, q;\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 q, %5, 0;\n"
+               "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(lead) : "memory");
 }
-MOET_DEVICE void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
-               ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+MOET_DEVICE void mma_ts(uint32_t lead, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile("{\n.reg .pred p, q;\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 q, %5, 0;\n"
+               "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
+               ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(lead) : "memory");
+}
+MOET_DEVICE void commit(uint32_t lead, uint64_t* bar) {
+  asm volatile("{\n.reg .pred q;\nsetp.ne.b32 q, %1, 0;\n"
+               "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n"
+               ::"r"(tc::smem_addr(bar)), "r"(lead) : "memory");
+}
+MOET_DEVICE uint32_t elect() {
+  uint32_t r;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xFFFFFFFF;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+  return r;
 }
 #define KV4_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
 #define KV4_W8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
@@ -157,8 +172,9 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
       tc::mbar_init(&sm.v_empty[i], 1);
       tc::mbar_init(&sm.s_full[i], 1);
       tc::mbar_init(&sm.p_full[i], 128);
+      tc::mbar_init(&sm.pv_done[i], 1);
     }
-    tc::mbar_init(&sm.o_full, 1);
+    tc::mbar_init(&sm.s_free, 128);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   for (int it = tid; it < TILES * 128 * 4; it += C::kWarps * 32) {   // kWarps * 32 is a multiple of 4: lanes stay together
@@ -215,7 +231,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
     if constexpr (TILES == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
     const int t = warp >> 2, r = t * 128 + (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_at = tmem + lanes + t * 128, o_at = tmem + lanes + C::kOCol + t * D;
+    const uint32_t s_at = tmem + lanes, p_at = s_at + C::kPCol + t * 64, o_at = tmem + lanes + C::kOCol + t * D;
     const int row = row0 + r, p = p0 + min(row, rows - 1) / a.G;
     const int pt_first = p0 + (row0 + t * 128) / a.G, pt_last = p0 + min(row0 + t * 128 + 127, rows - 1) / a.G;
     const float cs = sm.row_scale[r];
@@ -231,6 +247,8 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
 #pragma unroll
         for (int c = 0; c < BK / 32; c++) pr::ld32(s_at + c * 32, u[c]);
         tc::tmem_wait_ld();
+        tc::fence_before();
+        pr::arrive(&sm.s_free);              // the other tile's scores may come
         // the row's largest score; where it exceeds the reference by 2^8 (or there is none yet) the reference moves
         float top = -INFINITY, top1 = -INFINITY;
 #pragma unroll
@@ -245,11 +263,16 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
         top = fmaxf(top, top1);
         top *= cs;                           // cs >= 0; -inf stays (0 * -inf: NaN, which moves nothing)
         const bool move = m == -INFINITY ? top > -INFINITY : top > m + 8.f;
+        if (i > 0) {                         // the product before has read P and is in O
+          ok = tc::mbar_wait(&sm.pv_done[t], (i - 1) & 1);
+          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+          tc::fence_after();
+        }
         if (__any_sync(0xffffffffu, move)) {
           const float f = !move ? 1.f : m == -INFINITY ? 0.f : pr::exp2_fast(m - top);
           if (move) m = top;
           l *= f;
-          if (i > 0) {                       // S is complete, so the product before it, into O, is too
+          if (i > 0) {
 #pragma unroll 1
             for (int c = 0; c < D / 32; c++) {
               uint32_t u[32];
@@ -274,7 +297,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
             pr::add2(s0, s1, x, y);
             pk[k / 2] = pr::f16x2(x, y);
           }
-          pr::st16(s_at + c * 16, pk);
+          pr::st16(p_at + c * 16, pk);
         }
         l += s0 + s1;
         pr::wait_st();
@@ -283,7 +306,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
       }
       // ---- output
       if (nkb > 0 && ok) {
-        ok = tc::mbar_wait(&sm.o_full, 0);
+        ok = tc::mbar_wait(&sm.pv_done[t], (nkb - 1) & 1);
         if (!__all_sync(0xffffffffu, ok)) ok = false;
       }
       if (ok) {
@@ -438,46 +461,52 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
     }
   } else {
     if constexpr (TILES == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    if (warp == C::kSoftWarps + 4 && lane == 0) {
-    // ---- products
-    const uint32_t id_s = pr::idesc_f16(128, BK), id_o = pr::idesc_f16(128, D);
-    auto scores = [&](int t, int st) {
-      const uint32_t qa = tc::smem_addr(sm.q[t]), ka = tc::smem_addr(sm.k[st]);
-#pragma unroll
-      for (int k = 0; k < D / 16; k++)
-        pr::mma_ss(tmem + t * 128, tc::smem_desc(qa + k * 256, 128, kQSbo), tc::smem_desc(ka + k * 256, 128, kKSbo), id_s, k > 0);
-      tc::commit(&sm.s_full[t]);
-    };
-    auto outputs = [&](int t, int st, bool first) {
-      const uint32_t va = tc::smem_addr(sm.v[st]);
-#pragma unroll
-      for (int k = 0; k < BK / 16; k++)
-        pr::mma_ts(tmem + C::kOCol + t * D, tmem + t * 128 + k * 8, tc::smem_desc(va + k * 256, 128, kVSbo), id_o, !first || k > 0);
-    };
-    if (nkb > 0) {
-      ok = tc::mbar_wait(&sm.k_full[0], 0);
-      tc::fence_after();
-      if (ok) {
-        for (int t = 0; t < ntile; t++) scores(t, 0);
-        tc::commit(&sm.k_empty[0]);
-      }
-    }
-    for (int i = 0; i < nkb && ok; i++) {
-      const int st = i & 1, nx = st ^ 1;
-      ok = tc::mbar_wait(&sm.v_full[st], (i >> 1) & 1);
-      if (ok && i + 1 < nkb) ok = tc::mbar_wait(&sm.k_full[nx], ((i + 1) >> 1) & 1);
-      for (int t = 0; t < ntile && ok; t++) {
-        ok = tc::mbar_wait(&sm.p_full[t], i & 1);
-        if (!ok) break;
+    if (warp == C::kSoftWarps + 4) {
+      // ---- products: the whole warp waits, one lane issues
+      const uint32_t lead = pr::elect();
+      const uint32_t id_s = pr::idesc_f16(128, BK), id_o = pr::idesc_f16(128, D);
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint64_t q0 = tc::smem_desc(tc::smem_addr(sm.q[0]), 128, kQSbo), k0 = tc::smem_desc(tc::smem_addr(sm.k[0]), 128, kKSbo),
+                     v0 = tc::smem_desc(tc::smem_addr(sm.v[0]), 128, kVSbo);
+      // a descriptor moves on by its address in 16-byte steps: 256 bytes per depth of 16
+      uint32_t uses = 0;                       // of the one S buffer
+      auto scores = [&](int t, int st) {
+        if (uses > 0) ok = tc::mbar_wait(&sm.s_free, (uses - 1) & 1);
+        if (!ok) return;
+        uses++;
         tc::fence_after();
-        outputs(t, st, i == 0);
-        if (i + 1 < nkb) scores(t, nx);        // runs after the product that reads P, in the order of issue
+        const uint64_t qa = q0 + (uint32_t)t * (C::kQBytes >> 4), ka = k0 + (uint32_t)st * (C::kKBytes >> 4);
+#pragma unroll
+        for (int k = 0; k < D / 16; k++) pr::mma_ss(lead, tm, qa + k * 16, ka + k * 16, id_s, k > 0);
+        pr::commit(lead, &sm.s_full[t]);
+      };
+      auto outputs = [&](int t, int st, bool first) {
+        const uint64_t va = v0 + (uint32_t)st * (C::kKBytes >> 4);
+#pragma unroll
+        for (int k = 0; k < BK / 16; k++)
+          pr::mma_ts(lead, tm + C::kOCol + t * D, tm + C::kPCol + t * 64 + k * 8, va + k * 16, id_o, !first || k > 0);
+        pr::commit(lead, &sm.pv_done[t]);
+      };
+      if (nkb > 0) {
+        ok = tc::mbar_wait(&sm.k_full[0], 0);
+        for (int t = 0; t < ntile && ok; t++) scores(t, 0);
+        if (ok) pr::commit(lead, &sm.k_empty[0]);
       }
-      if (!ok) break;
-      tc::commit(&sm.v_empty[st]);
-      if (i + 1 < nkb) tc::commit(&sm.k_empty[nx]);
-    }
-    if (nkb > 0) tc::commit(&sm.o_full);
+      for (int i = 0; i < nkb && ok; i++) {
+        const int st = i & 1, nx = st ^ 1;
+        if (i + 1 < nkb) ok = tc::mbar_wait(&sm.k_full[nx], ((i + 1) >> 1) & 1);
+        if (ok) ok = tc::mbar_wait(&sm.v_full[st], (i >> 1) & 1);
+        for (int t = 0; t < ntile && ok; t++) {
+          if (i + 1 < nkb) scores(t, nx);      // under this tile's softmax
+          if (ok) ok = tc::mbar_wait(&sm.p_full[t], i & 1);
+          if (!ok) break;
+          tc::fence_after();
+          outputs(t, st, i == 0);
+        }
+        if (!ok) break;
+        pr::commit(lead, &sm.v_empty[st]);
+        if (i + 1 < nkb) pr::commit(lead, &sm.k_empty[nx]);
+      }
     }
   }
   __syncwarp();
