@@ -2,15 +2,14 @@
 // the tcgen05 tensor cores.  The mathematics and the layout of a batch are kv4_attend.cu's.
 //
 // A block takes two tiles of 128 rows ((token, head of the group) pairs of one K/V head; one
-// tile with D = 256) and walks over blocks of 128 (64) keys.  Per key block and tile
+// tile with D = 256) and walks over the keys.  Per step of 64 keys and tile
 //   S = Q K^T   f16 x f16 -> f32 in tensor memory,
-//   P = exp2(S c - m) as f16 in tensor memory (the A operand of the second product),
+//   P = exp2(S c - m), over S as f16 (the A operand of the second product),
 //   O += P V    f32 in tensor memory.
 // Roles: four warps convert keys and values from 4 bits into f16 operands in shared memory
 // (exact, kv4.cuh), once for both tiles; four warps per tile hold a row per thread and do the
-// softmax; one thread issues the products.  A row's scores go to registers at once, so the two
-// tiles share one S buffer and a tile's next scores are computed under its softmax; the order
-// of issue is S0' PV0 S1' PV1 (' = next key block).
+// softmax, 64 keys at a step; one warp issues the products.  Each tile has two S buffers, so its
+// next scores are computed under its softmax; the order of issue is S0' PV0 S1' PV1 (' = next step).
 //
 // The running maximum is only moved when a row's scores exceed it by 2^8 (P <= 256 in f16, sums
 // in f32): O is rescaled a few times per row, not per block.  Operands are
@@ -34,11 +33,12 @@ struct PromptArgs {
 };
 
 template <int D> struct PromptCfg {
-  static constexpr int BK = D == 256 ? 64 : 128;            // keys per block
+  static constexpr int BK = D == 256 ? 64 : 128;            // keys converted at a time
+  static constexpr int SK = 64, HALVES = BK / SK;           // keys of a softmax step: one page
   static constexpr int TILES = D == 256 ? 1 : 2;            // row tiles per block
-  static constexpr int kSoftWarps = 4 * TILES, kWarps = kSoftWarps + 8;   // + conversion, + products (one of four)
+  static constexpr int kSoftWarps = 4 * TILES, kWarps = kSoftWarps + 5;   // + conversion, + products
   static constexpr int kQBytes = 128 * D * 2, kKBytes = BK * D * 2;   // one operand tile; V's is K's size
-  static constexpr int kPCol = 128, kOCol = 256;            // tensor memory: S at 0, P of tile t at 128 + 64 t, O at 256 + D t
+  static constexpr int kOCol = 256;    // tensor memory: S of tile t and step n at 128 t + 64 (n & 1), P over it; O at 256 + D t
 };
 
 template <int D> struct PromptSmem {
@@ -47,7 +47,7 @@ template <int D> struct PromptSmem {
   uint8_t k[2][C::kKBytes];
   uint8_t v[2][C::kKBytes];
   float row_scale[C::TILES * 128];
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], s_free, p_full[2], pv_done[2];
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2], pv_done[2];
   uint32_t tmem;
 };
 
@@ -161,6 +161,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
   const int kb0 = a.window > 0 ? max(0, p_first - a.window + 1) / BK : 0;
   const int kb1 = p_last < 0 ? kb0 : p_last / BK + 1;              // key blocks [kb0, kb1)
   const int nkb = kb1 - kb0;
+  const int steps = nkb > 0 ? p_last / C::SK + 1 - kb0 * C::HALVES : 0;   // softmax steps
 
   // ---- queries as f16 operands (bf16 rows scaled to at most 512), barriers, tensor memory
   if (warp == 0) tc::tmem_alloc(&sm.tmem, 512);
@@ -170,11 +171,11 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
       tc::mbar_init(&sm.v_full[i], 128);
       tc::mbar_init(&sm.k_empty[i], 1);
       tc::mbar_init(&sm.v_empty[i], 1);
-      tc::mbar_init(&sm.s_full[i], 1);
+      tc::mbar_init(&sm.s_full[i][0], 1);
+      tc::mbar_init(&sm.s_full[i][1], 1);
       tc::mbar_init(&sm.p_full[i], 128);
       tc::mbar_init(&sm.pv_done[i], 1);
     }
-    tc::mbar_init(&sm.s_free, 128);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   for (int it = tid; it < TILES * 128 * 4; it += C::kWarps * 32) {   // kWarps * 32 is a multiple of 4: lanes stay together
@@ -224,35 +225,32 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
   const uint32_t tmem = sm.tmem;
   bool ok = true;
 
-  // Registers go where they are needed: the block starts with 128 a thread (512 threads) and ends with
-  // 256 x 168 + 128 x 104 + 128 x 72, the same sum.  (One tile: 384 threads start with 168.)
   if (warp < C::kSoftWarps) {
-    // ---- softmax: thread = row; its scores of a block all in registers
-    if constexpr (TILES == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+    // ---- softmax: thread = row; its scores of a step all in registers
     const int t = warp >> 2, r = t * 128 + (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_at = tmem + lanes, p_at = s_at + C::kPCol + t * 64, o_at = tmem + lanes + C::kOCol + t * D;
+    const uint32_t o_at = tmem + lanes + C::kOCol + t * D;
     const int row = row0 + r, p = p0 + min(row, rows - 1) / a.G;
     const int pt_first = p0 + (row0 + t * 128) / a.G, pt_last = p0 + min(row0 + t * 128 + 127, rows - 1) / a.G;
     const float cs = sm.row_scale[r];
     float m = -INFINITY, l = 0.f;
     if (t < ntile) {
-      for (int i = 0; i < nkb && ok; i++) {
-        const int j0 = (kb0 + i) * BK;
-        const bool edge = j0 + BK - 1 > pt_first || (a.window > 0 && j0 <= pt_last - a.window);
-        ok = tc::mbar_wait(&sm.s_full[t], i & 1);
+      for (int i = 0; i < steps && ok; i++) {
+        constexpr int SK = C::SK;
+        const int j0 = kb0 * BK + i * SK;
+        const uint32_t s_at = tmem + lanes + t * 128 + (i & 1) * SK;
+        const bool edge = j0 + SK - 1 > pt_first || (a.window > 0 && j0 <= pt_last - a.window);
+        ok = tc::mbar_wait(&sm.s_full[t][i & 1], (i >> 1) & 1);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         tc::fence_after();
-        uint32_t u[BK / 32][32];
+        uint32_t u[SK / 32][32];
 #pragma unroll
-        for (int c = 0; c < BK / 32; c++) pr::ld32(s_at + c * 32, u[c]);
+        for (int c = 0; c < SK / 32; c++) pr::ld32(s_at + c * 32, u[c]);
         tc::tmem_wait_ld();
-        tc::fence_before();
-        pr::arrive(&sm.s_free);              // the other tile's scores may come
         // the row's largest score; where it exceeds the reference by 2^8 (or there is none yet) the reference moves
         float top = -INFINITY, top1 = -INFINITY;
 #pragma unroll
-        for (int c = 0; c < BK / 32; c++) {
+        for (int c = 0; c < SK / 32; c++) {
           if (edge) hide<32>(u[c], j0 + c * 32, p, a.window);
 #pragma unroll
           for (int k = 0; k < 32; k += 4) {
@@ -263,16 +261,14 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
         top = fmaxf(top, top1);
         top *= cs;                           // cs >= 0; -inf stays (0 * -inf: NaN, which moves nothing)
         const bool move = m == -INFINITY ? top > -INFINITY : top > m + 8.f;
-        if (i > 0) {                         // the product before has read P and is in O
-          ok = tc::mbar_wait(&sm.pv_done[t], (i - 1) & 1);
-          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-          tc::fence_after();
-        }
         if (__any_sync(0xffffffffu, move)) {
           const float f = !move ? 1.f : m == -INFINITY ? 0.f : pr::exp2_fast(m - top);
           if (move) m = top;
           l *= f;
-          if (i > 0) {
+          if (i > 0) {                       // once the product before is in O
+            ok = tc::mbar_wait(&sm.pv_done[t], (i - 1) & 1);
+            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+            tc::fence_after();
 #pragma unroll 1
             for (int c = 0; c < D / 32; c++) {
               uint32_t u[32];
@@ -287,7 +283,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
         const float ref = m == -INFINITY ? 0.f : m;
         float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-        for (int c = 0; c < BK / 32; c++) {
+        for (int c = 0; c < SK / 32; c++) {
           uint32_t pk[16];
 #pragma unroll
           for (int k = 0; k < 32; k += 2) {
@@ -297,7 +293,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
             pr::add2(s0, s1, x, y);
             pk[k / 2] = pr::f16x2(x, y);
           }
-          pr::st16(p_at + c * 16, pk);
+          pr::st16(s_at + c * 16, pk);       // P takes the columns of the scores
         }
         l += s0 + s1;
         pr::wait_st();
@@ -306,7 +302,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
       }
       // ---- output
       if (nkb > 0 && ok) {
-        ok = tc::mbar_wait(&sm.pv_done[t], (nkb - 1) & 1);
+        ok = tc::mbar_wait(&sm.pv_done[t], (steps - 1) & 1);
         if (!__all_sync(0xffffffffu, ok)) ok = false;
       }
       if (ok) {
@@ -345,7 +341,6 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
     }
   } else if (warp < C::kSoftWarps + 4) {
     // ---- keys and values from 4 bits to f16 operands; codes are fetched a block ahead
-    if constexpr (TILES == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     const int dt = tid - C::kSoftWarps * 32;
     constexpr int KI = BK * 4 * L::NS / 128;                 // key pieces per thread: 4
     constexpr int W = L::SD / 32;                            // 32-bit words of a key piece
@@ -460,52 +455,52 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
       fetch_v(kb0 + i + 1);
     }
   } else {
-    if constexpr (TILES == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    if (warp == C::kSoftWarps + 4) {
-      // ---- products: the whole warp waits, one lane issues
-      const uint32_t lead = pr::elect();
-      const uint32_t id_s = pr::idesc_f16(128, BK), id_o = pr::idesc_f16(128, D);
-      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-      const uint64_t q0 = tc::smem_desc(tc::smem_addr(sm.q[0]), 128, kQSbo), k0 = tc::smem_desc(tc::smem_addr(sm.k[0]), 128, kKSbo),
-                     v0 = tc::smem_desc(tc::smem_addr(sm.v[0]), 128, kVSbo);
-      // a descriptor moves on by its address in 16-byte steps: 256 bytes per depth of 16
-      uint32_t uses = 0;                       // of the one S buffer
-      auto scores = [&](int t, int st) {
-        if (uses > 0) ok = tc::mbar_wait(&sm.s_free, (uses - 1) & 1);
-        if (!ok) return;
-        uses++;
-        tc::fence_after();
-        const uint64_t qa = q0 + (uint32_t)t * (C::kQBytes >> 4), ka = k0 + (uint32_t)st * (C::kKBytes >> 4);
+    // ---- products: the whole warp waits, one lane issues
+    const uint32_t lead = pr::elect();
+    const uint32_t id_s = pr::idesc_f16(128, C::SK), id_o = pr::idesc_f16(128, D);
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    const uint64_t q0 = tc::smem_desc(tc::smem_addr(sm.q[0]), 128, kQSbo), k0 = tc::smem_desc(tc::smem_addr(sm.k[0]), 128, kKSbo),
+                   v0 = tc::smem_desc(tc::smem_addr(sm.v[0]), 128, kVSbo);
+    // a descriptor moves on by its address in 16-byte steps: 256 bytes per depth of 16; a half is 64
+    // rows of K (8 groups) and 8 chunks of V's depth
+    auto scores = [&](int t, int n) {
+      const int st = n / C::HALVES & 1, half = n % C::HALVES;
+      const uint64_t qa = q0 + (uint32_t)t * (C::kQBytes >> 4);
+      const uint64_t ka = k0 + (uint32_t)st * (C::kKBytes >> 4) + (uint32_t)half * (8 * kKSbo >> 4);
 #pragma unroll
-        for (int k = 0; k < D / 16; k++) pr::mma_ss(lead, tm, qa + k * 16, ka + k * 16, id_s, k > 0);
-        pr::commit(lead, &sm.s_full[t]);
-      };
-      auto outputs = [&](int t, int st, bool first) {
-        const uint64_t va = v0 + (uint32_t)st * (C::kKBytes >> 4);
+      for (int k = 0; k < D / 16; k++) pr::mma_ss(lead, tm + t * 128 + (n & 1) * C::SK, qa + k * 16, ka + k * 16, id_s, k > 0);
+      pr::commit(lead, &sm.s_full[t][n & 1]);
+      if (t == ntile - 1 && half == C::HALVES - 1) pr::commit(lead, &sm.k_empty[st]);
+    };
+    auto outputs = [&](int t, int n) {
+      const int st = n / C::HALVES & 1, half = n % C::HALVES;
+      const uint64_t va = v0 + (uint32_t)st * (C::kKBytes >> 4) + (uint32_t)half * (8 * 128 >> 4);
 #pragma unroll
-        for (int k = 0; k < BK / 16; k++)
-          pr::mma_ts(lead, tm + C::kOCol + t * D, tm + C::kPCol + t * 64 + k * 8, va + k * 16, id_o, !first || k > 0);
-        pr::commit(lead, &sm.pv_done[t]);
-      };
-      if (nkb > 0) {
-        ok = tc::mbar_wait(&sm.k_full[0], 0);
-        for (int t = 0; t < ntile && ok; t++) scores(t, 0);
-        if (ok) pr::commit(lead, &sm.k_empty[0]);
-      }
-      for (int i = 0; i < nkb && ok; i++) {
-        const int st = i & 1, nx = st ^ 1;
-        if (i + 1 < nkb) ok = tc::mbar_wait(&sm.k_full[nx], ((i + 1) >> 1) & 1);
-        if (ok) ok = tc::mbar_wait(&sm.v_full[st], (i >> 1) & 1);
-        for (int t = 0; t < ntile && ok; t++) {
-          if (i + 1 < nkb) scores(t, nx);      // under this tile's softmax
-          if (ok) ok = tc::mbar_wait(&sm.p_full[t], i & 1);
+      for (int k = 0; k < C::SK / 16; k++)
+        pr::mma_ts(lead, tm + C::kOCol + t * D, tm + t * 128 + (n & 1) * C::SK + k * 8, va + k * 16, id_o, n > 0 || k > 0);
+      pr::commit(lead, &sm.pv_done[t]);
+      if (t == ntile - 1 && half == C::HALVES - 1) pr::commit(lead, &sm.v_empty[st]);
+    };
+    if (steps > 0) {
+      ok = tc::mbar_wait(&sm.k_full[0], 0);
+      tc::fence_after();
+      for (int t = 0; t < ntile && ok; t++) scores(t, 0);
+    }
+    for (int n = 0; n < steps && ok; n++) {
+      const int nx = n + 1, kb = n / C::HALVES, kx = nx / C::HALVES;
+      if (nx < steps && nx % C::HALVES == 0) ok = tc::mbar_wait(&sm.k_full[kx & 1], (kx >> 1) & 1);
+      if (ok && n % C::HALVES == 0) ok = tc::mbar_wait(&sm.v_full[kb & 1], (kb >> 1) & 1);
+      for (int t = 0; t < ntile && ok; t++) {
+        if (nx < steps) {                      // under this tile's softmax; its P of two steps before has been read
+          if (n > 0) ok = tc::mbar_wait(&sm.pv_done[t], (n - 1) & 1);
           if (!ok) break;
           tc::fence_after();
-          outputs(t, st, i == 0);
+          scores(t, nx);
         }
+        ok = tc::mbar_wait(&sm.p_full[t], n & 1);
         if (!ok) break;
-        pr::commit(lead, &sm.v_empty[st]);
-        if (i + 1 < nkb) pr::commit(lead, &sm.k_empty[nx]);
+        tc::fence_after();
+        outputs(t, n);
       }
     }
   }
