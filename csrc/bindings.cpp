@@ -110,25 +110,8 @@ void trellis_rot_out(torch::Tensor z, torch::Tensor eid, torch::Tensor sv, c10::
                      torch::Tensor out);
 void trellis_gemv(torch::Tensor xr, torch::Tensor trellis, torch::Tensor experts, torch::Tensor row_map,
                   torch::Tensor z, int64_t K, int64_t L, bool mad, double inv_rms, int64_t maxr);
-// kv4_cache.cu
-void kv4_append(torch::Tensor k, torch::Tensor v, torch::Tensor slots, torch::Tensor pages, torch::Tensor bounds,
-                torch::Tensor unit, int64_t k_exp, int64_t v_exp, torch::Tensor status);
-void kv4_read(torch::Tensor slots, torch::Tensor pages, int64_t k_exp, int64_t v_exp, torch::Tensor k, torch::Tensor v,
-              torch::Tensor status);
-// kv4_attend.cu
-std::tuple<int64_t, int64_t> kv4_attend_workspace(int64_t G, int64_t D, int64_t max_q, bool chosen);
-void kv4_attend(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_lens, torch::Tensor table, torch::Tensor pages,
-                c10::optional<torch::Tensor> sel, double scale, int64_t max_q, int64_t window, int64_t k_exp,
-                int64_t v_exp, torch::Tensor out, c10::optional<torch::Tensor> lse, torch::Tensor part,
-                torch::Tensor split, torch::Tensor status);
-// kv4_select.cu
-void kv4_select(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_lens, torch::Tensor table, torch::Tensor bounds,
-                torch::Tensor unit, int64_t max_q, int64_t first, int64_t last, torch::Tensor score,
-                torch::Tensor pages, torch::Tensor status);
-// kv4_prompt.cu
-void kv4_prompt(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_lens, torch::Tensor table, torch::Tensor pages,
-                double scale, int64_t max_q, int64_t window, int64_t k_exp, int64_t v_exp, torch::Tensor out,
-                c10::optional<torch::Tensor> lse, torch::Tensor status);
+// kv4_ops.cpp
+void register_kv4(pybind11::module& m);
 // hyper_conn.cu
 void hc_mix(torch::Tensor xs, c10::optional<torch::Tensor> upd, c10::optional<torch::Tensor> post,
             c10::optional<torch::Tensor> comb, c10::optional<torch::Tensor> fn, c10::optional<torch::Tensor> part);
@@ -164,6 +147,7 @@ void ws_gemm_fp8(torch::Tensor a, torch::Tensor sa, torch::Tensor w, torch::Tens
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   register_pack_io(m);
+  register_kv4(m);
 #ifdef MOET_SOURCE_FINGERPRINT
   m.attr("source_fingerprint") = MOET_SOURCE_FINGERPRINT;
 #endif
@@ -237,12 +221,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("trellis_rot_out", &trellis_rot_out, py::arg("z"), py::arg("eid"), py::arg("sv"), py::arg("scale"),
         py::arg("out"));
   m.def("trellis_gemv", &trellis_gemv);
-  m.def("kv4_append", &kv4_append);
-  m.def("kv4_read", &kv4_read);
-  m.def("kv4_select", &kv4_select);
-  m.def("kv4_attend_workspace", &kv4_attend_workspace);
-  m.def("kv4_attend", &kv4_attend);
-  m.def("kv4_prompt", &kv4_prompt);
   m.def("hc_mix", &hc_mix, py::arg("xs"), py::arg("upd") = py::none(), py::arg("post") = py::none(),
         py::arg("comb") = py::none(), py::arg("fn") = py::none(), py::arg("part") = py::none());
   m.def("hc_apply", &hc_apply, py::arg("xs"), py::arg("part"), py::arg("base"), py::arg("scale"), py::arg("eps"),

@@ -28,7 +28,6 @@ namespace moet {
 namespace kv4 {
 
 constexpr int kWarps = 4;
-constexpr int kMaxSeqs = 4096;
 
 struct AttendArgs {
   const void* q; long long q_tok; int q_head;
@@ -710,14 +709,13 @@ std::tuple<int64_t, int64_t> kv4_attend_workspace(int64_t G, int64_t D, int64_t 
   return {blocks * 2 * rt * (D + 2), blocks * kSplitInts};
 }
 
-void kv4_attend(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_lens, torch::Tensor table, torch::Tensor pages,
-                c10::optional<torch::Tensor> sel, double scale, int64_t max_q, int64_t window, int64_t k_exp,
-                int64_t v_exp, torch::Tensor out, c10::optional<torch::Tensor> lse, torch::Tensor part,
-                torch::Tensor split, torch::Tensor status) {
+void kv4_attend_launch(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_lens, torch::Tensor table,
+                       torch::Tensor pages, c10::optional<torch::Tensor> sel, double scale, int64_t max_q,
+                       int64_t window, int64_t k_exp, int64_t v_exp, torch::Tensor out,
+                       c10::optional<torch::Tensor> lse, torch::Tensor part, torch::Tensor split, torch::Tensor status) {
   const int T = (int)q.size(0), H = (int)pages.size(1), D = (int)(pages.size(2) / 72), G = (int)(q.size(1) / H);
   const int B = (int)seq_lens.size(0), W = (int)table.size(1);
   const bool chosen = sel.has_value() && sel->defined();
-  TORCH_CHECK(B <= kMaxSeqs, "kv4_attend: at most ", kMaxSeqs, " sequences, got ", B);
   const int nt = row_tiles(chosen ? G : max_q * G, D);
   AttendArgs a;
   a.q = q.data_ptr(); a.q_tok = q.stride(0); a.q_head = (int)q.stride(1);
@@ -733,7 +731,6 @@ void kv4_attend(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_lens, tor
   a.part = (float*)part.data_ptr(); a.split = (int*)split.data_ptr();
   a.min_units = kWarps;
   a.status = (int*)status.data_ptr();
-  if (T == 0 || B == 0) return;
   // the unit line is counted in 32 bits
   const int64_t line = chosen ? (int64_t)T * H * ((G + 8 * nt - 1) / (8 * nt)) * (a.budget + kTileCost)
                               : ((int64_t)T * G / (8 * nt) + B) * H * (W + kTileCost);

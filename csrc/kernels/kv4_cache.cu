@@ -322,39 +322,15 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(ReadArgs a) {
 
 static int dim_of(const torch::Tensor& pages) { return (int)(pages.size(2) / 72); }
 
-static void check_cache(const torch::Tensor& pages) {
-  TORCH_CHECK(pages.is_cuda() && pages.is_contiguous() && pages.scalar_type() == at::kByte && pages.dim() == 3,
-              "kv4: pages must be a contiguous uint8 CUDA tensor [pages, kv_heads, 72 * head_dim]");
-  const int D = dim_of(pages);
-  TORCH_CHECK(pages.size(2) == 72 * D && (D == 64 || D == 128 || D == 256), "kv4: head_dim must be 64, 128 or 256");
-}
-
-static void check_slots(const torch::Tensor& slots, const torch::Tensor& pages) {
-  TORCH_CHECK(slots.device() == pages.device() && slots.scalar_type() == at::kLong && slots.is_contiguous() &&
-                  slots.dim() == 1, "kv4: slots must be a contiguous int64 tensor [T] on the cache's device");
-}
-
 }  // namespace kv4
 }  // namespace moet
 
 using namespace moet;
 using namespace moet::kv4;
 
-void kv4_append(torch::Tensor k, torch::Tensor v, torch::Tensor slots, torch::Tensor pages, torch::Tensor bounds,
-                torch::Tensor unit, int64_t k_exp, int64_t v_exp, torch::Tensor status) {
-  check_cache(pages);
-  check_slots(slots, pages);
+void kv4_append_launch(torch::Tensor k, torch::Tensor v, torch::Tensor slots, torch::Tensor pages, torch::Tensor bounds,
+                       torch::Tensor unit, int64_t k_exp, int64_t v_exp, torch::Tensor status) {
   const int T = (int)slots.size(0), H = (int)pages.size(1), D = dim_of(pages);
-  for (const torch::Tensor* x : {&k, &v})
-    TORCH_CHECK(x->device() == pages.device() && x->dim() == 3 && x->size(0) == T && x->size(1) == H && x->size(2) == D &&
-                    (D == 1 || x->stride(2) == 1) &&
-                    (x->scalar_type() == at::kBFloat16 || x->scalar_type() == at::kHalf),
-                "kv4_append: k and v must be bf16 or f16 [T, kv_heads, head_dim] with unit inner stride");
-  TORCH_CHECK(k.scalar_type() == v.scalar_type(), "kv4_append: k and v must have one type");
-  TORCH_CHECK(bounds.is_contiguous() && bounds.scalar_type() == at::kChar && unit.is_contiguous() &&
-                  unit.scalar_type() == at::kFloat && bounds.numel() == pages.size(0) * H * 2 * D &&
-                  unit.numel() == pages.size(0) * H, "kv4_append: bounds / unit do not fit the cache");
-  if (T == 0) return;
   auto stream = at::cuda::getCurrentCUDAStream();
   AppendArgs a;
   a.k = {k.data_ptr(), k.stride(0), k.stride(1)};
@@ -388,18 +364,9 @@ void kv4_append(torch::Tensor k, torch::Tensor v, torch::Tensor slots, torch::Te
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
-void kv4_read(torch::Tensor slots, torch::Tensor pages, int64_t k_exp, int64_t v_exp, torch::Tensor k, torch::Tensor v,
-              torch::Tensor status) {
-  check_cache(pages);
-  check_slots(slots, pages);
+void kv4_read_launch(torch::Tensor slots, torch::Tensor pages, int64_t k_exp, int64_t v_exp, torch::Tensor k,
+                     torch::Tensor v, torch::Tensor status) {
   const int T = (int)slots.size(0), H = (int)pages.size(1), D = dim_of(pages);
-  for (const torch::Tensor* x : {&k, &v})
-    TORCH_CHECK(x->device() == pages.device() && x->is_contiguous() && x->numel() == (int64_t)T * H * D &&
-                    (x->scalar_type() == at::kBFloat16 || x->scalar_type() == at::kHalf) &&
-                    (uintptr_t)x->data_ptr() % 16 == 0,
-                "kv4_read: k and v must be contiguous bf16 or f16 [T, kv_heads, head_dim]");
-  TORCH_CHECK(k.scalar_type() == v.scalar_type(), "kv4_read: k and v must have one type");
-  if (T == 0) return;
   auto stream = at::cuda::getCurrentCUDAStream();
   ReadArgs a{(const long long*)slots.data_ptr(), T, H, pages.size(0) * kPage, (const uint8_t*)pages.data_ptr(),
              std::ldexp(1.f, (int)k_exp), std::ldexp(1.f, (int)v_exp), k.data_ptr(), v.data_ptr(),

@@ -521,9 +521,9 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
 using namespace moet;
 using namespace moet::kv4;
 
-void kv4_prompt(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_lens, torch::Tensor table, torch::Tensor pages,
-                double scale, int64_t max_q, int64_t window, int64_t k_exp, int64_t v_exp, torch::Tensor out,
-                c10::optional<torch::Tensor> lse, torch::Tensor status) {
+void kv4_prompt_launch(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_lens, torch::Tensor table,
+                       torch::Tensor pages, double scale, int64_t max_q, int64_t window, int64_t k_exp, int64_t v_exp,
+                       torch::Tensor out, c10::optional<torch::Tensor> lse, torch::Tensor status) {
   PromptArgs a;
   const int D = (int)(pages.size(2) / 72);
   a.T = (int)q.size(0); a.H = (int)pages.size(1); a.G = (int)(q.size(1) / a.H);
@@ -536,8 +536,7 @@ void kv4_prompt(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_lens, tor
   a.v_mul = std::ldexp(1.f, (int)v_exp);
   a.out = out.data_ptr(); a.lse = (float*)opt_ptr(lse);
   a.status = (int*)status.data_ptr();
-  if (a.T == 0 || a.B == 0) return;
-  TORCH_CHECK(a.B <= 65535 && a.H <= 65535, "kv4_prompt: too many sequences or heads");
+  TORCH_CHECK(a.H <= 65535, "kv4: too many heads");
   auto stream = at::cuda::getCurrentCUDAStream();
   auto go = [&](auto dim, auto t) {
     constexpr int DD = decltype(dim)::value;

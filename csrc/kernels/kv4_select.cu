@@ -274,9 +274,9 @@ __global__ void __launch_bounds__(kPickThreads) kv4_pick_kernel(SelectArgs a) {
 using namespace moet;
 using namespace moet::kv4;
 
-void kv4_select(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_lens, torch::Tensor table, torch::Tensor bounds,
-                torch::Tensor unit, int64_t max_q, int64_t first, int64_t last, torch::Tensor score,
-                torch::Tensor pages, torch::Tensor status) {
+void kv4_select_launch(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_lens, torch::Tensor table,
+                       torch::Tensor bounds, torch::Tensor unit, int64_t max_q, int64_t first, int64_t last,
+                       torch::Tensor score, torch::Tensor pages, torch::Tensor status) {
   SelectArgs a;
   const int D = (int)q.size(2);
   a.T = (int)q.size(0); a.H = (int)bounds.size(1); a.G = (int)(q.size(1) / a.H);
@@ -288,11 +288,6 @@ void kv4_select(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_lens, tor
   a.score = (float*)score.data_ptr(); a.first = (int)first; a.last = (int)last; a.budget = (int)pages.size(2);
   a.pages = (int*)pages.data_ptr();
   a.status = (int*)status.data_ptr();
-  TORCH_CHECK(a.G <= kScoreRows, "kv4_select: at most ", kScoreRows, " query heads per K/V head, got ", a.G);
-  TORCH_CHECK(first >= 0 && last >= 1 && first + last <= a.budget, "kv4_select: first + last pages exceed the budget");
-  TORCH_CHECK((a.W <= a.budget || score.numel() >= (int64_t)a.T * a.H * a.W) && pages.numel() == (int64_t)a.T * a.H * a.budget,
-              "kv4_select: score / pages do not fit the batch");
-  if (a.T == 0 || a.B == 0) return;
   a.gp = 1;
   while (a.gp < a.G && a.gp < 8) a.gp *= 2;
   if (a.G > 8) a.gp = (a.G + 7) / 8 * 8;
