@@ -104,12 +104,12 @@ constexpr int kTileCost = 8;
 // its own; a warp takes TS tokens per softmax step.
 template <int D, int NT> struct StepCfg {
   static constexpr int kSlots = D == 256 ? 2 : 3;                    // 2304, 4608 or 9216 bytes each
-  static constexpr int kRed = D == 256 ? 1 : 2;                      // buffers in which the warps are joined
+  static constexpr int kRed = D == 256 || NT == 2 ? 1 : 2;                     // buffers in which the warps are joined
   static constexpr int TS = NT == 1 ? 64 : 32;                       // as the registers allow
 };
 
 constexpr int kMaxBlocks = 4;       // blocks per SM, at most
-template <int D, int NT> constexpr int blocks_per_sm() { return D <= 128 && NT == 1 ? 3 : 2; }   // by registers
+template <int D, int NT> constexpr int blocks_per_sm() { return D <= 128 && NT <= 2 ? 3 : 2; }   // by registers
 
 template <int D, int NT> struct StepSmem {
   using C = StepCfg<D, NT>;

@@ -17,6 +17,8 @@
 #include "kv4.cuh"
 #include "torch_glue.h"
 
+#include <type_traits>
+
 namespace moet {
 namespace kv4 {
 
@@ -24,7 +26,7 @@ struct SelectArgs {
   const void* q; long long q_tok; int q_head;
   const int *cu_q, *seq_lens, *table; int B, W, T, H, G;
   int gp, tpc;                        // rows reserved per token (a power of two or a multiple of 8), tokens per block
-  int tiles, chunks;                  // token tiles per sequence, page chunks
+  int tiles, chunks, span;            // token tiles per sequence; chunks of 128 pages, in spans of so many per block
   const int8_t* bounds; const float* unit; int n_pages;
   float* score; int first, last, budget;
   int* pages;
@@ -57,15 +59,16 @@ __global__ void __launch_bounds__(kScoreWarps * 32) kv4_score_kernel(SelectArgs 
   __shared__ float unit_q[kScoreRows];
   pdl_entry();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int h = blockIdx.y, chunk = blockIdx.x % a.chunks, bt = blockIdx.x / a.chunks;
+  const int spans = (a.chunks + a.span - 1) / a.span;
+  const int h = blockIdx.y, chunk0 = blockIdx.x % spans * a.span, bt = blockIdx.x / spans;
   const int b = bt / a.tiles, tile = bt % a.tiles;
   int c0, nq, p0;
   seq_rows(a, b, c0, nq, p0);
   const int i0 = tile * a.tpc, ntok = min(a.tpc, nq - i0);
   if (ntok <= 0) return;
   const int end = rivals_end(a, p0 + i0 + ntok - 1);       // the last token's
-  const int page0 = chunk * (kScoreWarps * 16);
-  if (page0 >= end) return;
+  constexpr int kChunk = kScoreWarps * 16;
+  if (chunk0 * kChunk >= end) return;
   if (p0 + i0 + ntok - 1 < a.budget * kPage) return;       // every token takes all its pages
 
   // ---- rows: r = round(q / f) as [max(r, 0) | min(r, 0)]
@@ -76,10 +79,14 @@ __global__ void __launch_bounds__(kScoreWarps * 32) kv4_score_kernel(SelectArgs 
     const bool live = ti < ntok && gi < a.G;
     float v[E], amax = 0.f;
     if (live) {
+      T16 raw[E];
       const T16* p = (const T16*)a.q + (long long)(c0 + i0 + ti) * a.q_tok + (long long)(h * a.G + gi) * a.q_head + lane * E;
+      if constexpr (E == 8) *reinterpret_cast<uint4*>(raw) = *reinterpret_cast<const uint4*>(p);
+      else if constexpr (E == 4) *reinterpret_cast<uint2*>(raw) = *reinterpret_cast<const uint2*>(p);
+      else *reinterpret_cast<uint32_t*>(raw) = *reinterpret_cast<const uint32_t*>(p);
 #pragma unroll
       for (int e = 0; e < E; e++) {
-        float x = to_f32(p[e]);
+        float x = to_f32(raw[e]);
         x = x != x ? 0.f : fminf(fmaxf(x, -3.4028235e38f), 3.4028235e38f);
         v[e] = x;
         amax = fmaxf(amax, fabsf(x));
@@ -91,18 +98,23 @@ __global__ void __launch_bounds__(kScoreWarps * 32) kv4_score_kernel(SelectArgs 
     amax = warp_max(amax);
     const int ex = exp_for_127(amax);
     const float inv = pow2f(-ex);
+    int8_t pos[E], neg[E];
 #pragma unroll
     for (int e = 0; e < E; e++) {
       const int x = __float2int_rn(v[e] * inv);
-      rows[r * STRIDE + lane * E + e] = (int8_t)max(x, 0);
-      rows[r * STRIDE + D + lane * E + e] = (int8_t)min(x, 0);
+      pos[e] = (int8_t)max(x, 0);
+      neg[e] = (int8_t)min(x, 0);
     }
+    using Word = std::conditional_t<E == 8, uint2, std::conditional_t<E == 4, uint32_t, uint16_t>>;
+    *reinterpret_cast<Word*>(rows + r * STRIDE + lane * E) = *reinterpret_cast<const Word*>(pos);
+    *reinterpret_cast<Word*>(rows + r * STRIDE + D + lane * E) = *reinterpret_cast<const Word*>(neg);
     if (lane == 0) unit_q[r] = live ? pow2f(ex) : 0.f;
   }
   __syncthreads();
 
-  // ---- 16 pages per warp
-  const int pg = page0 + warp * 16;
+  // ---- 16 pages per warp and chunk
+  for (int chunk = chunk0; chunk < min(chunk0 + a.span, a.chunks); chunk++) {
+  const int pg = chunk * kChunk + warp * 16;
   if (pg >= end) return;
   uint4 x[2][CH];
   float u[2];
@@ -176,6 +188,7 @@ __global__ void __launch_bounds__(kScoreWarps * 32) kv4_score_kernel(SelectArgs 
       }
     }
   }
+  }
 }
 
 MOET_DEVICE uint32_t order_bits(float f) {
@@ -183,7 +196,102 @@ MOET_DEVICE uint32_t order_bits(float f) {
   return u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u);
 }
 
+// The row's sequence, first row, position and pages; the choice when all pages fit, and the pages that are always taken.
+struct Pick {
+  int n, end, want;         // pages; rivals are [first, end), `want` of them are taken (more than that: n > budget)
+  int* out;
+};
+MOET_DEVICE Pick pick_row(const SelectArgs& a, int tok, int h, int tid, int threads) {
+  int lo = 0, hi = a.B;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (max(0, min(a.cu_q[mid], a.T)) <= tok) lo = mid; else hi = mid;
+  }
+  int c0, nq, p0;
+  seq_rows(a, lo, c0, nq, p0);
+  const int p = tok - c0 < nq ? p0 + tok - c0 : -1;
+  Pick r;
+  r.n = p < 0 ? 0 : p / kPage + 1;
+  r.out = a.pages + ((long long)tok * a.H + h) * a.budget;
+  r.end = r.n - a.last;
+  r.want = 0;
+  if (r.n <= a.budget) {
+    for (int i = tid; i < a.budget; i += threads) r.out[i] = i < r.n ? i : -1;
+    return r;
+  }
+  r.want = a.budget - a.first - a.last;
+  for (int i = tid; i < a.first; i += threads) r.out[i] = i;
+  for (int i = tid; i < a.last; i += threads) r.out[a.budget - a.last + i] = r.end + i;
+  return r;
+}
+
+// A warp per (token, head), its keys in registers: up to 32 K pages.  The threshold is found bit by
+// bit from the highest bit in which the keys differ, and stops as soon as just `want` keys reach it.
+template <int K>
+__global__ void __launch_bounds__(128) kv4_pick_warp_kernel(SelectArgs a) {
+  pdl_entry();
+  const int lane = threadIdx.x & 31;
+  const long long id = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (id >= (long long)a.T * a.H) return;
+  const int tok = (int)(id / a.H), h = (int)(id % a.H);
+  const Pick r = pick_row(a, tok, h, lane, 32);
+  if (r.want == 0) return;
+  const float* row = a.score + id * a.W;
+  uint32_t key[K], top = 0, low = 0xFFFFFFFFu;
+#pragma unroll
+  for (int k = 0; k < K; k++) {
+    const int i = a.first + 32 * k + lane;
+    key[k] = i < r.end ? order_bits(__ldg(row + i)) : 0;       // 0 lies below every score
+    if (i < r.end) top = max(top, key[k]), low = min(low, key[k]);
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  low = __reduce_min_sync(0xffffffffu, low);
+  uint32_t t = top;
+  int above = -1;                                              // keys >= t, once that is known to be `want`
+  if (top != low) {
+    int bit = 31 - __clz(top ^ low);
+    t = top >> bit >> 1 << bit << 1;                           // the bits they share
+    for (; bit >= 0; bit--) {
+      const uint32_t cand = t | 1u << bit;
+      int n = 0;
+#pragma unroll
+      for (int k = 0; k < K; k++) n += key[k] >= cand;
+      n = __reduce_add_sync(0xffffffffu, n);
+      if (n >= r.want) t = cand;
+      if (n == r.want) {
+        above = n;
+        break;
+      }
+    }
+  }
+  int ties = 0;                                                // places for keys that equal t
+  if (above < 0) {
+    int n = 0;
+#pragma unroll
+    for (int k = 0; k < K; k++) n += key[k] > t;
+    ties = r.want - __reduce_add_sync(0xffffffffu, n);
+  }
+  int at = a.first;
+  const uint32_t below = (1u << lane) - 1;
+#pragma unroll
+  for (int k = 0; k < K; k++) {
+    const int i = a.first + 32 * k + lane;
+    bool take = i < r.end && (above >= 0 ? key[k] >= t : key[k] > t);
+    if (ties > 0) {
+      const bool eq = i < r.end && key[k] == t;
+      const uint32_t be = __ballot_sync(0xffffffffu, eq);
+      take |= eq && __popc(be & below) < ties;
+      ties -= min(ties, __popc(be));
+    }
+    const uint32_t b = __ballot_sync(0xffffffffu, take);
+    if (take) r.out[at + __popc(b & below)] = i;
+    at += __popc(b);
+  }
+}
+
 constexpr int kPickThreads = 128;
+
+// A block per (token, head) for longer rows: four passes of a radix search over the row in memory.
 
 __global__ void __launch_bounds__(kPickThreads) kv4_pick_kernel(SelectArgs a) {
   pdl_entry();
@@ -193,22 +301,9 @@ __global__ void __launch_bounds__(kPickThreads) kv4_pick_kernel(SelectArgs a) {
   __shared__ int remain_s;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int tok = blockIdx.x / a.H, h = blockIdx.x % a.H;
-  int lo = 0, hi = a.B;                                    // the token's sequence
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (max(0, min(a.cu_q[mid], a.T)) <= tok) lo = mid; else hi = mid;
-  }
-  int c0, nq, p0;
-  seq_rows(a, lo, c0, nq, p0);
-  const int p = tok - c0 < nq ? p0 + tok - c0 : -1, n = p < 0 ? 0 : p / kPage + 1;
-  int* out = a.pages + ((long long)tok * a.H + h) * a.budget;
-  if (n <= a.budget) {
-    for (int i = tid; i < a.budget; i += kPickThreads) out[i] = i < n ? i : -1;
-    return;
-  }
-  const int end = n - a.last, want = a.budget - a.first - a.last;   // rivals: [first, end), more than `want`
-  for (int i = tid; i < a.first; i += kPickThreads) out[i] = i;
-  for (int i = tid; i < a.last; i += kPickThreads) out[a.budget - a.last + i] = end + i;
+  const Pick r = pick_row(a, tok, h, tid, kPickThreads);
+  const int end = r.end, want = r.want;
+  int* out = r.out;
   if (want == 0) return;
   const float* row = a.score + ((long long)tok * a.H + h) * a.W;
   uint32_t prefix = 0, mask = 0;
@@ -294,7 +389,10 @@ void kv4_select_launch(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_le
   a.tpc = kScoreRows / a.gp;
   a.tiles = (int)((std::min<int64_t>(max_q, a.T) + a.tpc - 1) / a.tpc);
   a.chunks = (a.W + kScoreWarps * 16 - 1) / (kScoreWarps * 16);
-  const int64_t blocks = (int64_t)a.B * a.tiles * a.chunks;
+  // As many chunks per block as leave four blocks per SM: a block converts its rows once per span.
+  const int64_t per_chunk = (int64_t)a.B * a.tiles * a.H;
+  a.span = (int)std::max<int64_t>(1, std::min<int64_t>(a.chunks, per_chunk * a.chunks / (4 * 148)));
+  const int64_t blocks = (int64_t)a.B * a.tiles * ((a.chunks + a.span - 1) / a.span);
   TORCH_CHECK(blocks < (int64_t)1 << 31 && (int64_t)a.T * a.H < (int64_t)1 << 31, "kv4_select: too much work for one call");
   auto stream = at::cuda::getCurrentCUDAStream();
   const dim3 grid((unsigned)blocks, a.H), block(kScoreWarps * 32);
@@ -308,6 +406,10 @@ void kv4_select_launch(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_le
     else if (D == 128) go(std::integral_constant<int, 128>{});
     else go(std::integral_constant<int, 256>{});
   }
-  launch_k(kv4_pick_kernel, dim3((unsigned)((int64_t)a.T * a.H)), dim3(kPickThreads), 0, stream, a);
+  const dim3 warps((unsigned)(((int64_t)a.T * a.H + 3) / 4)), four(128);
+  if (a.W <= 256) launch_k(kv4_pick_warp_kernel<8>, warps, four, 0, stream, a);
+  else if (a.W <= 512) launch_k(kv4_pick_warp_kernel<16>, warps, four, 0, stream, a);
+  else if (a.W <= 1024) launch_k(kv4_pick_warp_kernel<32>, warps, four, 0, stream, a);
+  else launch_k(kv4_pick_kernel, dim3((unsigned)((int64_t)a.T * a.H)), dim3(kPickThreads), 0, stream, a);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
