@@ -51,10 +51,15 @@ MOET_DEVICE void seq_rows(const SelectArgs& a, int b, int& c0, int& nq, int& p0)
 // pages of a row at position p that compete for a place: [first, n - last), n = p / 64 + 1
 MOET_DEVICE int rivals_end(const SelectArgs& a, int p) { return p < 0 ? 0 : p / kPage + 1 - a.last; }
 
-template <int D, typename T16>
+// d as a float without the conversion pipe: |d| <= 256 * 127^2 < 2^22
+MOET_DEVICE float small_int(int d) { return __int_as_float(0x4B400000 + d) - 12582912.f; }
+
+// GP: rows reserved per token, 1, 2, 4 or 8; 16 stands for a multiple of 8 (a.gp).
+template <int D, int GP, typename T16>
 __global__ void __launch_bounds__(kScoreWarps * 32) kv4_score_kernel(SelectArgs a) {
   constexpr int KB = 2 * D, STRIDE = KB + 64;       // rows 64 bytes apart in the banks: 16-byte reads do not meet
   constexpr int CH = KB / 64;                       // 16-byte pieces of a lane per page
+  constexpr int kChunk = kScoreWarps * 16;
   __shared__ __align__(16) int8_t rows[kScoreRows * STRIDE];
   __shared__ float unit_q[kScoreRows];
   pdl_entry();
@@ -67,33 +72,49 @@ __global__ void __launch_bounds__(kScoreWarps * 32) kv4_score_kernel(SelectArgs 
   const int i0 = tile * a.tpc, ntok = min(a.tpc, nq - i0);
   if (ntok <= 0) return;
   const int end = rivals_end(a, p0 + i0 + ntok - 1);       // the last token's
-  constexpr int kChunk = kScoreWarps * 16;
   if (chunk0 * kChunk >= end) return;
   if (p0 + i0 + ntok - 1 < a.budget * kPage) return;       // every token takes all its pages
 
-  // ---- rows: r = round(q / f) as [max(r, 0) | min(r, 0)]
-  const int nrows = ntok * a.gp;
+  // 16 pages per warp and chunk; the first ones come while the rows are converted
+  uint4 x[2][CH];
+  float u[2];
+  auto fetch = [&](int pg) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const int page = pg + g + 8 * i;
+      int phys = 0;
+      if (page < end) {                                    // end <= W
+        phys = a.table[(long long)b * a.W + page];
+        if (phys < 0 || phys >= a.n_pages) {
+          set_status(a.status, kBadIndex);
+          phys = 0;
+        }
+      }
+      const int8_t* p = a.bounds + ((long long)phys * a.H + h) * KB + t * 16;
+#pragma unroll
+      for (int c = 0; c < CH; c++) x[i][c] = *reinterpret_cast<const uint4*>(p + c * 64);
+      u[i] = a.unit[(long long)phys * a.H + h];
+    }
+  };
+  fetch(chunk0 * kChunk + warp * 16);
+
+  // ---- rows: r = round(q / f) as [max(r, 0) | min(r, 0)]; a place without a row repeats the token's first
+  const int gp = GP == 16 ? a.gp : GP, nrows = ntok * gp;
   constexpr int E = D / 32;                                // values per lane
   for (int r = warp; r < ((nrows + 7) & ~7); r += kScoreWarps) {
-    const int ti = r / a.gp, gi = r % a.gp;
-    const bool live = ti < ntok && gi < a.G;
+    const int ti = min(r / gp, ntok - 1), gi = r % gp < a.G ? r % gp : 0;
     float v[E], amax = 0.f;
-    if (live) {
-      T16 raw[E];
-      const T16* p = (const T16*)a.q + (long long)(c0 + i0 + ti) * a.q_tok + (long long)(h * a.G + gi) * a.q_head + lane * E;
-      if constexpr (E == 8) *reinterpret_cast<uint4*>(raw) = *reinterpret_cast<const uint4*>(p);
-      else if constexpr (E == 4) *reinterpret_cast<uint2*>(raw) = *reinterpret_cast<const uint2*>(p);
-      else *reinterpret_cast<uint32_t*>(raw) = *reinterpret_cast<const uint32_t*>(p);
+    T16 raw[E];
+    const T16* p = (const T16*)a.q + (long long)(c0 + i0 + ti) * a.q_tok + (long long)(h * a.G + gi) * a.q_head + lane * E;
+    if constexpr (E == 8) *reinterpret_cast<uint4*>(raw) = *reinterpret_cast<const uint4*>(p);
+    else if constexpr (E == 4) *reinterpret_cast<uint2*>(raw) = *reinterpret_cast<const uint2*>(p);
+    else *reinterpret_cast<uint32_t*>(raw) = *reinterpret_cast<const uint32_t*>(p);
 #pragma unroll
-      for (int e = 0; e < E; e++) {
-        float x = to_f32(raw[e]);
-        x = x != x ? 0.f : fminf(fmaxf(x, -3.4028235e38f), 3.4028235e38f);
-        v[e] = x;
-        amax = fmaxf(amax, fabsf(x));
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; e++) v[e] = 0.f;
+    for (int e = 0; e < E; e++) {
+      float y = to_f32(raw[e]);
+      y = y != y ? 0.f : fminf(fmaxf(y, -3.4028235e38f), 3.4028235e38f);
+      v[e] = y;
+      amax = fmaxf(amax, fabsf(y));
     }
     amax = warp_max(amax);
     const int ex = exp_for_127(amax);
@@ -101,93 +122,75 @@ __global__ void __launch_bounds__(kScoreWarps * 32) kv4_score_kernel(SelectArgs 
     int8_t pos[E], neg[E];
 #pragma unroll
     for (int e = 0; e < E; e++) {
-      const int x = __float2int_rn(v[e] * inv);
-      pos[e] = (int8_t)max(x, 0);
-      neg[e] = (int8_t)min(x, 0);
+      const int y = __float2int_rn(v[e] * inv);
+      pos[e] = (int8_t)max(y, 0);
+      neg[e] = (int8_t)min(y, 0);
     }
     using Word = std::conditional_t<E == 8, uint2, std::conditional_t<E == 4, uint32_t, uint16_t>>;
     *reinterpret_cast<Word*>(rows + r * STRIDE + lane * E) = *reinterpret_cast<const Word*>(pos);
     *reinterpret_cast<Word*>(rows + r * STRIDE + D + lane * E) = *reinterpret_cast<const Word*>(neg);
-    if (lane == 0) unit_q[r] = live ? pow2f(ex) : 0.f;
+    if (lane == 0) unit_q[r] = pow2f(ex);
   }
   __syncthreads();
 
-  // ---- 16 pages per warp and chunk
-  for (int chunk = chunk0; chunk < min(chunk0 + a.span, a.chunks); chunk++) {
-  const int pg = chunk * kChunk + warp * 16;
-  if (pg >= end) return;
-  uint4 x[2][CH];
-  float u[2];
+  const int wide = gp / 8;                                 // n-tiles of one token, GP = 16
+  const int ntiles = (nrows + 7) / 8, chunk1 = min(chunk0 + a.span, a.chunks);
+  const long long tstep = (long long)a.H * a.W;
+  for (int chunk = chunk0; chunk < chunk1; chunk++) {
+    const int pg = chunk * kChunk + warp * 16;
+    if (pg >= end) return;
+    if (chunk > chunk0) fetch(pg);
+    const bool in0 = pg + g < end, in1 = pg + g + 8 < end;
+    float* out = a.score + ((long long)(c0 + i0) * a.H + h) * a.W + pg + g;     // + token * H * W
+    float best0 = -INFINITY, best1 = -INFINITY;
+    int left = wide, ti = GP == 1 ? 2 * t : GP == 2 ? t : GP == 4 ? t >> 1 : 0;   // this lane's token in the n-tile
+    out += ti * tstep;
+    for (int n = 0; n < ntiles; n++) {
+      int d[4] = {0, 0, 0, 0};
+      const int8_t* rp = rows + (n * 8 + g) * STRIDE + t * 16;
 #pragma unroll
-  for (int i = 0; i < 2; i++) {
-    const int page = pg + g + 8 * i;
-    int phys = 0;
-    if (page < end) {                                      // end <= W
-      phys = a.table[(long long)b * a.W + page];
-      if (phys < 0 || phys >= a.n_pages) {
-        set_status(a.status, kBadIndex);
-        phys = 0;
+      for (int c = 0; c < CH; c++) {
+        const uint4 y = *reinterpret_cast<const uint4*>(rp + c * 64);
+        mma_s8_16832(d, x[0][c].x, x[1][c].x, x[0][c].y, x[1][c].y, y.x, y.y);
+        mma_s8_16832(d, x[0][c].z, x[1][c].z, x[0][c].w, x[1][c].w, y.z, y.w);
       }
-    }
-    const int8_t* p = a.bounds + ((long long)phys * a.H + h) * KB + t * 16;
-#pragma unroll
-    for (int c = 0; c < CH; c++) x[i][c] = *reinterpret_cast<const uint4*>(p + c * 64);
-    u[i] = a.unit[(long long)phys * a.H + h];
-  }
-  const int wide = (a.gp + 7) / 8;                         // n-tiles of one token
-  float best[2] = {-INFINITY, -INFINITY};
-  const int ntiles = (nrows + 7) / 8;
-  for (int n = 0; n < ntiles; n++) {
-    int d[4] = {0, 0, 0, 0};
-    const int8_t* rp = rows + (n * 8 + g) * STRIDE + t * 16;
-#pragma unroll
-    for (int c = 0; c < CH; c++) {
-      const uint4 y = *reinterpret_cast<const uint4*>(rp + c * 64);
-      mma_s8_16832(d, x[0][c].x, x[1][c].x, x[0][c].y, x[1][c].y, y.x, y.y);
-      mma_s8_16832(d, x[0][c].z, x[1][c].z, x[0][c].w, x[1][c].w, y.z, y.w);
-    }
-    const int r0 = n * 8 + 2 * t;
-    const float f0 = unit_q[r0], f1 = unit_q[r0 + 1];
-    float s[4];                                            // (page g, row 2t), (g, 2t+1), (g + 8, 2t), (g + 8, 2t + 1)
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-      const float f = (k & 1) ? f1 : f0;
-      s[k] = f > 0.f ? (float)d[k] * f * u[k >> 1] : -INFINITY;
-    }
-    float* out = a.score + ((long long)(c0 + i0) * a.H + h) * a.W;       // + token * H * W + page
-    const long long tstep = (long long)a.H * a.W;
-    if (a.gp == 1) {
-#pragma unroll
-      for (int k = 0; k < 4; k++) {
-        const int ti = r0 + (k & 1), page = pg + g + 8 * (k >> 1);
-        if (ti < ntok && page < end) out[ti * tstep + page] = s[k];
+      const float2 f = *reinterpret_cast<const float2*>(&unit_q[n * 8 + 2 * t]);
+      // (page g, row 2t), (g, 2t+1), (g + 8, 2t), (g + 8, 2t + 1); the page's unit is positive and comes last
+      float m0 = small_int(d[0]) * f.x, m1 = small_int(d[2]) * f.x;
+      const float s0 = small_int(d[1]) * f.y, s1 = small_int(d[3]) * f.y;
+      if constexpr (GP == 1) {
+        if (ti < ntok) {
+          if (in0) out[0] = m0 * u[0];
+          if (in1) out[8] = m1 * u[1];
+        }
+        if (ti + 1 < ntok) {
+          if (in0) out[tstep] = s0 * u[0];
+          if (in1) out[tstep + 8] = s1 * u[1];
+        }
+        ti += 8, out += 8 * tstep;
+        continue;
       }
-      continue;
-    }
-    float m[2] = {fmaxf(s[0], s[1]), fmaxf(s[2], s[3])};
-    if (a.gp >= 4) {
-#pragma unroll
-      for (int i = 0; i < 2; i++) m[i] = fmaxf(m[i], __shfl_xor_sync(0xffffffffu, m[i], 1));
-    }
-    if (a.gp >= 8) {
-#pragma unroll
-      for (int i = 0; i < 2; i++) {
-        m[i] = fmaxf(m[i], __shfl_xor_sync(0xffffffffu, m[i], 2));
-        best[i] = fmaxf(best[i], m[i]);
-        m[i] = best[i];
+      m0 = fmaxf(m0, s0), m1 = fmaxf(m1, s1);
+      if constexpr (GP >= 4) {
+        m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, 1));
+        m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, 1));
       }
-      if (n % wide != wide - 1) continue;                  // the token goes on in the next tile
-      best[0] = best[1] = -INFINITY;
-    }
-    const int ti = r0 / a.gp;
-    if (r0 % a.gp == 0 || (a.gp > 8 && t == 0)) {
-#pragma unroll
-      for (int i = 0; i < 2; i++) {
-        const int page = pg + g + 8 * i;
-        if (ti < ntok && page < end) out[ti * tstep + page] = m[i];
+      if constexpr (GP >= 8) {
+        m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, 2));
+        m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, 2));
       }
+      if constexpr (GP == 16) {
+        m0 = best0 = fmaxf(best0, m0);
+        m1 = best1 = fmaxf(best1, m1);
+        if (--left > 0) continue;                          // the token goes on in the next n-tile
+        left = wide, best0 = best1 = -INFINITY;
+      }
+      const bool mine = ti < ntok && (GP == 2 || (GP == 4 ? (t & 1) == 0 : t == 0));
+      if (mine && in0) out[0] = m0 * u[0];
+      if (mine && in1) out[8] = m1 * u[1];
+      constexpr int kTok = GP == 2 ? 4 : GP == 4 ? 2 : 1;   // tokens of an n-tile
+      ti += kTok, out += kTok * tstep;
     }
-  }
   }
 }
 
@@ -396,10 +399,19 @@ void kv4_select_launch(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_le
   TORCH_CHECK(blocks < (int64_t)1 << 31 && (int64_t)a.T * a.H < (int64_t)1 << 31, "kv4_select: too much work for one call");
   auto stream = at::cuda::getCurrentCUDAStream();
   const dim3 grid((unsigned)blocks, a.H), block(kScoreWarps * 32);
+  auto launch = [&](auto dim, auto gp, auto t) {
+    launch_k(kv4_score_kernel<decltype(dim)::value, decltype(gp)::value, decltype(t)>, grid, block, 0, stream, a);
+  };
+  auto by_type = [&](auto dim, auto gp) {
+    if (q.scalar_type() == at::kHalf) launch(dim, gp, __half{});
+    else launch(dim, gp, __nv_bfloat16{});
+  };
   auto go = [&](auto dim) {
-    constexpr int DD = decltype(dim)::value;
-    if (q.scalar_type() == at::kHalf) launch_k(kv4_score_kernel<DD, __half>, grid, block, 0, stream, a);
-    else launch_k(kv4_score_kernel<DD, __nv_bfloat16>, grid, block, 0, stream, a);
+    if (a.gp == 1) by_type(dim, std::integral_constant<int, 1>{});
+    else if (a.gp == 2) by_type(dim, std::integral_constant<int, 2>{});
+    else if (a.gp == 4) by_type(dim, std::integral_constant<int, 4>{});
+    else if (a.gp == 8) by_type(dim, std::integral_constant<int, 8>{});
+    else by_type(dim, std::integral_constant<int, 16>{});
   };
   if (a.W > a.budget) {               // else every token takes all its pages
     if (D == 64) go(std::integral_constant<int, 64>{});
