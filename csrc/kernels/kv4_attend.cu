@@ -734,7 +734,7 @@ void kv4_attend_launch(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_le
   // the unit line is counted in 32 bits
   const int64_t line = chosen ? (int64_t)T * H * ((G + 8 * nt - 1) / (8 * nt)) * (a.budget + kTileCost)
                               : ((int64_t)T * G / (8 * nt) + B) * H * (W + kTileCost);
-  TORCH_CHECK(line < (int64_t)1 << 31, "kv4_attend: too much work for one call (", line, " units)");
+  TORCH_CHECK(line < (int64_t)1 << 31, "kv4: too much work for one call");
   auto stream = at::cuda::getCurrentCUDAStream();
   auto go = [&](auto dim, auto n, auto t) {
     constexpr int DD = decltype(dim)::value, NT = decltype(n)::value;

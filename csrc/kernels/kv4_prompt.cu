@@ -205,7 +205,8 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
       const int e = amax > 0.f ? max(-110, min(110, (int)(__float_as_uint(amax) >> 23) - 127 - 8)) : 0;
       mul = pow2f(-e), back = pow2f(e);
     }
-    if (t == 0) sm.row_scale[r] = back * fabsf(a.scale_log2);     // the scale's sign goes to the row: scores only grow
+    // the scale's sign goes to the row, so that scores only grow; above 0, so that -inf stays what it is
+    if (t == 0) sm.row_scale[r] = fmaxf(back * fabsf(a.scale_log2), 1e-30f);
     mul = copysignf(mul, a.scale_log2);
     uint8_t* dst = sm.q[r >> 7] + ((r & 127) >> 3) * kQSbo + (r & 7) * 16;
 #pragma unroll
@@ -233,7 +234,8 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
     const int row = row0 + r, p = p0 + min(row, rows - 1) / a.G;
     const int pt_first = p0 + (row0 + t * 128) / a.G, pt_last = p0 + min(row0 + t * 128 + 127, rows - 1) / a.G;
     const float cs = sm.row_scale[r];
-    float m = -INFINITY, l = 0.f;
+    // the reference is the product m + rest, exactly: the largest score's own difference is 0 at any size
+    float m = -INFINITY, rest = 0.f, l = 0.f;
     if (t < ntile) {
       for (int i = 0; i < steps && ok; i++) {
         constexpr int SK = C::SK;
@@ -259,11 +261,12 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
           }
         }
         top = fmaxf(top, top1);
-        top *= cs;                           // cs >= 0; -inf stays (0 * -inf: NaN, which moves nothing)
+        const float raw = top;
+        top *= cs;
         const bool move = m == -INFINITY ? top > -INFINITY : top > m + 8.f;
         if (__any_sync(0xffffffffu, move)) {
           const float f = !move ? 1.f : m == -INFINITY ? 0.f : pr::exp2_fast(m - top);
-          if (move) m = top;
+          if (move) m = top, rest = __fmaf_rn(raw, cs, -top);
           l *= f;
           if (i > 0) {                       // once the product before is in O
             ok = tc::mbar_wait(&sm.pv_done[t], (i - 1) & 1);
@@ -289,6 +292,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
           for (int k = 0; k < 32; k += 2) {
             float x = __uint_as_float(u[c][k]), y = __uint_as_float(u[c][k + 1]);
             pr::fma2(x, y, cs, -ref);
+            pr::add2(x, y, -rest, -rest);
             x = pr::exp2_fast(x), y = pr::exp2_fast(y);
             pr::add2(s0, s1, x, y);
             pk[k / 2] = pr::f16x2(x, y);

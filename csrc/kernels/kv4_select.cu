@@ -396,7 +396,7 @@ void kv4_select_launch(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_le
   const int64_t per_chunk = (int64_t)a.B * a.tiles * a.H;
   a.span = (int)std::max<int64_t>(1, std::min<int64_t>(a.chunks, per_chunk * a.chunks / (4 * 148)));
   const int64_t blocks = (int64_t)a.B * a.tiles * ((a.chunks + a.span - 1) / a.span);
-  TORCH_CHECK(blocks < (int64_t)1 << 31 && (int64_t)a.T * a.H < (int64_t)1 << 31, "kv4_select: too much work for one call");
+  TORCH_CHECK(blocks < (int64_t)1 << 31 && (int64_t)a.T * a.H < (int64_t)1 << 31, "kv4: too much work for one call");
   auto stream = at::cuda::getCurrentCUDAStream();
   const dim3 grid((unsigned)blocks, a.H), block(kScoreWarps * 32);
   auto launch = [&](auto dim, auto gp, auto t) {

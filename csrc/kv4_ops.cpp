@@ -6,6 +6,7 @@
 
 #include <map>
 #include <mutex>
+#include <string>
 
 using at::Tensor;
 using c10::optional;
@@ -27,6 +28,10 @@ namespace {
 struct Cache {
   int64_t n, H, D;
 };
+
+// Numbers enter a message as text: a stream that formats them itself crashes where the interpreter's
+// C++ runtime and this module's have different locale tables.
+std::string num(int64_t x) { return std::to_string(x); }
 
 Cache check_cache(const Tensor& pages, const Tensor& bounds, const Tensor& unit, const Tensor& status, int64_t k_exp,
                   int64_t v_exp) {
@@ -57,17 +62,17 @@ void check_slots(const Tensor& slots, const Tensor& pages) {
 int64_t check_batch(Tensor& q, const Tensor& cu_q, const Tensor& seq_lens, const Tensor& table, const Tensor& pages,
                     const Cache& c, int64_t& max_q) {
   TORCH_CHECK(q.device() == pages.device() && half_type(q) && q.dim() == 3 && q.size(2) == c.D,
-              "kv4: q must be bf16 or f16 [rows, heads, ", c.D, "] on the cache's device");
-  TORCH_CHECK(q.size(1) >= c.H && q.size(1) % c.H == 0, "kv4: q's heads must be a multiple of the ", c.H, " K/V heads");
+              "kv4: q must be bf16 or f16 [rows, heads, ", num(c.D), "] on the cache's device");
+  TORCH_CHECK(q.size(1) >= c.H && q.size(1) % c.H == 0, "kv4: q's heads must be a multiple of the ", num(c.H), " K/V heads");
   const auto int32_on = [&](const Tensor& x, int64_t dim) {
     return x.device() == pages.device() && x.scalar_type() == at::kInt && x.dim() == dim && x.is_contiguous();
   };
   TORCH_CHECK(int32_on(seq_lens, 1) && seq_lens.size(0) <= 4096,
               "kv4: seq_lens must be a contiguous int32 tensor of at most 4096 sequences on the cache's device");
   const int64_t B = seq_lens.size(0);
-  TORCH_CHECK(int32_on(cu_q, 1) && cu_q.size(0) == B + 1, "kv4: cu_q must be a contiguous int32 tensor [", B + 1, "]");
+  TORCH_CHECK(int32_on(cu_q, 1) && cu_q.size(0) == B + 1, "kv4: cu_q must be a contiguous int32 tensor [", num(B + 1), "]");
   TORCH_CHECK(int32_on(table, 2) && table.size(0) == B && table.size(1) >= 1 && table.size(1) <= (1 << 24),
-              "kv4: block_table must be a contiguous int32 tensor [", B, ", pages >= 1]");
+              "kv4: block_table must be a contiguous int32 tensor [", num(B), ", pages >= 1]");
   TORCH_CHECK(q.size(0) == 0 || B > 0, "kv4: rows without a sequence");
   TORCH_CHECK(q.size(0) < (int64_t)1 << 31, "kv4: too many rows");
   if (max_q < 0) max_q = q.size(0);
@@ -105,7 +110,7 @@ void kv4_append(Tensor k, Tensor v, Tensor slots, Tensor pages, Tensor bounds, T
   for (const Tensor* x : {&k, &v})
     TORCH_CHECK(x->device() == pages.device() && x->dim() == 3 && x->size(0) == T && x->size(1) == c.H &&
                     x->size(2) == c.D && (T == 0 || x->stride(2) == 1) && half_type(*x) && x->scalar_type() == k.scalar_type(),
-                "kv4: k and v must be bf16 or f16 [", T, ", ", c.H, ", ", c.D,
+                "kv4: k and v must be bf16 or f16 [", num(T), ", ", num(c.H), ", ", num(c.D),
                 "] of one type, inner stride 1, on the cache's device");
   TORCH_CHECK(T * c.H * (c.D / 16) < (int64_t)1 << 38, "kv4: too many rows for one call");
   if (T == 0) return;
@@ -131,8 +136,8 @@ Tensor kv4_select(Tensor q, Tensor cu_q, Tensor seq_lens, Tensor table, int64_t 
   const c10::cuda::CUDAGuard guard(pages.device());
   const int64_t G = check_batch(q, cu_q, seq_lens, table, pages, c, max_q);
   TORCH_CHECK(first >= 0 && last >= 1 && first + last <= budget && budget < (1 << 24),
-              "kv4: need first >= 0, last >= 1 and first + last <= budget, got ", first, ", ", last, ", ", budget);
-  TORCH_CHECK(G <= 64, "kv4: select takes at most 64 query heads per K/V head, got ", G);
+              "kv4: need first >= 0, last >= 1 and first + last <= budget, got ", num(first), ", ", num(last), ", ", num(budget));
+  TORCH_CHECK(G <= 64, "kv4: select takes at most 64 query heads per K/V head, got ", num(G));
   const int64_t T = q.size(0), W = table.size(1);
   Tensor chosen = at::empty({T, c.H, budget}, seq_lens.options());
   Tensor score = at::empty({W > budget ? T * c.H * W : 0}, unit.options());
@@ -155,7 +160,7 @@ std::tuple<Tensor, optional<Tensor>> kv4_attend(Tensor q, Tensor cu_q, Tensor se
   if (chosen.has_value())
     TORCH_CHECK(chosen->device() == pages.device() && chosen->scalar_type() == at::kInt && chosen->is_contiguous() &&
                     chosen->dim() == 3 && chosen->size(0) == T && chosen->size(1) == c.H && chosen->size(2) >= 1,
-                "kv4: pages must be a contiguous int32 tensor [", T, ", ", c.H, ", n >= 1] on the cache's device");
+                "kv4: pages must be a contiguous int32 tensor [", num(T), ", ", num(c.H), ", n >= 1] on the cache's device");
   Tensor out = at::empty({T, q.size(1), c.D}, q.options());
   optional<Tensor> lse;
   if (return_lse) lse = at::empty({T, q.size(1)}, unit.options());

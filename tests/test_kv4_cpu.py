@@ -1,0 +1,79 @@
+"""The 4-bit grouped-query cache page on the CPU: rounding, byte layout, bounds; refusals that need no GPU."""
+import math
+import random
+
+import pytest
+import torch
+
+from vllm_moet_b200.formats import kv4
+from vllm_moet_b200.formats.codebook import E2M1_VALUES
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_page_layout_round_trip(D):
+    g = torch.Generator().manual_seed(D)
+    kc, vc = (torch.randint(0, 16, (64, D), generator=g, dtype=torch.uint8) for _ in range(2))
+    ks, vs = (torch.randint(0, 127, (64, D // 16), generator=g, dtype=torch.uint8) for _ in range(2))
+    page = kv4.pack_page(kc, ks, vc, vs)
+    assert page.shape == (72 * D,)
+    for got, want in zip(kv4.unpack_page(page), (kc, ks, vc, vs)):
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_every_byte_is_used_once(D):
+    kb, kn, vb, vn, ks, vs = kv4._places(D)
+    half = torch.cat([(kb * 2 + kn).flatten(), (vb * 2 + vn).flatten()])
+    whole = torch.cat([ks.flatten(), vs.flatten()])
+    used = torch.cat([half, whole * 2, whole * 2 + 1])
+    assert torch.equal(used.sort().values, torch.arange(2 * 72 * D))
+    # a position's value bytes are its own: rows can be written in any order
+    owner = torch.arange(64)[:, None].expand(64, D)
+    for b in vb.unique():
+        assert len(owner[vb == b].unique()) == 1
+
+
+def test_rounding_is_to_nearest_with_ties_to_even():
+    """Against a search over every code, on values that lie on and beside the midpoints."""
+    rng = random.Random(5)
+    rows = []
+    for _ in range(200):
+        s = rng.choice([2.0 ** -5, 0.8125, 3.25, 2.0 ** -13])
+        row = [rng.choice([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, 0.0, 0.1, 5.9]) * s * rng.choice([-1, 1]) for _ in range(15)]
+        rows.append(row + [6 * s])
+    x = torch.tensor(rows, dtype=torch.float64)
+    codes, s8 = kv4.quantise(x)
+    scale = s8.view(torch.float8_e4m3fn).double() / 64
+    mags = E2M1_VALUES.double()[:8]
+    for r in range(x.shape[0]):
+        for i in range(16):
+            q = abs(float(x[r, i])) / float(scale[r, 0])
+            best = min(range(8), key=lambda c: (abs(q - float(mags[c])), c % 2))
+            assert int(codes[r, i]) & 7 == best, (q, best)
+
+
+def test_zeros_and_saturation():
+    codes, s8 = kv4.quantise(torch.zeros(2, 64))
+    assert not s8.any() and not codes.any()
+    codes, s8 = kv4.quantise(torch.full((1, 64), 1e6))
+    assert (kv4.values(codes, s8) == 42).all()              # 6 * 448 / 64
+    codes, s8 = kv4.quantise(torch.full((1, 64), 1e6), exp=4)
+    assert (kv4.values(codes, s8, exp=4) == 6 * 448 * 16).all()
+
+
+def test_bounds_hold_every_key():
+    g = torch.Generator().manual_seed(3)
+    k = torch.randn(64, 128, generator=g).double() * torch.rand(128, generator=g) * 8
+    b, unit = kv4.bounds(k)
+    assert math.log2(unit) == int(math.log2(unit)) and k.abs().max() <= 127 * unit and k.abs().max() > 63 * unit
+    assert (b[0].double() * unit >= k.amax(0)).all() and (b[1].double() * unit <= k.amin(0)).all()
+    b, unit = kv4.bounds(torch.zeros(64, 64))
+    assert unit == 1 and not b.any()
+
+
+def test_cache_refuses_what_it_cannot_hold():
+    from vllm_moet_b200.ops.kv4 import KV4Cache
+    for args, kw in (((4, 2, 96), {}), ((0, 2, 64), {}), ((4, 0, 64), {}), ((4, 2, 64), {"k_exp": 5}),
+                     ((4, 2, 64), {"v_exp": -15}), ((4, 2, 64), {"device": "cpu"})):
+        with pytest.raises(ValueError):
+            KV4Cache(*args, **kw)

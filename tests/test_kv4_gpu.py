@@ -1,0 +1,563 @@
+"""KV4Cache (4-bit paged K/V cache) against a plain implementation in 64 bits."""
+import math
+
+import pytest
+import torch
+
+from vllm_moet_b200.formats import kv4
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.fixture(scope="module")
+def KV4Cache():
+    from vllm_moet_b200.ops.kv4 import KV4Cache
+    return KV4Cache
+
+
+class Batch:
+    """Sequences with all their raw keys / values, a page table and the query rows."""
+
+    def __init__(self, lens, news, H, G, D, dtype=torch.bfloat16, seed=0, spare=2, q_scale=1.0, width=None):
+        g = torch.Generator().manual_seed(seed)
+        self.lens, self.news, self.H, self.G, self.D, self.dtype = lens, news, H, G, D, dtype
+        pages = [-(-n // 64) for n in lens]
+        self.n_pages = sum(pages) + spare
+        perm = torch.randperm(self.n_pages, generator=g).int()
+        self.table = torch.full((len(lens), width or max(max(pages), 1)), -7, dtype=torch.int32)
+        at, slots = 0, []
+        for b, w in enumerate(pages):
+            self.table[b, :w] = perm[at:at + w]
+            j = torch.arange(lens[b])
+            slots.append(self.table[b, j // 64].long() * 64 + j % 64)
+            at += w
+        self.slots = torch.cat(slots) if slots else torch.zeros(0, dtype=torch.int64)
+        total = sum(lens)
+        self.k = (torch.randn(total, H, D, generator=g) * 1.3 + 0.4).to(dtype)
+        self.v = torch.randn(total, H, D, generator=g).to(dtype)
+        self.q = (torch.randn(sum(news), H * G, D, generator=g) * q_scale).to(dtype)
+        self.cu = torch.tensor([0] + news).cumsum(0).int()
+        self.seq_lens = torch.tensor(lens, dtype=torch.int32)
+
+    def cache(self, KV4Cache, **kw):
+        c = KV4Cache(self.n_pages, self.H, self.D, device=DEV, **kw)
+        c.append(self.k.to(DEV), self.v.to(DEV), self.slots.to(DEV))
+        return c
+
+    def args(self):
+        return self.q.to(DEV), self.cu.to(DEV), self.seq_lens.to(DEV), self.table.to(DEV)
+
+    def held(self, x, exp=-6):
+        return kv4.values(*kv4.quantise(x, exp), exp).double()
+
+    def oracle(self, scale, window=0, pages=None):
+        """(out, lse, sum p |v| / sum p, positions seen) per row, in 64 bits."""
+        T, Hq, D, G = self.q.shape[0], self.H * self.G, self.D, self.G
+        out = torch.zeros(T, Hq, D, dtype=torch.float64)
+        mag = torch.zeros_like(out)
+        lse = torch.full((T, Hq), -math.inf, dtype=torch.float64)
+        k, v = self.held(self.k), self.held(self.v)
+        at = 0
+        for b, (n, m) in enumerate(zip(self.lens, self.news)):
+            for i in range(m):
+                row, p = int(self.cu[b]) + i, n - m + i
+                for h in range(self.H):
+                    keys = [j for j in range(max(0, p - window + 1) if window else 0, p + 1)]
+                    if pages is not None:
+                        ok = set(x for x in pages[row, h].tolist() if x >= 0)
+                        keys = [j for j in keys if j // 64 in ok]
+                    if not keys:
+                        continue
+                    idx = torch.tensor(keys) + at
+                    s = self.q[row, h * G:(h + 1) * G].double() @ k[idx, h].T * scale
+                    pr = torch.softmax(s, -1)
+                    out[row, h * G:(h + 1) * G] = pr @ v[idx, h]
+                    mag[row, h * G:(h + 1) * G] = pr @ v[idx, h].abs()
+                    lse[row, h * G:(h + 1) * G] = torch.logsumexp(s, -1)
+            at += n
+        return out, lse, mag
+
+
+def check(got, lse, want, keys):
+    """Half an ulp of the output (2^-8 of a bf16 value, 2^-11 of an f16 one), P rounded to f16 (2^-11 of every
+    term, and 2^-25 of each of at most `keys` terms that are subnormal), and 2^-11 for the f32 scores, whose
+    errors (2^-24 of sums of up to 256 terms of size 2^5 or so) enter the exponent."""
+    o, l, mag = want
+    half = 2.0 ** -8 if got.dtype == torch.bfloat16 else 2.0 ** -11
+    got, lse = got.double().cpu(), lse.double().cpu()
+    top = mag.amax(-1, keepdim=True)
+    bound = half * o.abs() + (2.0 ** -10 + half * 2.0 ** -10) * mag + keys * 2.0 ** -25 * top + 1e-12
+    assert torch.isfinite(got).all()
+    assert ((got - o).abs() <= bound).all(), float(((got - o).abs() - bound).max())
+    empty = l == -math.inf
+    assert torch.equal(lse == -math.inf, empty)
+    assert (got[empty] == 0).all()
+    assert ((lse - l).abs()[~empty] <= 2.0 ** -11).all()
+
+
+# ------------------------------------------------------------------------------ write and read
+@pytest.mark.parametrize("D,H,dtype", [(64, 3, torch.float16), (128, 2, torch.bfloat16), (256, 1, torch.float16),
+                                       (64, 1, torch.bfloat16), (128, 8, torch.float16), (256, 2, torch.bfloat16)])
+def test_append_gives_the_golden_bytes_and_bounds(KV4Cache, D, H, dtype):
+    g = torch.Generator().manual_seed(D + H)
+    T, P = 150, 4
+    k = (torch.randn(T, H, D, generator=g) * torch.rand(T, H, D // 16, 1, generator=g).repeat(1, 1, 1, 16).view(T, H, D) * 9).to(dtype)
+    v = (torch.randn(T, H, D, generator=g) * 0.02).to(dtype)
+    k[5] = 0
+    k[7, 0, :16] = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5, 6, -0.25, -0.75, -1.25, -1.75, -2.5, -3.5, -5, -6]).to(dtype)
+    v[9, 0, 0] = 60000.0                                       # saturates its block
+    slots = torch.randperm(P * 64, generator=g)[:T]            # any order; pages partly written
+    slots[3] = -1
+    c = KV4Cache(P, H, D, device=DEV)
+    c.append(k.to(DEV), v.to(DEV), slots.to(DEV))
+    kc = torch.zeros(P * 64, H, D, dtype=torch.uint8)
+    ks = torch.zeros(P * 64, H, D // 16, dtype=torch.uint8)
+    vc, vs = kc.clone(), ks.clone()
+    live = slots >= 0
+    a, b = kv4.quantise(k)
+    kc[slots[live]], ks[slots[live]] = a[live], b[live]
+    a, b = kv4.quantise(v)
+    vc[slots[live]], vs[slots[live]] = a[live], b[live]
+    for p in range(P):
+        rows = slice(p * 64, p * 64 + 64)
+        for h in range(H):
+            assert torch.equal(c.pages[p, h].cpu(), kv4.pack_page(kc[rows, h], ks[rows, h], vc[rows, h], vs[rows, h]))
+            want, unit = kv4.bounds(kv4.values(kc[rows, h], ks[rows, h]))
+            assert torch.equal(c.bounds[p, h].cpu(), want) and float(c.unit[p, h]) == unit
+    c.check()
+    for dt in (torch.bfloat16, torch.float16):
+        rk, rv = c.read(slots.to(DEV), dt)
+        want_k = torch.where(live[:, None, None], kv4.values(*kv4.quantise(k)), 0.0)
+        want_v = torch.where(live[:, None, None], kv4.values(*kv4.quantise(v)), 0.0)
+        assert rk.dtype == dt and torch.equal(rk.float().cpu(), want_k) and torch.equal(rv.float().cpu(), want_v)
+
+
+@pytest.mark.parametrize("exp", [-14, 0, 4])
+def test_exponents(KV4Cache, exp):
+    g = torch.Generator().manual_seed(1)
+    k = (torch.randn(64, 1, 64, generator=g) * 2.0 ** (exp + 5)).to(torch.float16)
+    c = KV4Cache(1, 1, 64, device=DEV, k_exp=exp, v_exp=exp)
+    slots = torch.arange(64, device=DEV)
+    c.append(k.to(DEV), -k.to(DEV), slots)
+    rk, rv = c.read(slots, torch.float16)
+    want = kv4.values(*kv4.quantise(k, exp), exp)
+    assert torch.equal(rk.float().cpu(), want) and torch.equal(rv.float().cpu(), -want)
+    b, unit = kv4.bounds(want[:, 0])
+    assert torch.equal(c.bounds[0, 0].cpu(), b) and float(c.unit[0, 0]) == unit
+
+
+def test_strided_and_unaligned_rows(KV4Cache):
+    """Slices of a fused projection's output, and rows that do not start on 16 bytes."""
+    g = torch.Generator().manual_seed(2)
+    H, D, T = 2, 128, 33
+    qkv = torch.randn(T, 8, D, generator=g).to(torch.bfloat16).to(DEV)
+    odd = torch.randn(T, 2 * H * (D + 1) + 1, generator=g).to(torch.bfloat16).to(DEV)
+    slots = torch.arange(T, device=DEV)
+    for k, v in ((qkv[:, 4:6], qkv[:, 6:8]),
+                 (odd[:, 1:1 + H * (D + 1)].unflatten(1, (H, D + 1))[..., 1:], odd[:, 1:1 + H * (D + 1)].unflatten(1, (H, D + 1))[..., :D])):
+        c = KV4Cache(1, H, D, device=DEV)
+        c.append(k, v, slots)
+        rk, rv = c.read(slots)
+        assert torch.equal(rk.float().cpu(), kv4.values(*kv4.quantise(k.cpu())))
+        assert torch.equal(rv.float().cpu(), kv4.values(*kv4.quantise(v.cpu())))
+
+
+def test_status_of_bad_slots_and_values(KV4Cache):
+    c = KV4Cache(2, 1, 64, device=DEV)
+    x = torch.ones(2, 1, 64, dtype=torch.bfloat16, device=DEV)
+    c.append(x, x, torch.tensor([0, 128], device=DEV))
+    assert int(c.status) == 1
+    with pytest.raises(RuntimeError, match="out of range"):
+        c.check()
+    c.status.zero_()
+    k, v = c.read(torch.tensor([128, 0], device=DEV))
+    one = kv4.values(*kv4.quantise(x.cpu()))[0].to(DEV)                 # 1 is held as 6 * 11/64
+    assert int(c.status) == 1 and (k[0] == 0).all() and torch.equal(k[1].float(), one)
+    c.status.zero_()
+    y = x.clone()
+    y[0, 0, 3], y[0, 0, 20], y[1, 0, 5] = math.nan, -math.inf, math.inf
+    c.append(y, x, torch.tensor([1, 2], device=DEV))
+    assert int(c.status) == 4
+    k, _ = c.read(torch.tensor([1, 2], device=DEV))
+    assert float(k[0, 0, 3]) == 0 and float(k[0, 0, 20]) == -42 and float(k[1, 0, 5]) == 42
+    # block 1 of row 0 holds an infinity: its other values vanish beside it; a NaN leaves its block as it was
+    assert torch.equal(k[0, 0, :3].float(), one[0, :3]) and (k[0, 0, 32:].float() == one[0, 32:]).all()
+
+
+def test_bounds_follow_rewritten_rows(KV4Cache):
+    """A rejected draft's row is written again: the page's bounds are those of what it holds now."""
+    g = torch.Generator().manual_seed(4)
+    c = KV4Cache(1, 1, 64, device=DEV)
+    k = torch.randn(64, 1, 64, generator=g).to(torch.bfloat16)
+    k[63] *= 30
+    c.append(k.to(DEV), k.to(DEV), torch.arange(64, device=DEV))
+    k[63] /= 64
+    c.append(k[63:].to(DEV), k[63:].to(DEV), torch.tensor([63], device=DEV))
+    want, unit = kv4.bounds(kv4.values(*kv4.quantise(k))[:, 0])
+    assert torch.equal(c.bounds[0, 0].cpu(), want) and float(c.unit[0, 0]) == unit
+
+
+# ---------------------------------------------------------------------------------- attention
+STEP = [
+    ([1], [1], 1, 1, 64, torch.bfloat16, 0),
+    ([64], [1], 2, 8, 128, torch.bfloat16, 0),
+    ([65, 63, 0, 129], [1, 1, 1, 1], 2, 3, 128, torch.float16, 0),
+    ([200, 1, 70], [3, 2, 3], 2, 5, 256, torch.bfloat16, 0),          # verify rows; one sequence shorter than its rows
+    ([300, 128], [2, 0], 1, 12, 64, torch.float16, 0),                # a sequence without rows
+    ([500], [4], 1, 6, 128, torch.bfloat16, 100),                     # window
+    ([130, 64], [1, 1], 1, 40, 128, torch.bfloat16, 1),               # more heads than a tile; window of one
+    ([777], [1], 4, 16, 256, torch.float16, 300),
+]
+PROMPT = [
+    ([100], [100], 1, 1, 64, torch.bfloat16, 0),
+    ([300, 65, 7, 130], [130, 65, 9, 1], 2, 2, 128, torch.bfloat16, 0),
+    ([400], [70], 1, 5, 256, torch.float16, 0),
+    ([257, 0], [33, 3], 2, 8, 64, torch.float16, 0),
+    ([450], [90], 1, 4, 128, torch.bfloat16, 37),
+    ([129], [129], 1, 3, 128, torch.float16, 64),
+]
+
+
+@pytest.mark.parametrize("lens,news,H,G,D,dtype,window", STEP + PROMPT)
+def test_attend(KV4Cache, lens, news, H, G, D, dtype, window):
+    x = Batch(lens, news, H, G, D, dtype, seed=sum(lens), q_scale=2.0)
+    c = x.cache(KV4Cache)
+    scale = D ** -0.5
+    out, lse = c.attend(*x.args(), scale, max_q=max(news), window=window, return_lse=True)
+    c.check()
+    assert out.dtype == dtype
+    check(out, lse, x.oracle(scale, window), max(lens))
+    again = c.attend(*x.args(), scale, max_q=max(news), window=window)
+    assert torch.equal(again, out)                                   # and bit for bit again
+
+
+@pytest.mark.parametrize("max_q,scale", [(3, 0.3), (200, 0.3), (3, -0.2), (200, -0.2), (3, 0.0), (200, 0.0)])
+def test_both_kernels_and_any_scale(KV4Cache, max_q, scale):
+    """max_q only chooses the kernel; negative and zero scales."""
+    x = Batch([333, 90], [3, 2], 2, 4, 128, seed=9)
+    c = x.cache(KV4Cache)
+    out, lse = c.attend(*x.args(), scale, max_q=max_q, return_lse=True)
+    check(out, lse, x.oracle(scale), 333)
+
+
+@pytest.mark.parametrize("max_q", [2, 500])
+def test_large_and_tiny_queries(KV4Cache, max_q):
+    """bf16 rows far outside f16's range, a row of zeros, and scores that move the running maximum late."""
+    x = Batch([640], [2], 1, 4, 128, seed=10)
+    x.q[0, 0] *= 2.0 ** 60
+    x.q[0, 1] *= 2.0 ** -70
+    x.q[1, 0] = 0
+    x.q[1, 2] *= 40
+    x.k[600:] *= 3                                                   # the largest keys come last
+    c = x.cache(KV4Cache)
+    q, cu, sl, tb = x.args()
+    out = c.attend(q, cu, sl, tb, 2.0 ** -3, max_q=max_q)
+    o, _, mag = x.oracle(2.0 ** -3)
+    rows = [(0, 1), (0, 2), (0, 3), (1, 0), (1, 1), (1, 3)]
+    for r, h in rows:
+        assert ((out[r, h].double().cpu() - o[r, h]).abs() <= 2.0 ** -8 * o[r, h].abs() + 2.0 ** -9 * mag[r, h] + 1e-6).all()
+    # scores of 2^60: one key takes all (its f32 score is the largest)
+    assert torch.isfinite(out).all()
+
+
+def test_unwritten_bytes_may_be_anything(KV4Cache):
+    """NaN scales in positions that no row sees, in both kernels and over chosen pages."""
+    x = Batch([70, 1], [2, 1], 1, 4, 128, seed=11)
+    c = x.cache(KV4Cache)
+    ref = c.attend(*x.args(), 0.1, max_q=2)
+    k, v = (t.to(DEV) for t in (x.k, x.v))
+    c.pages.fill_(0xFF)
+    c.append(k, v, x.slots.to(DEV))
+    for max_q in (2, 100):
+        assert torch.allclose(c.attend(*x.args(), 0.1, max_q=max_q).float(), ref.float(), atol=2e-2)
+        assert torch.isfinite(c.attend(*x.args(), 0.1, max_q=max_q)).all()
+    pages = torch.tensor([[[1, 0]], [[0, 1]], [[0, -1]]], dtype=torch.int32, device=DEV)
+    assert torch.equal(c.attend(*x.args(), 0.1, max_q=2, pages=pages), ref) or torch.allclose(
+        c.attend(*x.args(), 0.1, max_q=2, pages=pages).float(), ref.float(), atol=2e-2)
+
+
+def test_a_bad_row_stays_its_own(KV4Cache):
+    x = Batch([100], [3], 1, 4, 64, seed=12)
+    c = x.cache(KV4Cache)
+    ref = {m: c.attend(*x.args(), 0.1, max_q=m) for m in (3, 100)}
+    x.q[1, 2, 5] = math.nan
+    for m in (3, 100):
+        out = c.attend(*x.args(), 0.1, max_q=m)
+        assert torch.isnan(out[1, 2]).all()
+        out[1, 2], ref[m][1, 2] = 0, 0
+        assert torch.equal(out, ref[m])
+
+
+@pytest.mark.parametrize("lens,news,H,G,D,dtype", [
+    ([640, 65, 30], [1, 2, 1], 2, 8, 128, torch.bfloat16), ([900], [40], 1, 3, 64, torch.float16),
+    ([520, 1], [2, 3], 2, 20, 256, torch.bfloat16)])
+def test_attend_over_chosen_pages(KV4Cache, lens, news, H, G, D, dtype):
+    x = Batch(lens, news, H, G, D, dtype, seed=13)
+    c = x.cache(KV4Cache)
+    g = torch.Generator().manual_seed(1)
+    T = sum(news)
+    pages = torch.full((T, H, 5), -1, dtype=torch.int32)
+    for r in range(T):
+        for h in range(H):
+            some = torch.randperm(max(1, max(lens) // 64), generator=g)[:5].int()   # in any order, past the end too
+            pages[r, h, :some.numel()] = some
+    pages[0, 0] = -1                                                  # a row without pages
+    out, lse = c.attend(*x.args(), 0.09, max_q=max(news), pages=pages.to(DEV), return_lse=True)
+    for r in range(T):                                                # what lies past a row's own position is not seen
+        b = int(torch.searchsorted(x.cu, torch.tensor(r, dtype=torch.int32), right=True)) - 1
+        p = lens[b] - news[b] + r - int(x.cu[b])
+        pages[r][pages[r] * 64 > p] = -1
+    check(out, lse, x.oracle(0.09, pages=pages), 320)
+
+
+def test_many_sequences(KV4Cache):
+    """More sequences than threads of a block, most of them short, tiles split over blocks."""
+    g = torch.Generator().manual_seed(14)
+    lens = [int(x) for x in torch.randint(0, 40, (300,), generator=g)]
+    lens[7], lens[250] = 1500, 900
+    x = Batch(lens, [1] * 300, 1, 2, 64, seed=15)
+    c = x.cache(KV4Cache)
+    out, lse = c.attend(*x.args(), 0.2, max_q=1, return_lse=True)
+    check(out, lse, x.oracle(0.2), 1500)
+
+
+def test_offsets_past_32_bits(KV4Cache):
+    """A pool of 5 GB: the last pages are written, read and attended to."""
+    H, D = 8, 256
+    P = 5 * 2 ** 30 // (H * 72 * D)
+    c = KV4Cache(P, H, D, device=DEV)
+    g = torch.Generator().manual_seed(16)
+    k = torch.randn(80, H, D, generator=g).to(torch.bfloat16)
+    table = torch.tensor([[P - 1, P - 2]], dtype=torch.int32)
+    j = torch.arange(80)
+    slots = table[0, j // 64].long() * 64 + j % 64
+    c.append(k.to(DEV), k.to(DEV), slots.to(DEV))
+    rk, _ = c.read(slots.to(DEV))
+    held = kv4.values(*kv4.quantise(k))
+    assert torch.equal(rk.float().cpu(), held)
+    q = torch.randn(1, H, D, generator=g).to(torch.bfloat16)
+    s = torch.einsum("hd,nhd->hn", q[0].double(), held.double()) * 0.06
+    want = torch.einsum("hn,nhd->hd", torch.softmax(s, -1), held.double())
+    for max_q in (1, 100):
+        out = c.attend(q.to(DEV), torch.tensor([0, 1], dtype=torch.int32, device=DEV),
+                       torch.tensor([80], dtype=torch.int32, device=DEV), table.to(DEV), 0.06, max_q=max_q)
+        assert (out[0].double().cpu() - want).abs().max() <= 2.0 ** -8 * want.abs().max()
+    del c
+    torch.cuda.empty_cache()
+
+
+def test_bad_page_is_skipped_and_reported(KV4Cache):
+    x = Batch([200], [1], 1, 2, 64, seed=17)
+    for max_q in (1, 200):
+        c = x.cache(KV4Cache)
+        q, cu, sl, tb = x.args()
+        bad = tb.clone()
+        bad[0, 1] = x.n_pages
+        c.attend(q, cu, sl, bad, 0.1, max_q=max_q)
+        assert int(c.status) == 1
+    c = x.cache(KV4Cache)
+    c.attend(q, cu, sl, tb, 0.1, pages=torch.tensor([[[0, 9]]], dtype=torch.int32, device=DEV))
+    assert int(c.status) == 1
+
+
+def test_queries_in_any_layout(KV4Cache):
+    x = Batch([150], [2], 2, 4, 128, seed=18)
+    c = x.cache(KV4Cache)
+    q, cu, sl, tb = x.args()
+    ref = c.attend(q, cu, sl, tb, 0.1, max_q=2)
+    wide = torch.zeros(2, 8 + 4, 128, dtype=q.dtype, device=DEV)
+    wide[:, 2:10] = q
+    assert torch.equal(c.attend(wide[:, 2:10], cu, sl, tb, 0.1, max_q=2), ref)
+    odd = torch.zeros(2 * 8 * 129 + 1, dtype=q.dtype, device=DEV)[1:].view(2, 8, 129)
+    odd[..., :128] = q
+    assert torch.equal(c.attend(odd[..., :128], cu, sl, tb, 0.1, max_q=2), ref)
+    t = q.transpose(1, 2).contiguous().transpose(1, 2)               # inner stride not 1
+    assert torch.equal(c.attend(t, cu, sl, tb, 0.1, max_q=2), ref)
+
+
+# ---------------------------------------------------------------------------- choosing pages
+def choose(x, budget, first, last):
+    """The definition: exact scores in 64 bits, ties to the lowest page."""
+    T = x.q.shape[0]
+    pages = torch.full((T, x.H, budget), -1, dtype=torch.int32)
+    held, at = x.held(x.k), 0
+    for b, (n, m) in enumerate(zip(x.lens, x.news)):
+        w = -(-n // 64)
+        k = torch.cat([held[at:at + n], torch.zeros(w * 64 - n, x.H, x.D, dtype=torch.float64)]).view(w, 64, x.H, x.D)
+        bnd = [[kv4.bounds(k[i, :, h]) for h in range(x.H)] for i in range(w)]
+        at += n
+        for i in range(m):
+            row, p = int(x.cu[b]) + i, n - m + i
+            if p < 0:
+                continue
+            cnt = p // 64 + 1
+            for h in range(x.H):
+                if cnt <= budget:
+                    pages[row, h, :cnt] = torch.arange(cnt)
+                    continue
+                q = torch.nan_to_num(x.q[row, h * x.G:(h + 1) * x.G].double(), nan=0.0, posinf=3.4028235e38, neginf=-3.4028235e38)
+                f = torch.tensor([kv4.bounds(y[None])[1] for y in q])
+                r = torch.round(q / f[:, None])
+                score = []
+                for page in range(first, cnt - last):
+                    e, unit = bnd[page][h]
+                    s = r.clamp(min=0) @ e[0].double() + r.clamp(max=0) @ e[1].double()
+                    score.append((-float((s * f).max()) * unit, page))
+                best = [pg for _, pg in sorted(score)[:budget - first - last]]
+                chosen = list(range(first)) + sorted(best) + list(range(cnt - last, cnt))
+                pages[row, h] = torch.tensor(chosen)
+    return pages
+
+
+@pytest.mark.parametrize("lens,news,H,G,D,dtype,budget,first,last", [
+    ([1000, 64, 0, 700], [1, 1, 1, 1], 2, 8, 128, torch.bfloat16, 6, 1, 2),
+    ([900, 30], [3, 2], 1, 1, 64, torch.float16, 4, 0, 1),
+    ([700], [70], 2, 2, 64, torch.bfloat16, 5, 1, 1),
+    ([650], [9], 1, 4, 256, torch.float16, 3, 1, 2),                  # nothing left to compete for
+    ([800, 400], [2, 17], 1, 5, 128, torch.bfloat16, 7, 2, 2),
+    ([640], [1], 1, 12, 128, torch.bfloat16, 5, 1, 2),
+    ([640], [2], 1, 64, 64, torch.float16, 5, 1, 2),
+    ([700], [3], 3, 3, 128, torch.bfloat16, 20, 1, 2),                # budget larger than the pages
+])
+def test_select(KV4Cache, lens, news, H, G, D, dtype, budget, first, last):
+    x = Batch(lens, news, H, G, D, dtype, seed=budget + sum(lens))
+    c = x.cache(KV4Cache)
+    got = c.select(*x.args(), budget, first=first, last=last, max_q=max(news))
+    c.check()
+    assert torch.equal(got.cpu(), choose(x, budget, first, last))
+
+
+def test_select_ties_go_to_the_lowest_page(KV4Cache):
+    x = Batch([64 * 12], [1], 1, 2, 64, seed=20)
+    x.k[:] = x.k[:1]                                                  # every page the same
+    c = x.cache(KV4Cache)
+    assert c.select(*x.args(), 6)[0, 0].tolist() == [0, 1, 2, 3, 10, 11]
+    x.q[:] = 0                                                        # every score zero
+    assert c.select(*x.args(), 6)[0, 0].tolist() == [0, 1, 2, 3, 10, 11]
+    x.q[0, 0, 0], x.q[0, 1, 3] = math.nan, math.inf
+    got = c.select(*x.args(), 6)
+    assert torch.equal(got.cpu(), choose(x, 6, 1, 2))
+
+
+@pytest.mark.parametrize("width", [250, 500, 1000, 1100, 5000])
+def test_select_of_long_rows(KV4Cache, width):
+    """Each way of finding the threshold, on bounds that are set directly: with ties, in every width."""
+    g = torch.Generator().manual_seed(width)
+    c = KV4Cache(width, 1, 64, device=DEV)
+    c.bounds.copy_(torch.randint(-3, 4, c.bounds.shape, generator=g).to(torch.int8))
+    c.unit.copy_(2.0 ** torch.randint(-2, 3, c.unit.shape, generator=g).float())
+    q = torch.zeros(3, 1, 64, dtype=torch.bfloat16)
+    q[0, 0, 5], q[1, 0, :3], q[2] = 1, torch.tensor([1.0, -1.0, 0.5]), torch.randn(1, 64, generator=g).bfloat16()
+    table = torch.randperm(width, generator=g).int()[None]
+    cu = torch.tensor([0, 3], dtype=torch.int32)
+    sl = torch.tensor([width * 64], dtype=torch.int32)
+    for budget in (4, 33, width - 1):
+        got = c.select(q.to(DEV), cu.to(DEV), sl.to(DEV), table.to(DEV), budget).cpu()
+        b, u = c.bounds.cpu()[table[0].long(), 0].double(), c.unit.cpu()[table[0].long(), 0].double()
+        for r in range(3):
+            f = kv4.bounds(q[r].double())[1]
+            y = torch.round(q[r, 0].double() / f)
+            s = (b[:, 0] @ y.clamp(min=0) + b[:, 1] @ y.clamp(max=0)) * f * u
+            order = sorted(range(1, width - 2), key=lambda i: (-float(s[i]), i))[:budget - 3]
+            assert got[r, 0].tolist() == [0] + sorted(order) + [width - 2, width - 1]
+
+
+def test_chosen_pages_hold_the_best_key(KV4Cache):
+    """The score is an upper bound: a page with a key far above the others is always taken."""
+    x = Batch([64 * 40], [1], 2, 4, 128, seed=21)
+    c0 = x.k.clone()
+    x.k = (c0 * 0.1).to(x.dtype)
+    q = x.q[0].view(2, 4, 128)
+    for h in range(2):
+        x.k[64 * 17 + 5, h] = (q[h, 2] * 4).to(x.dtype)
+    c = x.cache(KV4Cache)
+    got = c.select(*x.args(), 8)
+    assert all(17 in got[0, h].tolist() for h in range(2))
+
+
+# ------------------------------------------------------------------------ streams, graphs, refusals
+def test_other_stream_and_graph(KV4Cache):
+    x = Batch([700, 300], [1, 1], 2, 8, 128, seed=22)
+    c = x.cache(KV4Cache)
+    args = x.args()
+    ref_pages = c.select(*args, 5, max_q=1)
+    ref = c.attend(*args, 0.1, max_q=1, pages=ref_pages)
+    full = c.attend(*args, 0.1, max_q=1)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        pages = c.select(*args, 5, max_q=1)
+        out = c.attend(*args, 0.1, max_q=1, pages=pages)
+    s.synchronize()
+    assert torch.equal(pages, ref_pages) and torch.equal(out, ref)
+    g = torch.cuda.CUDAGraph()
+    slots = torch.zeros(2, dtype=torch.int64, device=DEV)
+    kn, vn = (torch.zeros(2, 2, 128, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    slots.fill_(-1)
+    with torch.cuda.graph(g):
+        c.append(kn, vn, slots)
+        pages = c.select(*args, 5, max_q=1)
+        out = c.attend(*args, 0.1, max_q=1, pages=pages)
+        whole = c.attend(*args, 0.1, max_q=1)
+    for _ in range(3):
+        out.zero_(), whole.zero_(), pages.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(pages, ref_pages) and torch.equal(out, ref) and torch.equal(whole, full)
+    c.check()
+
+
+def test_empty_calls(KV4Cache):
+    x = Batch([10], [0], 1, 2, 64, seed=23)
+    c = x.cache(KV4Cache)
+    out, lse = c.attend(*x.args(), 0.1, return_lse=True)
+    assert out.shape == (0, 2, 64) and lse.shape == (0, 2)
+    assert c.select(*x.args(), 4).shape == (0, 1, 4)
+    e = torch.zeros(0, 1, 64, dtype=torch.bfloat16, device=DEV)
+    none = torch.zeros(0, dtype=torch.int64, device=DEV)
+    c.append(e, e, none)
+    assert c.read(none)[0].shape == (0, 1, 64)
+
+
+def test_refusals(KV4Cache):
+    x = Batch([100], [2], 2, 2, 64, seed=24)
+    c = x.cache(KV4Cache)
+    q, cu, sl, tb = x.args()
+    k = torch.zeros(3, 2, 64, dtype=torch.bfloat16, device=DEV)
+    s = torch.arange(3, device=DEV)
+    bad = [
+        lambda: c.append(k, k, s.int()),
+        lambda: c.append(k, k, s[:2]),
+        lambda: c.append(k.float(), k.float(), s),
+        lambda: c.append(k, k.half(), s),
+        lambda: c.append(k.cpu(), k, s),
+        lambda: c.append(k[:, :1], k, s),
+        lambda: c.append(k.transpose(1, 2).contiguous().transpose(1, 2), k, s),
+        lambda: c.read(s, torch.float32),
+        lambda: c.read(s.cpu()),
+        lambda: c.attend(q.float(), cu, sl, tb, 1.0),
+        lambda: c.attend(q[:, :3], cu, sl, tb, 1.0),
+        lambda: c.attend(q[..., :32], cu, sl, tb, 1.0),
+        lambda: c.attend(q, cu.long(), sl, tb, 1.0),
+        lambda: c.attend(q, cu[:1], sl, tb, 1.0),
+        lambda: c.attend(q, cu, sl.cpu(), tb, 1.0),
+        lambda: c.attend(q, cu, sl, tb[0], 1.0),
+        lambda: c.attend(q, cu, sl, tb.long(), 1.0),
+        lambda: c.attend(q, cu, sl, tb, 1.0, max_q=0),
+        lambda: c.attend(q, cu, sl, tb, 1.0, window=-1),
+        lambda: c.attend(q, cu, sl, tb, 1.0, pages=torch.zeros(2, 2, 3, device=DEV)),
+        lambda: c.attend(q, cu, sl, tb, 1.0, pages=torch.zeros(2, 1, 3, dtype=torch.int32, device=DEV)),
+        lambda: c.select(q, cu, sl, tb, 2),
+        lambda: c.select(q, cu, sl, tb, 4, last=0),
+        lambda: c.select(q, cu, sl, tb, 4, first=-1),
+        lambda: c.select(torch.zeros(2, 2 * 65, 64, dtype=q.dtype, device=DEV), cu, sl, tb, 4),
+        lambda: c.attend(q, torch.zeros(4098, dtype=torch.int32, device=DEV), torch.zeros(4097, dtype=torch.int32, device=DEV),
+                         torch.zeros(4097, 1, dtype=torch.int32, device=DEV), 1.0),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises((RuntimeError, ValueError, TypeError)):
+            call()
+            pytest.fail(f"call {i} was not refused")
+    c.check()
+    assert torch.isfinite(c.attend(q, cu, sl, tb, 0.1)).all()        # and the cache still works
