@@ -14,6 +14,8 @@
 #include "kv4.cuh"
 #include "torch_glue.h"
 
+#include <type_traits>
+
 namespace moet {
 namespace kv4 {
 
@@ -27,37 +29,37 @@ struct AppendArgs {
   int* status;
 };
 
-template <typename T16> MOET_DEVICE uint32_t pack2(float a, float b);
-template <> MOET_DEVICE uint32_t pack2<__nv_bfloat16>(float a, float b) { return pack_bf16x2(a, b); }
-template <> MOET_DEVICE uint32_t pack2<__half>(float a, float b) {
-  __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<uint32_t*>(&h);
-}
-
 template <typename T16, bool VEC>
-MOET_DEVICE void load16(const T16* p, float (&x)[16]) {
-  T16 h[16];
+MOET_DEVICE void load16(const T16* p, uint32_t (&w)[8]) {
   if (VEC) {
-    reinterpret_cast<uint4*>(h)[0] = ldg_stream_u4(p);
-    reinterpret_cast<uint4*>(h)[1] = ldg_stream_u4(p + 8);
+    const uint4 a = ldg_stream_u4(p), b = ldg_stream_u4(p + 8);
+    w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
   } else {
+    const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
 #pragma unroll
-    for (int i = 0; i < 16; i++) h[i] = p[i];
+    for (int i = 0; i < 8; i++) w[i] = q[2 * i] | (uint32_t)q[2 * i + 1] << 16;
   }
-#pragma unroll
-  for (int i = 0; i < 16; i++) x[i] = to_f32(h[i]);
 }
+template <typename T16> MOET_DEVICE float2 widen(uint32_t w);
+template <> MOET_DEVICE float2 widen<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
+template <> MOET_DEVICE float2 widen<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+template <typename T16> constexpr uint32_t kInf16 = std::is_same<T16, __half>::value ? 0x7C00u : 0x7F80u;
 
-// The block's scale byte, and its values over the scale (what a code is rounded from) in x.
-MOET_DEVICE uint32_t scale_of(float (&x)[16], float inv_exp, bool& bad, float& s) {
-  float amax = 0.f;
-  bool odd = false;
+// The scale byte of 16 values, and the values over the scale (what the codes are rounded from) in x.
+// The largest magnitude is found on the 16-bit patterns, which also shows what is not finite.
+template <typename T16> MOET_DEVICE uint32_t scale_of(const uint32_t (&w)[8], float (&x)[16], float inv_exp, bool& bad) {
+  uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < 16; i++) {
-    odd |= !(fabsf(x[i]) <= 3.3895314e38f);      // NaN or infinite (bf16's largest finite value)
-    amax = fmaxf(amax, fabsf(x[i]));
+  for (int i = 0; i < 8; i++) {
+    top = __vmaxu2(top, w[i] & 0x7FFF7FFFu);
+    const float2 f = widen<T16>(w[i]);
+    x[2 * i] = f.x, x[2 * i + 1] = f.y;
   }
-  if (odd) {
+  top = max(top >> 16, top & 0xFFFFu);
+  float amax = widen<T16>(top).x;
+  if (top >= kInf16<T16>) {                              // NaN counts as 0, an infinity as a value past every scale
     bad = true;
     amax = 0.f;
 #pragma unroll
@@ -66,9 +68,13 @@ MOET_DEVICE uint32_t scale_of(float (&x)[16], float inv_exp, bool& bad, float& s
       amax = fmaxf(amax, fabsf(x[i]));
     }
   }
-  const float want = fminf(__fmul_rn(__fdiv_rn(amax, 6.f), inv_exp), 448.f);
-  const uint32_t s8 = f32_to_e4m3(want);
-  s = __fdiv_rn(e4m3_to_f32((uint8_t)s8), inv_exp);     // inv_exp is a power of two: exact
+  const float want = __fmul_rn(__fdiv_rn(amax, 6.f), inv_exp);
+  const uint32_t s8 = f32_to_e4m3(fminf(want, 448.f));
+  const float s = __fdiv_rn(e4m3_to_f32((uint8_t)s8), inv_exp);     // inv_exp is a power of two: exact
+  if (want > 448.f) {                                    // saturated: 6 s is the largest that can be held
+#pragma unroll
+    for (int i = 0; i < 16; i++) x[i] = fminf(fmaxf(x[i], -8.f * s), 8.f * s);
+  }
   if (s8 == 0) {
 #pragma unroll
     for (int i = 0; i < 16; i++) x[i] = copysignf(0.f, x[i]);
@@ -76,9 +82,8 @@ MOET_DEVICE uint32_t scale_of(float (&x)[16], float inv_exp, bool& bad, float& s
     const float r = __frcp_rn(s);
 #pragma unroll
     for (int i = 0; i < 16; i++) {
-      const float c = fminf(fmaxf(x[i], -8.f * s), 8.f * s);    // beyond 6 s all the same; keeps the fma finite
-      const float y = __fmul_rn(c, r);
-      x[i] = __fmaf_rn(__fmaf_rn(-y, s, c), r, y);
+      const float y = __fmul_rn(x[i], r);
+      x[i] = __fmaf_rn(__fmaf_rn(-y, s, x[i]), r, y);
     }
   }
   return s8;
@@ -103,21 +108,23 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(AppendArgs a) {
   const long long idx = (long long)blockIdx.x * 256 + threadIdx.x;
   const long long row = idx / L::NB;
   const int b = (int)(idx % L::NB), bs = b % (L::SD / 16), slab = b / (L::SD / 16);
-  const int tok = (int)(row / a.H), h = (int)(row % a.H);
-  bool live = row < (long long)a.T * a.H, bad = false;
-  const long long slot = live ? a.slots[tok] : -1;
+  const int tok = (int)((uint32_t)row / (uint32_t)a.H), h = (int)row - tok * a.H;      // rows are counted in 31 bits
+  const bool there = row < (long long)a.T * a.H;
+  bool bad = false;
+  const long long slot = there ? a.slots[tok] : -1;
   if (slot >= a.n_slots) set_status(a.status, kBadIndex);
-  live = slot >= 0 && slot < a.n_slots;
+  const bool live = slot >= 0 && slot < a.n_slots;
   const int j = (int)(slot % kPage);                                   // position in its page
   uint8_t* page = a.pages + ((slot / kPage) * a.H + h) * (long long)L::kPageBytes;
-  float x[16], y[16], s;
+  uint32_t xw[8], yw[8];
+  float x[16], y[16];
 #pragma unroll
-  for (int i = 0; i < 16; i++) x[i] = y[i] = 0.f;
-  if (live) {
-    load16<T16, VEC>((const T16*)a.k.p + tok * a.k.tok + h * a.k.head + b * 16, x);
-    load16<T16, VEC>((const T16*)a.v.p + tok * a.v.tok + h * a.v.head + b * 16, y);
+  for (int i = 0; i < 8; i++) xw[i] = yw[i] = 0;
+  if (there) {                           // without waiting for the slot
+    load16<T16, VEC>((const T16*)a.k.p + tok * a.k.tok + h * a.k.head + b * 16, xw);
+    load16<T16, VEC>((const T16*)a.v.p + tok * a.v.tok + h * a.v.head + b * 16, yw);
   }
-  const uint32_t k8 = scale_of(x, a.k_inv, bad, s), v8 = scale_of(y, a.v_inv, bad, s);
+  const uint32_t k8 = scale_of<T16>(xw, x, a.k_inv, bad), v8 = scale_of<T16>(yw, y, a.v_inv, bad);
   uint8_t* kc = page + L::KC + slab * L::kSlabBytes + j * (L::SD / 2);
   uint8_t* vc = page + L::VC + slab * L::kSlabBytes + (j >> 1) * L::SD + (j & 1) * (L::SD / 16);
   if constexpr (L::SD == 128) {
@@ -152,10 +159,10 @@ struct BoundsArgs {
   const uint8_t* pages; int8_t* bounds; float* unit; float k_mul;     // k_mul = 2^k_exp
 };
 
-// A warp per touched page and head.  The block looks at `win` slots and lists the last of each
-// run in one page; max and min are taken in f16, where the held values are exact.
+// A warp per touched page and head.  The block looks at `win` slots (64 in a prompt, where a run in
+// one page is long; 2 where every slot may be a page of its own) and lists the last of each run in one page; max and min are taken in f16, where the held values are exact.
 template <int D>
-__global__ void __launch_bounds__(256) kv4_bounds_kernel(BoundsArgs a) {
+__global__ void __launch_bounds__(64) kv4_bounds_kernel(BoundsArgs a) {
   using L = Lay<D>;
   pdl_entry();
   __shared__ int list[64], count;
@@ -172,7 +179,7 @@ __global__ void __launch_bounds__(256) kv4_bounds_kernel(BoundsArgs a) {
   __syncthreads();
   const int n = count, t = lane & 3;
   constexpr int W = L::SD / 32;                    // 32-bit words of a piece
-  for (int e = warp; e < n; e += 8) {
+  for (int e = warp; e < n; e += 2) {
     const long long page = list[e];
     const uint8_t* base = a.pages + (page * a.H + h) * (long long)L::kPageBytes;
     __half2 hi[L::NS][W][4], lo[L::NS][W][4];
@@ -240,15 +247,24 @@ __global__ void __launch_bounds__(256) kv4_bounds_kernel(BoundsArgs a) {
   }
 }
 
-// four bytes' low codes and high codes
-MOET_DEVICE void values4(uint32_t w, float* lo, float* hi) {
-  uint32_t r[4];
-  e2m1x8_to_f16(w, r);
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r[i]));
-    lo[i] = f.x, hi[i] = f.y;
-  }
+// the low (or, shift 4, the high) codes of four bytes as two f16x2, in order
+MOET_DEVICE void values4(uint32_t w, int shift, uint32_t& a, uint32_t& b) {
+  uint32_t t = (w >> shift) & 0x0F0F0F0Fu;
+  t |= t >> 4;                                             // bytes 0 and 2 now hold two codes each
+  asm("{\n.reg .b8 b0, b1, b2, b3;\nmov.b32 {b0, b1, b2, b3}, %2;\n"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\ncvt.rn.f16x2.e2m1x2 %1, b2;\n}\n" : "=r"(a), "=r"(b) : "r"(t));
+}
+// values of f16 pairs in the output's type
+template <typename T16> MOET_DEVICE uint32_t out2(uint32_t v);
+template <> MOET_DEVICE uint32_t out2<__half>(uint32_t v) { return v; }
+template <> MOET_DEVICE uint32_t out2<__nv_bfloat16>(uint32_t v) {
+  const float2 f = widen<__half>(v);
+  return pack_bf16x2(f.x, f.y);
+}
+// a scale times 2^exp, in both halves: every product with a code is exact in f16 (exp in [-14, 4])
+MOET_DEVICE uint32_t scale2(uint8_t s8, float mul) {
+  const __half2 h = __float2half2_rn(e4m3_to_f32(s8) * mul);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 struct ReadArgs {
@@ -258,66 +274,67 @@ struct ReadArgs {
   int* status;
 };
 
-// One thread per (row, block of 16); a row that is skipped (slot < 0) reads as zeros.
-template <int D, typename T16>
+// One thread per (row, half block of 8): one 16-byte store for the key, one for the value, a warp's
+// stores contiguous.  A row that is skipped (slot < 0) reads as zeros.  A row costs two loads one after
+// the other (its slot, its codes): a thread takes U rows at once where there are rows enough.
+template <int D, typename T16, int U>
 __global__ void __launch_bounds__(256) kv4_read_kernel(ReadArgs a) {
   using L = Lay<D>;
   pdl_entry();
-  const long long idx = (long long)blockIdx.x * 256 + threadIdx.x;
-  const long long row = idx / L::NB;
-  if (row >= (long long)a.T * a.H) return;
-  const int b = (int)(idx % L::NB), bs = b % (L::SD / 16), slab = b / (L::SD / 16);
-  const int tok = (int)(row / a.H), h = (int)(row % a.H);
-  const long long slot = a.slots[tok];
-  if (slot >= a.n_slots) set_status(a.status, kBadIndex);
-  const bool live = slot >= 0 && slot < a.n_slots;
-  float x[16], y[16];
+  const int part = threadIdx.x % (2 * L::NB), b = part >> 1, half = part & 1;     // the same for every row
+  const int bs = b % (L::SD / 16), slab = b / (L::SD / 16);
+  constexpr int kRows = 256 / (2 * L::NB);                                        // of a block, at a time
+  const uint32_t row0 = blockIdx.x * (uint32_t)(kRows * U) + threadIdx.x / (2 * L::NB), rows = (uint32_t)a.T * a.H;
+  long long slot[U];
+  int h[U];
 #pragma unroll
-  for (int i = 0; i < 16; i++) x[i] = y[i] = 0.f;
-  if (live) {
-    const int j = (int)(slot % kPage);
-    const uint8_t* page = a.pages + ((slot / kPage) * a.H + h) * (long long)L::kPageBytes;
-    const float ks = e4m3_to_f32(page[L::KS + j * L::NB + b]) * a.k_mul;
-    const float vs = e4m3_to_f32(page[L::VS + (j >> 1) * (2 * L::NB) + 2 * b + (j & 1)]) * a.v_mul;
-    const uint8_t* kc = page + L::KC + slab * L::kSlabBytes + j * (L::SD / 2);
-    const uint8_t* vc = page + L::VC + slab * L::kSlabBytes + (j >> 1) * L::SD + (j & 1) * (L::SD / 16);
-    if constexpr (L::SD == 128) {
-      uint32_t c[4];
-      load_words<4>(kc + (bs >> 1) * 16, c);
-#pragma unroll
-      for (int w = 0; w < 4; w++) {      // this block's codes are the low or the high halves
-        float lo[4], hi[4];
-        values4(c[w], lo, hi);
-#pragma unroll
-        for (int i = 0; i < 4; i++) x[4 * w + i] = ((b & 1) ? hi[i] : lo[i]) * ks;
-      }
-      load_words<2>(vc + bs * 16, *reinterpret_cast<uint32_t(*)[2]>(c));
-      values4(c[0], y, y + 8);
-      values4(c[1], y + 4, y + 12);
-    } else {
-      uint32_t c[2];
-      load_words<2>(kc + bs * 8, c);
-      values4(c[0], x, x + 8);
-      values4(c[1], x + 4, x + 12);
-      values4(*reinterpret_cast<const uint32_t*>(vc + (2 * bs) * 8), y, y + 4);
-      values4(*reinterpret_cast<const uint32_t*>(vc + (2 * bs + 1) * 8), y + 8, y + 12);
-#pragma unroll
-      for (int i = 0; i < 16; i++) x[i] *= ks;
-    }
-#pragma unroll
-    for (int i = 0; i < 16; i++) y[i] *= vs;
+  for (int u = 0; u < U; u++) {
+    const uint32_t row = row0 + u * kRows, tok = row / (uint32_t)a.H;
+    h[u] = (int)(row - tok * a.H);
+    slot[u] = row < rows ? a.slots[tok] : -1;
   }
-  uint32_t o[8];
+  uint32_t kw[U][2], vw[U][2];
+  uint8_t k8[U], v8[U];
 #pragma unroll
-  for (int i = 0; i < 8; i++) o[i] = pack2<T16>(x[2 * i], x[2 * i + 1]);
-  uint4* dst = reinterpret_cast<uint4*>((T16*)a.k + row * D + b * 16);
-  dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
-  dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
+  for (int u = 0; u < U; u++) {
+    kw[u][0] = kw[u][1] = vw[u][0] = vw[u][1] = 0;
+    k8[u] = v8[u] = 0;
+    if (slot[u] >= a.n_slots) set_status(a.status, kBadIndex);
+    if (slot[u] >= 0 && slot[u] < a.n_slots) {
+      const int j = (int)(slot[u] % kPage);
+      const uint8_t* page = a.pages + ((slot[u] / kPage) * a.H + h[u]) * (long long)L::kPageBytes;
+      const uint8_t* kc = page + L::KC + slab * L::kSlabBytes + j * (L::SD / 2);
+      const uint8_t* vc = page + L::VC + slab * L::kSlabBytes + (j >> 1) * L::SD + (j & 1) * (L::SD / 16);
+      load_words<2>(kc + (L::SD == 128 ? (bs >> 1) * 16 + half * 8 : bs * 8), kw[u]);
+      if constexpr (L::SD == 128) load_words<2>(vc + bs * 16, vw[u]);
+      else vw[u][0] = *reinterpret_cast<const uint32_t*>(vc + (2 * bs + half) * 8);
+      k8[u] = page[L::KS + j * L::NB + b];
+      v8[u] = page[L::VS + (j >> 1) * (2 * L::NB) + 2 * b + (j & 1)];
+    }
+  }
 #pragma unroll
-  for (int i = 0; i < 8; i++) o[i] = pack2<T16>(y[2 * i], y[2 * i + 1]);
-  dst = reinterpret_cast<uint4*>((T16*)a.v + row * D + b * 16);
-  dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
-  dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
+  for (int u = 0; u < U; u++) {
+    const uint32_t row = row0 + u * kRows;
+    if (row >= rows) return;
+    const uint32_t ks = scale2(k8[u], a.k_mul), vs = scale2(v8[u], a.v_mul);
+    // SD = 128: a piece's low codes are one block's, its high codes the next block's; SD = 64: its two halves
+    const int up = 4 * (L::SD == 128 ? b & 1 : half);
+    uint32_t x[4], y[4];
+    values4(kw[u][0], up, x[0], x[1]);
+    values4(kw[u][1], up, x[2], x[3]);
+    if constexpr (L::SD == 128) {
+      values4(vw[u][0], 4 * half, y[0], y[1]);
+      values4(vw[u][1], 4 * half, y[2], y[3]);
+    } else {
+      values4(vw[u][0], 0, y[0], y[1]);
+      values4(vw[u][0], 4, y[2], y[3]);
+    }
+    const long long at = (long long)row * D + b * 16 + half * 8;
+    *reinterpret_cast<uint4*>((T16*)a.k + at) = make_uint4(out2<T16>(mul_f16x2(x[0], ks)), out2<T16>(mul_f16x2(x[1], ks)),
+                                                           out2<T16>(mul_f16x2(x[2], ks)), out2<T16>(mul_f16x2(x[3], ks)));
+    *reinterpret_cast<uint4*>((T16*)a.v + at) = make_uint4(out2<T16>(mul_f16x2(y[0], vs)), out2<T16>(mul_f16x2(y[1], vs)),
+                                                           out2<T16>(mul_f16x2(y[2], vs)), out2<T16>(mul_f16x2(y[3], vs)));
+  }
 }
 
 static int dim_of(const torch::Tensor& pages) { return (int)(pages.size(2) / 72); }
@@ -350,9 +367,9 @@ void kv4_append_launch(torch::Tensor k, torch::Tensor v, torch::Tensor slots, to
     using T16 = decltype(t);
     if (vec) launch_k(kv4_append_kernel<DD, T16, true>, grid, dim3(256), 0, stream, a);
     else launch_k(kv4_append_kernel<DD, T16, false>, grid, dim3(256), 0, stream, a);
-    BoundsArgs c{a.slots, T, H, a.n_slots, T >= 4096 ? 64 : 8, a.pages, (int8_t*)bounds.data_ptr(),
+    BoundsArgs c{a.slots, T, H, a.n_slots, T >= 4096 ? 64 : 2, a.pages, (int8_t*)bounds.data_ptr(),
                  (float*)unit.data_ptr(), std::ldexp(1.f, (int)k_exp)};
-    launch_k(kv4_bounds_kernel<DD>, dim3((T + c.win - 1) / c.win, H), dim3(256), 0, stream, c);
+    launch_k(kv4_bounds_kernel<DD>, dim3((T + c.win - 1) / c.win, H), dim3(64), 0, stream, c);
   };
   auto by_type = [&](auto dim) {
     if (k.scalar_type() == at::kHalf) go(dim, __half{});
@@ -371,12 +388,19 @@ void kv4_read_launch(torch::Tensor slots, torch::Tensor pages, int64_t k_exp, in
   ReadArgs a{(const long long*)slots.data_ptr(), T, H, pages.size(0) * kPage, (const uint8_t*)pages.data_ptr(),
              std::ldexp(1.f, (int)k_exp), std::ldexp(1.f, (int)v_exp), k.data_ptr(), v.data_ptr(),
              (int*)status.data_ptr()};
-  const long long threads = (long long)T * H * (D / 16);
-  const dim3 grid((unsigned)((threads + 255) / 256));
+  const long long threads = (long long)T * H * (D / 8);
+  const int per = threads >= 2ll * 148 * 2048 ? 4 : 1;
+  const dim3 grid((unsigned)((threads + 256 * per - 1) / (256 * per)));
+  auto launch = [&](auto dim, auto t, auto u) {
+    launch_k(kv4_read_kernel<decltype(dim)::value, decltype(t), decltype(u)::value>, grid, dim3(256), 0, stream, a);
+  };
+  auto by_type = [&](auto dim, auto u) {
+    if (k.scalar_type() == at::kHalf) launch(dim, __half{}, u);
+    else launch(dim, __nv_bfloat16{}, u);
+  };
   auto go = [&](auto dim) {
-    constexpr int DD = decltype(dim)::value;
-    if (k.scalar_type() == at::kHalf) launch_k(kv4_read_kernel<DD, __half>, grid, dim3(256), 0, stream, a);
-    else launch_k(kv4_read_kernel<DD, __nv_bfloat16>, grid, dim3(256), 0, stream, a);
+    if (per == 4) by_type(dim, std::integral_constant<int, 4>{});
+    else by_type(dim, std::integral_constant<int, 1>{});
   };
   if (D == 64) go(std::integral_constant<int, 64>{});
   else if (D == 128) go(std::integral_constant<int, 128>{});

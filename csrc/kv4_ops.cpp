@@ -112,7 +112,7 @@ void kv4_append(Tensor k, Tensor v, Tensor slots, Tensor pages, Tensor bounds, T
                     x->size(2) == c.D && (T == 0 || x->stride(2) == 1) && half_type(*x) && x->scalar_type() == k.scalar_type(),
                 "kv4: k and v must be bf16 or f16 [", num(T), ", ", num(c.H), ", ", num(c.D),
                 "] of one type, inner stride 1, on the cache's device");
-  TORCH_CHECK(T * c.H * (c.D / 16) < (int64_t)1 << 38, "kv4: too many rows for one call");
+  TORCH_CHECK(T * c.H < (int64_t)1 << 31, "kv4: too many rows for one call");
   if (T == 0) return;
   const c10::cuda::CUDAGuard guard(pages.device());
   kv4_append_launch(k, v, slots, pages, bounds, unit, k_exp, v_exp, status);
@@ -123,6 +123,7 @@ std::tuple<Tensor, Tensor> kv4_read(Tensor slots, at::ScalarType dtype, Tensor p
   const Cache c = check_cache(pages, bounds, unit, status, k_exp, v_exp);
   check_slots(slots, pages);
   TORCH_CHECK(dtype == at::kBFloat16 || dtype == at::kHalf, "kv4: read gives bf16 or f16");
+  TORCH_CHECK(slots.size(0) * c.H < (int64_t)1 << 31, "kv4: too many rows for one call");
   const c10::cuda::CUDAGuard guard(pages.device());
   const auto opt = pages.options().dtype(dtype);
   Tensor k = at::empty({slots.size(0), c.H, c.D}, opt), v = at::empty({slots.size(0), c.H, c.D}, opt);

@@ -561,3 +561,13 @@ def test_refusals(KV4Cache):
             pytest.fail(f"call {i} was not refused")
     c.check()
     assert torch.isfinite(c.attend(q, cu, sl, tb, 0.1)).all()        # and the cache still works
+
+
+def test_demo_layer_from_prompt_to_decode():
+    """The draft layer of `tools.kv4_demo`: 4-bit keys and values cost what they cost (two e2m1 roundings of
+    about 2^-3.3 relative each, averaged over thousands of positions), choosing all pages changes nothing."""
+    from vllm_moet_b200.tools.kv4_demo import run
+    got = run(hidden=512, heads=8, kv_heads=2, head_dim=64, streams=2, prompt=700, chunk=256, tokens=6, budget=64, sink=None)
+    assert got["bytes_per_position"] * 32 == got["bf16_bytes_per_position"] * 9
+    assert got["all_pages_rel_err"] < 0.2
+    assert abs(got["chosen_pages_rel_err"] - got["all_pages_rel_err"]) < 2e-3      # 64 pages hold every position
