@@ -20,6 +20,8 @@
 #include "tcgen05.cuh"
 #include "torch_glue.h"
 
+#include <algorithm>
+
 namespace moet {
 namespace kv4 {
 
@@ -29,6 +31,8 @@ struct PromptArgs {
   const uint8_t* pages; int n_pages;
   float scale_log2, v_mul;
   void* out; float* lse;
+  int tiles, splits;                  // row tiles of the longest sequence; stretches of a tile's keys
+  float* part;                        // with splits > 1: their outputs, maxima and sums
   int* status;
 };
 
@@ -131,6 +135,11 @@ template <> MOET_DEVICE uint32_t down2<__half>(float a, float b) { return f16x2(
 template <> MOET_DEVICE uint32_t down2<__nv_bfloat16>(float a, float b) { return pack_bf16x2(a, b); }
 }  // namespace pr
 
+// where the part of one stretch of a tile's keys lies: rows x D outputs, then the rows' maxima and sums
+template <int D> MOET_DEVICE long long prompt_part(const PromptArgs& a, int b, int h, int tile, int split) {
+  return ((((long long)b * a.H + h) * a.tiles + tile) * a.splits + split) * (PromptCfg<D>::TILES * 128 * (D + 2));
+}
+
 // scores of keys j0 .. that the row at position p does not see -> -inf
 template <int N> MOET_DEVICE void hide(uint32_t (&u)[N], int j0, int p, int window) {
 #pragma unroll
@@ -153,15 +162,17 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
   const int c0 = max(0, min(a.cu_q[b], a.T)), nq = max(0, max(0, min(a.cu_q[b + 1], a.T)) - c0);
   const int rows = nq * a.G, p0 = min(a.seq_lens[b], a.W * kPage) - nq;
   const int ntiles_seq = (rows + TILES * 128 - 1) / (TILES * 128);
-  const int tile = ntiles_seq - 1 - (int)blockIdx.x;               // the longest stretches of keys first
+  const int tile = ntiles_seq - 1 - (int)(blockIdx.x / a.splits), split = blockIdx.x % a.splits;   // the longest first
   if (tile < 0) return;
   const int row0 = tile * TILES * 128, live = min(rows - row0, TILES * 128);
   const int p_first = p0 + row0 / a.G, p_last = p0 + (row0 + live - 1) / a.G;
   const int ntile = (live + 127) / 128;
-  const int kb0 = a.window > 0 ? max(0, p_first - a.window + 1) / BK : 0;
-  const int kb1 = p_last < 0 ? kb0 : p_last / BK + 1;              // key blocks [kb0, kb1)
+  const int from = a.window > 0 ? max(0, p_first - a.window + 1) / BK : 0;
+  const int to = p_last < 0 ? from : p_last / BK + 1;              // the tile's key blocks [from, to), shared out evenly
+  const int per = (to - from + a.splits - 1) / a.splits;
+  const int kb0 = min(to, from + split * per), kb1 = min(to, kb0 + per);
   const int nkb = kb1 - kb0;
-  const int steps = nkb > 0 ? p_last / C::SK + 1 - kb0 * C::HALVES : 0;   // softmax steps
+  const int steps = nkb > 0 ? min(p_last / C::SK + 1, kb1 * C::HALVES) - kb0 * C::HALVES : 0;   // softmax steps
 
   // ---- queries as f16 operands (bf16 rows scaled to at most 512), barriers, tensor memory
   if (warp == 0) tc::tmem_alloc(&sm.tmem, 512);
@@ -312,17 +323,23 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
       if (ok) {
         tc::fence_after();
         const float inv = l > 0.f ? __fdividef(a.v_mul, l) : l;
+        float* part = nullptr;
+        if (a.splits > 1) {
+          part = a.part + prompt_part<D>(a, b, h, tile, split);
+          part[TILES * 128 * D + r] = m;
+          part[TILES * 128 * (D + 1) + r] = l;
+        }
         const long long at = (long long)(c0 + row / a.G) * a.H * a.G + h * a.G + row % a.G;
         const bool on = r < live;
         constexpr int E = L::SD / 8;         // values of a lane's piece; column (i, g) of a slab = value E g + i
 #pragma unroll
         for (int sl = 0; sl < L::NS; sl++)
 #pragma unroll
-          for (int part = 0; part < E / 8; part++) {      // 64 columns: values i = 8 part .. + 7 of all pieces
+          for (int part_i = 0; part_i < E / 8; part_i++) {      // 64 columns: values i = 8 part_i .. + 7 of all pieces
             uint32_t u[2][32];
             if (nkb > 0) {
-              pr::ld32(o_at + sl * L::SD + part * 64, u[0]);
-              pr::ld32(o_at + sl * L::SD + part * 64 + 32, u[1]);
+              pr::ld32(o_at + sl * L::SD + part_i * 64, u[0]);
+              pr::ld32(o_at + sl * L::SD + part_i * 64 + 32, u[1]);
               tc::tmem_wait_ld();
             } else {
 #pragma unroll
@@ -333,14 +350,24 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
               for (int g = 0; g < 8; g++) {
                 float x[8];
 #pragma unroll
-                for (int k = 0; k < 8; k++) x[k] = __uint_as_float(u[(k * 8 + g) >> 5][(k * 8 + g) & 31]) * inv;
-                *reinterpret_cast<uint4*>((T16*)a.out + at * D + sl * L::SD + E * g + part * 8) =
+                for (int k = 0; k < 8; k++) x[k] = __uint_as_float(u[(k * 8 + g) >> 5][(k * 8 + g) & 31]);
+                if (part) {                  // as it is: the join divides
+                  if (nkb > 0) {
+                    float4* to4 = reinterpret_cast<float4*>(part + r * D + sl * L::SD + E * g + part_i * 8);
+                    to4[0] = make_float4(x[0], x[1], x[2], x[3]);
+                    to4[1] = make_float4(x[4], x[5], x[6], x[7]);
+                  }
+                  continue;
+                }
+#pragma unroll
+                for (int k = 0; k < 8; k++) x[k] *= inv;
+                *reinterpret_cast<uint4*>((T16*)a.out + at * D + sl * L::SD + E * g + part_i * 8) =
                     make_uint4(pr::down2<T16>(x[0], x[1]), pr::down2<T16>(x[2], x[3]), pr::down2<T16>(x[4], x[5]),
                                pr::down2<T16>(x[6], x[7]));
               }
             }
           }
-        if (on && a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.6931471805599453f;
+        if (on && a.lse && !part) a.lse[at] = l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.6931471805599453f;
       }
     }
   } else if (warp < C::kSoftWarps + 4) {
@@ -519,15 +546,66 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
   }
 }
 
+// Joins a tile's stretches, in their order: a thread per 8 values of a row.
+template <int D, typename T16>
+__global__ void __launch_bounds__(256) kv4_prompt_join_kernel(PromptArgs a) {
+  constexpr int RT = PromptCfg<D>::TILES * 128;
+  pdl_entry();
+  const int b = blockIdx.z / a.H, h = blockIdx.z % a.H, tile = blockIdx.y;
+  const int it = blockIdx.x * 256 + threadIdx.x, r = it / (D / 8), d = it % (D / 8) * 8;
+  const int c0 = max(0, min(a.cu_q[b], a.T)), nq = max(0, max(0, min(a.cu_q[b + 1], a.T)) - c0);
+  const int row = tile * RT + r;
+  if (row >= nq * a.G) return;
+  const float* p = a.part + prompt_part<D>(a, b, h, tile, 0);
+  constexpr int PF = RT * (D + 2);
+  float M = -INFINITY;
+  for (int s = 0; s < a.splits; s++) M = fmaxf(M, p[s * PF + RT * D + r]);
+  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, sum = 0.f;
+#pragma unroll 2
+  for (int s = 0; s < a.splits; s++) {
+    const float m = p[s * PF + RT * D + r], l = p[s * PF + RT * (D + 1) + r];
+    if (m == -INFINITY && l == 0.f) continue;          // a stretch of which the row saw nothing
+    const float w = m == -INFINITY ? 1.f : pr::exp2_fast(m - M);   // NaN sums have no maximum
+    const float4 y = *reinterpret_cast<const float4*>(p + s * PF + r * D + d), z = *reinterpret_cast<const float4*>(p + s * PF + r * D + d + 4);
+    x[0] += w * y.x, x[1] += w * y.y, x[2] += w * y.z, x[3] += w * y.w;
+    x[4] += w * z.x, x[5] += w * z.y, x[6] += w * z.z, x[7] += w * z.w;
+    sum += w * l;
+  }
+  const float inv = sum > 0.f ? __fdividef(a.v_mul, sum) : sum;
+  const long long at = (long long)(c0 + row / a.G) * a.H * a.G + h * a.G + row % a.G;
+  *reinterpret_cast<uint4*>((T16*)a.out + at * D + d) =
+      make_uint4(pr::down2<T16>(x[0] * inv, x[1] * inv), pr::down2<T16>(x[2] * inv, x[3] * inv),
+                 pr::down2<T16>(x[4] * inv, x[5] * inv), pr::down2<T16>(x[6] * inv, x[7] * inv));
+  if (a.lse && d == 0) a.lse[at] = sum == 0.f ? -INFINITY : (M + __log2f(sum)) * 0.6931471805599453f;
+}
+
+static int64_t prompt_tiles(int64_t T, int64_t G, int64_t D, int64_t max_q) {
+  const int64_t rt = D == 256 ? 128 : 256;
+  return (std::min(max_q, T) * G + rt - 1) / rt;
+}
+
 }  // namespace kv4
 }  // namespace moet
 
 using namespace moet;
 using namespace moet::kv4;
 
+// Stretches into which a tile's keys are split: where the tiles alone leave SMs empty, as many as fill
+// them, of at least 512 keys (below that a stretch's set-up, about 5 us, outweighs its keys).
+int64_t kv4_prompt_splits(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t max_q, int64_t W, int64_t window) {
+  const int64_t all = prompt_tiles(T, G, D, max_q) * H * B;
+  const int64_t keys = window > 0 ? std::min(W * kPage, window + max_q) : W * kPage;
+  return std::max<int64_t>(1, std::min({(int64_t)148 / all, keys / 512, (int64_t)64}));
+}
+// floats of `part` for so many stretches
+int64_t kv4_prompt_workspace(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t max_q, int64_t splits) {
+  return splits == 1 ? 0 : prompt_tiles(T, G, D, max_q) * H * B * splits * (D == 256 ? 128 : 256) * (D + 2);
+}
+
 void kv4_prompt_launch(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_lens, torch::Tensor table,
                        torch::Tensor pages, double scale, int64_t max_q, int64_t window, int64_t k_exp, int64_t v_exp,
-                       torch::Tensor out, c10::optional<torch::Tensor> lse, torch::Tensor status) {
+                       torch::Tensor out, c10::optional<torch::Tensor> lse, int64_t splits,
+                       c10::optional<torch::Tensor> part, torch::Tensor status) {
   PromptArgs a;
   const int D = (int)(pages.size(2) / 72);
   a.T = (int)q.size(0); a.H = (int)pages.size(1); a.G = (int)(q.size(1) / a.H);
@@ -540,16 +618,19 @@ void kv4_prompt_launch(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_le
   a.v_mul = std::ldexp(1.f, (int)v_exp);
   a.out = out.data_ptr(); a.lse = (float*)opt_ptr(lse);
   a.status = (int*)status.data_ptr();
-  TORCH_CHECK(a.H <= 65535, "kv4: too many heads");
+  a.tiles = (int)prompt_tiles(a.T, a.G, D, max_q); a.splits = (int)splits;
+  a.part = (float*)opt_ptr(part);
+  TORCH_CHECK(a.H <= 65535 && (splits == 1 || a.part), "kv4: too many heads, or no workspace");
   auto stream = at::cuda::getCurrentCUDAStream();
   auto go = [&](auto dim, auto t) {
     constexpr int DD = decltype(dim)::value;
     using T16 = decltype(t);
     using C = PromptCfg<DD>;
-    const int64_t rows = std::min<int64_t>(max_q, a.T) * a.G;
-    const dim3 grid((unsigned)((rows + C::TILES * 128 - 1) / (C::TILES * 128)), a.H, a.B);
+    const dim3 grid((unsigned)(a.tiles * a.splits), a.H, a.B);
     moet_allow_max_smem(kv4_prompt_kernel<DD, T16>);
     launch_k(kv4_prompt_kernel<DD, T16>, grid, dim3(C::kWarps * 32), sizeof(PromptSmem<DD>), stream, a);
+    if (a.splits > 1)     // at most 148 tiles
+      launch_k(kv4_prompt_join_kernel<DD, T16>, dim3(C::TILES * 128 * DD / 8 / 256, a.tiles, a.B * a.H), dim3(256), 0, stream, a);
   };
   auto by_type = [&](auto dim) {
     if (q.scalar_type() == at::kHalf) go(dim, __half{});

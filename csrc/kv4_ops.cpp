@@ -4,6 +4,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include <algorithm>
 #include <map>
 #include <mutex>
 #include <string>
@@ -21,7 +22,10 @@ void kv4_attend_launch(Tensor q, Tensor cu_q, Tensor seq_lens, Tensor table, Ten
                        double scale, int64_t max_q, int64_t window, int64_t k_exp, int64_t v_exp, Tensor out,
                        optional<Tensor> lse, Tensor part, Tensor split, Tensor status);
 void kv4_prompt_launch(Tensor q, Tensor cu_q, Tensor seq_lens, Tensor table, Tensor pages, double scale, int64_t max_q,
-                       int64_t window, int64_t k_exp, int64_t v_exp, Tensor out, optional<Tensor> lse, Tensor status);
+                       int64_t window, int64_t k_exp, int64_t v_exp, Tensor out, optional<Tensor> lse, int64_t splits,
+                       optional<Tensor> part, Tensor status);
+int64_t kv4_prompt_splits(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t max_q, int64_t W, int64_t window);
+int64_t kv4_prompt_workspace(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t max_q, int64_t splits);
 
 namespace {
 
@@ -90,13 +94,15 @@ std::pair<Tensor, Tensor> workspace(const Tensor& like, int64_t floats, int64_t 
   const auto stream = c10::cuda::getCurrentCUDAStream();
   cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
   C10_CUDA_CHECK(cudaStreamIsCapturing(stream, &capturing));
-  const auto make = [&] {
-    return std::make_pair(at::empty({floats}, like.options().dtype(at::kFloat)), at::empty({ints}, like.options().dtype(at::kInt)));
+  const auto make = [&](int64_t f, int64_t n) {
+    return std::make_pair(at::empty({f}, like.options().dtype(at::kFloat)), at::empty({n}, like.options().dtype(at::kInt)));
   };
-  if (capturing != cudaStreamCaptureStatusNone) return make();
+  if (capturing != cudaStreamCaptureStatusNone) return make(floats, ints);
   std::lock_guard<std::mutex> lock(mu);
   auto& w = (*kept)[{like.get_device(), (void*)stream.stream()}];
-  if (!w.first.defined() || w.first.numel() < floats || w.second.numel() < ints) w = make();
+  if (!w.first.defined()) w = make(floats, ints);
+  if (w.first.numel() < floats || w.second.numel() < ints)
+    w = make(std::max(floats, w.first.numel()), std::max(ints, w.second.numel()));
   return w;
 }
 
@@ -167,7 +173,10 @@ std::tuple<Tensor, optional<Tensor>> kv4_attend(Tensor q, Tensor cu_q, Tensor se
   if (return_lse) lse = at::empty({T, q.size(1)}, unit.options());
   if (T) {
     if (!chosen.has_value() && max_q * G > kPromptRows) {
-      kv4_prompt_launch(q, cu_q, seq_lens, table, pages, scale, max_q, window, k_exp, v_exp, out, lse, status);
+      const int64_t B = seq_lens.size(0), splits = kv4_prompt_splits(T, B, c.H, G, c.D, max_q, table.size(1), window);
+      optional<Tensor> part;
+      if (splits > 1) part = workspace(pages, kv4_prompt_workspace(T, B, c.H, G, c.D, max_q, splits), 0).first;
+      kv4_prompt_launch(q, cu_q, seq_lens, table, pages, scale, max_q, window, k_exp, v_exp, out, lse, splits, part, status);
     } else {
       const auto [floats, ints] = kv4_attend_workspace(G, c.D, max_q, chosen.has_value());
       auto [part, split] = workspace(pages, floats, ints);
