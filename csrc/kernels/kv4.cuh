@@ -75,18 +75,21 @@ template <typename T16> MOET_DEVICE float to_f32(T16 x);
 template <> MOET_DEVICE float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
 template <> MOET_DEVICE float to_f32(__half x) { return __half2float(x); }
 
-// the two scale bytes of a lane's key codes: `row` = the token's scales, sl the slab, t the piece
+// the scale bytes of a lane's key codes, as they are held (two, or one with SD = 64): `row` = the
+// token's scales, sl the slab, t the piece; and the f16x2 they stand for
 template <int D> MOET_DEVICE uint16_t raw_key_scales(const uint8_t* row, int sl, int t) {
   if constexpr (Lay<D>::SD == 128) return *reinterpret_cast<const uint16_t*>(row + sl * 8 + 2 * t);
-  const uint32_t b = row[t];
-  return (uint16_t)(b | b << 8);
+  return row[t];
+}
+template <int D> MOET_DEVICE uint32_t key_scales_f16(uint16_t raw) {
+  return e4m3x2_to_f16(Lay<D>::SD == 128 ? raw : (uint16_t)(raw | raw << 8));
 }
 // of a lane's value codes, one per token of the pair: `row` = the pair's scales, g the piece
 template <int D> MOET_DEVICE uint16_t raw_value_scales(const uint8_t* row, int sl, int g) {
   return *reinterpret_cast<const uint16_t*>(row + 2 * (Lay<D>::SD == 128 ? sl * 8 + g : g >> 1));
 }
 template <int D> MOET_DEVICE uint32_t key_scales(const uint8_t* row, int sl, int t) {
-  return e4m3x2_to_f16(raw_key_scales<D>(row, sl, t));
+  return key_scales_f16<D>(raw_key_scales<D>(row, sl, t));
 }
 template <int D> MOET_DEVICE uint32_t value_scales(const uint8_t* row, int sl, int g) {
   return e4m3x2_to_f16(raw_value_scales<D>(row, sl, g));

@@ -666,12 +666,12 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(AttendArgs a) {
   const float ref = fm[r] == -INFINITY ? 0.f : fm[r];
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-  for (int p = grp; p < parts; p += GROUPS) {
+  for (int p = grp; p < parts && grp < GROUPS; p += GROUPS) {     // 24 rows leave the last 64 threads over
     const float w = fast_exp2(__ldcg(at(p) + RT * D + r) - ref);
     const float4 y = __ldcg(reinterpret_cast<const float4*>(at(p) + r * D + d));
     x.x += w * y.x, x.y += w * y.y, x.z += w * y.z, x.w += w * y.w;
   }
-  sum[grp][it] = x;
+  if (grp < GROUPS) sum[grp][it] = x;
   __syncthreads();
   if (grp || row0 + r >= rows) return;
 #pragma unroll
@@ -695,7 +695,9 @@ static int sm_count() {
 }
 
 // query rows of a tile / 8: the fewest that hold a sequence's rows, as the registers allow
-static int row_tiles(int64_t rows, int D) { return rows <= 8 ? 1 : (rows <= 16 || D == 256) ? 2 : 4; }
+static int row_tiles(int64_t rows, int D) {
+  return rows <= 8 ? 1 : (rows <= 16 || D == 256) ? 2 : rows <= 24 ? 3 : 4;
+}
 
 }  // namespace kv4
 }  // namespace moet
@@ -753,7 +755,10 @@ void kv4_attend_launch(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_le
     constexpr int DD = decltype(dim)::value;
     if (nt == 1) by_type(dim, std::integral_constant<int, 1>{});
     else if (nt == 2) by_type(dim, std::integral_constant<int, 2>{});
-    else if constexpr (DD != 256) by_type(dim, std::integral_constant<int, 4>{});
+    else if constexpr (DD != 256) {
+      if (nt == 3) by_type(dim, std::integral_constant<int, 3>{});
+      else by_type(dim, std::integral_constant<int, 4>{});
+    }
   };
   if (D == 64) by_rows(std::integral_constant<int, 64>{});
   else if (D == 128) by_rows(std::integral_constant<int, 128>{});

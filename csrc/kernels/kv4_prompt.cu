@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
 #pragma unroll
       for (int x = 0; x < KI; x++) {
         const int sl = x * 32 / BK, j = x * 32 % BK + kj;
-        const uint32_t f16s = e4m3x2_to_f16(ks[x]);
+        const uint32_t f16s = key_scales_f16<D>(ks[x]);
         uint8_t* dst = sm.k[st] + (j >> 3) * kKSbo + (j & 7) * 16 + (sl * (L::SD / 8) + kt * (E2 / 4)) * 128;
 #pragma unroll
         for (int w = 0; w < W; w++) {

@@ -152,8 +152,11 @@ Tensor kv4_select(Tensor q, Tensor cu_q, Tensor seq_lens, Tensor table, int64_t 
   return chosen;
 }
 
-// Query rows of one sequence and K/V head above which attention runs on the tcgen05 kernel.
-constexpr int64_t kPromptRows = 64;
+// Query rows of one sequence and K/V head above which attention runs on the tcgen05 kernel, which
+// converts each key and value once for 256 rows (128 with D = 256) where the other does for 32 (16).
+// us, other / tcgen05, 8 K/V heads, B200: 8 sequences of 30000, D = 128: 32 rows 211 / 215, 40 rows
+// 391 / 216; D = 256: 32 rows 317 / 377, 40 rows 458 / 380; 32 sequences of 4000, D = 64: 64 rows 126 / 132.
+int64_t prompt_rows(int64_t D) { return D == 64 ? 64 : 32; }
 
 std::tuple<Tensor, optional<Tensor>> kv4_attend(Tensor q, Tensor cu_q, Tensor seq_lens, Tensor table, double scale,
                                                 int64_t max_q, int64_t window, optional<Tensor> chosen, bool return_lse,
@@ -172,7 +175,7 @@ std::tuple<Tensor, optional<Tensor>> kv4_attend(Tensor q, Tensor cu_q, Tensor se
   optional<Tensor> lse;
   if (return_lse) lse = at::empty({T, q.size(1)}, unit.options());
   if (T) {
-    if (!chosen.has_value() && max_q * G > kPromptRows) {
+    if (!chosen.has_value() && max_q * G > prompt_rows(c.D)) {
       const int64_t B = seq_lens.size(0), splits = kv4_prompt_splits(T, B, c.H, G, c.D, max_q, table.size(1), window);
       optional<Tensor> part;
       if (splits > 1) part = workspace(pages, kv4_prompt_workspace(T, B, c.H, G, c.D, max_q, splits), 0).first;

@@ -208,6 +208,9 @@ STEP = [
     ([500], [4], 1, 6, 128, torch.bfloat16, 100),                     # window
     ([130, 64], [1, 1], 1, 40, 128, torch.bfloat16, 1),               # more heads than a tile; window of one
     ([777], [1], 4, 16, 256, torch.float16, 300),
+    ([900, 40], [3, 3], 1, 7, 128, torch.bfloat16, 0),                # three row groups of eight
+    ([3000], [3], 1, 8, 64, torch.bfloat16, 0),                       # and split over blocks
+    ([700], [4], 2, 8, 128, torch.float16, 0),
 ]
 PROMPT = [
     ([100], [100], 1, 1, 64, torch.bfloat16, 0),
@@ -216,6 +219,9 @@ PROMPT = [
     ([257, 0], [33, 3], 2, 8, 64, torch.float16, 0),
     ([450], [90], 1, 4, 128, torch.bfloat16, 37),
     ([129], [129], 1, 3, 128, torch.float16, 64),
+    ([3000], [60], 1, 2, 64, torch.bfloat16, 0),                      # a tile's keys split over blocks
+    ([2100, 1030], [40, 40], 1, 2, 256, torch.bfloat16, 0),
+    ([2500], [40], 1, 1, 128, torch.float16, 1100),
 ]
 
 
