@@ -95,6 +95,13 @@ template <int D> MOET_DEVICE uint32_t value_scales(const uint8_t* row, int sl, i
   return e4m3x2_to_f16(raw_value_scales<D>(row, sl, g));
 }
 
+// The grid's threads fetch `bytes` from p on into L2, a line each as far as they reach.  A prefetch uses
+// no value, so it may come before the wait for the kernel that is still writing there.
+MOET_DEVICE void grid_prefetch(const void* p, long long bytes) {
+  const long long at = ((long long)(blockIdx.x + gridDim.x * blockIdx.y) * blockDim.x + threadIdx.x) * 128;
+  if (at < bytes) prefetch_l2(static_cast<const uint8_t*>(p) + at);
+}
+
 MOET_DEVICE float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }   // -126 <= e <= 127
 
 // Smallest e >= -100 with amax <= 127 * 2^e; 0 for amax = 0 (finite amax >= 0).

@@ -225,8 +225,11 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, NT>()) kv4_atten
     for (int i = 0; i < NSLOT; i++) tc::mbar_init(&sm.bar[warp][i], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  // what is read first is fetched into L2 while the kernel before still runs (a prefetch uses no value)
-  if (tid == 0) prefetch_l2(a.q), prefetch_l2(a.seq_lens), prefetch_l2(a.cu_q), prefetch_l2(a.table);
+  // what is read first is fetched into L2 while the kernel before still runs
+  grid_prefetch(a.seq_lens, a.B * 4ll);
+  grid_prefetch(a.cu_q, a.B * 4ll);
+  grid_prefetch(a.table, (long long)a.B * a.W * 4);
+  grid_prefetch(a.q, ((long long)(a.T - 1) * a.q_tok + (a.H * a.G - 1ll) * a.q_head + D) * 2);
   pdl_entry();
 
   // the line of units: prefix sums over the sequences (all pages), or over nothing (chosen pages)

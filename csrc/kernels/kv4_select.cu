@@ -62,6 +62,10 @@ __global__ void __launch_bounds__(kScoreWarps * 32) kv4_score_kernel(SelectArgs 
   constexpr int kChunk = kScoreWarps * 16;
   __shared__ __align__(16) int8_t rows[kScoreRows * STRIDE];
   __shared__ float unit_q[kScoreRows];
+  grid_prefetch(a.seq_lens, a.B * 4ll);
+  grid_prefetch(a.cu_q, a.B * 4ll);
+  grid_prefetch(a.table, (long long)a.B * a.W * 4);
+  grid_prefetch(a.q, ((long long)(a.T - 1) * a.q_tok + (a.H * a.G - 1ll) * a.q_head + D) * 2);
   pdl_entry();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int spans = (a.chunks + a.span - 1) / a.span;
@@ -78,25 +82,34 @@ __global__ void __launch_bounds__(kScoreWarps * 32) kv4_score_kernel(SelectArgs 
   // 16 pages per warp and chunk; the first ones come while the rows are converted
   uint4 x[2][CH];
   float u[2];
-  auto fetch = [&](int pg) {
+  int phys[2];
+  auto look_up = [&](int pg) {
 #pragma unroll
     for (int i = 0; i < 2; i++) {
       const int page = pg + g + 8 * i;
-      int phys = 0;
-      if (page < end) {                                    // end <= W
-        phys = a.table[(long long)b * a.W + page];
-        if (phys < 0 || phys >= a.n_pages) {
-          set_status(a.status, kBadIndex);
-          phys = 0;
-        }
-      }
-      const int8_t* p = a.bounds + ((long long)phys * a.H + h) * KB + t * 16;
-#pragma unroll
-      for (int c = 0; c < CH; c++) x[i][c] = *reinterpret_cast<const uint4*>(p + c * 64);
-      u[i] = a.unit[(long long)phys * a.H + h];
+      phys[i] = page < end ? a.table[(long long)b * a.W + page] : 0;      // end <= W
     }
   };
-  fetch(chunk0 * kChunk + warp * 16);
+  auto row_of = [&](int i) {
+    if (phys[i] < 0 || phys[i] >= a.n_pages) {
+      set_status(a.status, kBadIndex);
+      phys[i] = 0;
+    }
+    return ((long long)phys[i] * a.H + h) * KB;
+  };
+  auto fetch = [&]() {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const int8_t* p = a.bounds + row_of(i) + t * 16;
+#pragma unroll
+      for (int c = 0; c < CH; c++) x[i][c] = *reinterpret_cast<const uint4*>(p + c * 64);
+      u[i] = a.unit[(long long)phys[i] * a.H + h];
+    }
+  };
+  look_up(chunk0 * kChunk + warp * 16);
+  fetch();
+  const bool more = a.span > 1;
+  if (more) look_up((chunk0 + 1) * kChunk + warp * 16);
 
   // ---- rows: r = round(q / f) as [max(r, 0) | min(r, 0)]; a place without a row repeats the token's first
   const int gp = GP == 16 ? a.gp : GP, nrows = ntok * gp;
@@ -139,7 +152,17 @@ __global__ void __launch_bounds__(kScoreWarps * 32) kv4_score_kernel(SelectArgs 
   for (int chunk = chunk0; chunk < chunk1; chunk++) {
     const int pg = chunk * kChunk + warp * 16;
     if (pg >= end) return;
-    if (chunk > chunk0) fetch(pg);
+    if (chunk > chunk0) {
+      fetch();
+      if (chunk + 1 < chunk1) look_up(pg + kChunk);
+    }
+    if (chunk + 1 < chunk1) {                              // the next chunk's bounds on their way to L2
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const int8_t* p = a.bounds + row_of(i);
+        if (t * 128 < KB) prefetch_l2(p + t * 128);
+      }
+    }
     const bool in0 = pg + g < end, in1 = pg + g + 8 < end;
     float* out = a.score + ((long long)(c0 + i0) * a.H + h) * a.W + pg + g;     // + token * H * W
     float best0 = -INFINITY, best1 = -INFINITY;
