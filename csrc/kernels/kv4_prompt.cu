@@ -21,6 +21,7 @@
 #include "torch_glue.h"
 
 #include <algorithm>
+#include <tuple>
 
 namespace moet {
 namespace kv4 {
@@ -31,8 +32,8 @@ struct PromptArgs {
   const uint8_t* pages; int n_pages;
   float scale_log2, v_mul;
   void* out; float* lse;
-  int tiles, splits;                  // row tiles of the longest sequence; stretches of a tile's keys
-  float* part;                        // with splits > 1: their outputs, maxima and sums
+  int whole, splits;                  // tiles that a block takes whole, stretches of keys of each of the others
+  float* part;                        // the stretches' outputs, maxima and sums
   int* status;
 };
 
@@ -136,8 +137,8 @@ template <> MOET_DEVICE uint32_t down2<__nv_bfloat16>(float a, float b) { return
 }  // namespace pr
 
 // where the part of one stretch of a tile's keys lies: rows x D outputs, then the rows' maxima and sums
-template <int D> MOET_DEVICE long long prompt_part(const PromptArgs& a, int b, int h, int tile, int split) {
-  return ((((long long)b * a.H + h) * a.tiles + tile) * a.splits + split) * (PromptCfg<D>::TILES * 128 * (D + 2));
+template <int D> MOET_DEVICE long long prompt_part(const PromptArgs& a, int entry, int split) {
+  return ((long long)entry * a.splits + split) * (PromptCfg<D>::TILES * 128 * (D + 2));
 }
 
 // scores of keys j0 .. that the row at position p does not see -> -inf
@@ -158,18 +159,22 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_entry();
 
-  const int b = blockIdx.z, h = blockIdx.y;
+  // tiles in order: the longest stretches of keys (a sequence's last rows) of every sequence and head first
+  const int entry = (int)blockIdx.x < a.whole ? blockIdx.x : a.whole + (int)(blockIdx.x - a.whole) / a.splits;
+  const int split = (int)blockIdx.x < a.whole ? 0 : (int)(blockIdx.x - a.whole) % a.splits;
+  const int splits = (int)blockIdx.x < a.whole ? 1 : a.splits;
+  const int b = entry % a.B, h = entry / a.B % a.H, back = entry / (a.B * a.H);
   const int c0 = max(0, min(a.cu_q[b], a.T)), nq = max(0, max(0, min(a.cu_q[b + 1], a.T)) - c0);
   const int rows = nq * a.G, p0 = min(a.seq_lens[b], a.W * kPage) - nq;
   const int ntiles_seq = (rows + TILES * 128 - 1) / (TILES * 128);
-  const int tile = ntiles_seq - 1 - (int)(blockIdx.x / a.splits), split = blockIdx.x % a.splits;   // the longest first
+  const int tile = ntiles_seq - 1 - back;
   if (tile < 0) return;
   const int row0 = tile * TILES * 128, live = min(rows - row0, TILES * 128);
   const int p_first = p0 + row0 / a.G, p_last = p0 + (row0 + live - 1) / a.G;
   const int ntile = (live + 127) / 128;
   const int from = a.window > 0 ? max(0, p_first - a.window + 1) / BK : 0;
   const int to = p_last < 0 ? from : p_last / BK + 1;              // the tile's key blocks [from, to), shared out evenly
-  const int per = (to - from + a.splits - 1) / a.splits;
+  const int per = (to - from + splits - 1) / splits;
   const int kb0 = min(to, from + split * per), kb1 = min(to, kb0 + per);
   const int nkb = kb1 - kb0;
   const int steps = nkb > 0 ? min(p_last / C::SK + 1, kb1 * C::HALVES) - kb0 * C::HALVES : 0;   // softmax steps
@@ -324,8 +329,8 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
         tc::fence_after();
         const float inv = l > 0.f ? __fdividef(a.v_mul, l) : l;
         float* part = nullptr;
-        if (a.splits > 1) {
-          part = a.part + prompt_part<D>(a, b, h, tile, split);
+        if (splits > 1) {
+          part = a.part + prompt_part<D>(a, entry - a.whole, split);
           part[TILES * 128 * D + r] = m;
           part[TILES * 128 * (D + 1) + r] = l;
         }
@@ -551,12 +556,12 @@ template <int D, typename T16>
 __global__ void __launch_bounds__(256) kv4_prompt_join_kernel(PromptArgs a) {
   constexpr int RT = PromptCfg<D>::TILES * 128;
   pdl_entry();
-  const int b = blockIdx.z / a.H, h = blockIdx.z % a.H, tile = blockIdx.y;
+  const int entry = a.whole + blockIdx.y, b = entry % a.B, h = entry / a.B % a.H, back = entry / (a.B * a.H);
   const int it = blockIdx.x * 256 + threadIdx.x, r = it / (D / 8), d = it % (D / 8) * 8;
   const int c0 = max(0, min(a.cu_q[b], a.T)), nq = max(0, max(0, min(a.cu_q[b + 1], a.T)) - c0);
-  const int row = tile * RT + r;
-  if (row >= nq * a.G) return;
-  const float* p = a.part + prompt_part<D>(a, b, h, tile, 0);
+  const int tile = (nq * a.G + RT - 1) / RT - 1 - back, row = tile * RT + r;
+  if (tile < 0 || row >= nq * a.G) return;
+  const float* p = a.part + prompt_part<D>(a, blockIdx.y, 0);
   constexpr int PF = RT * (D + 2);
   float M = -INFINITY;
   for (int s = 0; s < a.splits; s++) M = fmaxf(M, p[s * PF + RT * D + r]);
@@ -590,22 +595,35 @@ static int64_t prompt_tiles(int64_t T, int64_t G, int64_t D, int64_t max_q) {
 using namespace moet;
 using namespace moet::kv4;
 
-// Stretches into which a tile's keys are split: where the tiles alone leave SMs empty, as many as fill
-// them, of at least 512 keys (below that a stretch's set-up, about 5 us, outweighs its keys).
-int64_t kv4_prompt_splits(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t max_q, int64_t W, int64_t window) {
-  const int64_t all = prompt_tiles(T, G, D, max_q) * H * B;
+// {tiles taken whole, stretches of keys of each of the others, floats of `part`}.  Tiles that fill all SMs
+// are taken whole.  The rest (all, where there are fewer tiles than SMs) would leave SMs idle: its keys
+// are split so that the last wave is even, into stretches of at least 512 keys (below that a stretch's
+// set-up, about 5 us, outweighs its keys), unless four or more waves come before it.
+// 2048 x 4 rows, 8 heads, 16384 keys: 256 tiles, 556 us whole, 550 us with the last 108 in
+// quarters; with D = 256 (512 tiles) 1289 and 1092 us.
+std::tuple<int64_t, int64_t, int64_t> kv4_prompt_plan(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t max_q,
+                                                      int64_t W, int64_t window) {
+  constexpr int64_t kSms = 148;
+  const int64_t n = prompt_tiles(T, G, D, max_q) * H * B, rest = n % kSms;
   const int64_t keys = window > 0 ? std::min(W * kPage, window + max_q) : W * kPage;
-  return std::max<int64_t>(1, std::min({(int64_t)148 / all, keys / 512, (int64_t)64}));
-}
-// floats of `part` for so many stretches
-int64_t kv4_prompt_workspace(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t max_q, int64_t splits) {
-  return splits == 1 ? 0 : prompt_tiles(T, G, D, max_q) * H * B * splits * (D == 256 ? 128 : 256) * (D + 2);
+  if (rest == 0 || n >= 4 * kSms) return {n, 1, 0};
+  int64_t best = 1;
+  if (n < kSms) {
+    best = std::min<int64_t>({kSms / n, keys / 512, 64});
+  } else {
+    for (int64_t s = 2; s <= std::min<int64_t>(keys / 512, 8); s++) {       // waves of stretches / s, 3 % for a split
+      const auto cost = [&](int64_t x) { return (double)((rest * x + kSms - 1) / kSms) / x + 0.03 * (x - 1); };
+      if (cost(s) < cost(best)) best = s;
+    }
+  }
+  if (best <= 1) return {n, 1, 0};
+  return {n - rest, best, rest * best * (D == 256 ? 128 : 256) * (D + 2)};
 }
 
 void kv4_prompt_launch(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_lens, torch::Tensor table,
                        torch::Tensor pages, double scale, int64_t max_q, int64_t window, int64_t k_exp, int64_t v_exp,
-                       torch::Tensor out, c10::optional<torch::Tensor> lse, int64_t splits,
-                       c10::optional<torch::Tensor> part, torch::Tensor status) {
+                       torch::Tensor out, c10::optional<torch::Tensor> lse, int64_t whole,
+                       int64_t splits, c10::optional<torch::Tensor> part, torch::Tensor status) {
   PromptArgs a;
   const int D = (int)(pages.size(2) / 72);
   a.T = (int)q.size(0); a.H = (int)pages.size(1); a.G = (int)(q.size(1) / a.H);
@@ -618,19 +636,20 @@ void kv4_prompt_launch(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_le
   a.v_mul = std::ldexp(1.f, (int)v_exp);
   a.out = out.data_ptr(); a.lse = (float*)opt_ptr(lse);
   a.status = (int*)status.data_ptr();
-  a.tiles = (int)prompt_tiles(a.T, a.G, D, max_q); a.splits = (int)splits;
+  const int64_t n = prompt_tiles(a.T, a.G, D, max_q) * a.H * a.B, rest = n - whole;
+  a.whole = (int)whole; a.splits = (int)splits;
   a.part = (float*)opt_ptr(part);
-  TORCH_CHECK(a.H <= 65535 && (splits == 1 || a.part), "kv4: too many heads, or no workspace");
+  TORCH_CHECK(n < (int64_t)1 << 30 && (rest == 0 || a.part), "kv4: too much work for one call, or no workspace");
   auto stream = at::cuda::getCurrentCUDAStream();
   auto go = [&](auto dim, auto t) {
     constexpr int DD = decltype(dim)::value;
     using T16 = decltype(t);
     using C = PromptCfg<DD>;
-    const dim3 grid((unsigned)(a.tiles * a.splits), a.H, a.B);
+    const dim3 grid((unsigned)(whole + rest * splits));
     moet_allow_max_smem(kv4_prompt_kernel<DD, T16>);
     launch_k(kv4_prompt_kernel<DD, T16>, grid, dim3(C::kWarps * 32), sizeof(PromptSmem<DD>), stream, a);
-    if (a.splits > 1)     // at most 148 tiles
-      launch_k(kv4_prompt_join_kernel<DD, T16>, dim3(C::TILES * 128 * DD / 8 / 256, a.tiles, a.B * a.H), dim3(256), 0, stream, a);
+    if (rest > 0)         // fewer than 148 tiles
+      launch_k(kv4_prompt_join_kernel<DD, T16>, dim3(C::TILES * 128 * DD / 8 / 256, (unsigned)rest), dim3(256), 0, stream, a);
   };
   auto by_type = [&](auto dim) {
     if (q.scalar_type() == at::kHalf) go(dim, __half{});

@@ -22,10 +22,10 @@ void kv4_attend_launch(Tensor q, Tensor cu_q, Tensor seq_lens, Tensor table, Ten
                        double scale, int64_t max_q, int64_t window, int64_t k_exp, int64_t v_exp, Tensor out,
                        optional<Tensor> lse, Tensor part, Tensor split, Tensor status);
 void kv4_prompt_launch(Tensor q, Tensor cu_q, Tensor seq_lens, Tensor table, Tensor pages, double scale, int64_t max_q,
-                       int64_t window, int64_t k_exp, int64_t v_exp, Tensor out, optional<Tensor> lse, int64_t splits,
-                       optional<Tensor> part, Tensor status);
-int64_t kv4_prompt_splits(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t max_q, int64_t W, int64_t window);
-int64_t kv4_prompt_workspace(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t max_q, int64_t splits);
+                       int64_t window, int64_t k_exp, int64_t v_exp, Tensor out, optional<Tensor> lse, int64_t whole,
+                       int64_t splits, optional<Tensor> part, Tensor status);
+std::tuple<int64_t, int64_t, int64_t> kv4_prompt_plan(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t max_q,
+                                                      int64_t W, int64_t window);
 
 namespace {
 
@@ -176,10 +176,11 @@ std::tuple<Tensor, optional<Tensor>> kv4_attend(Tensor q, Tensor cu_q, Tensor se
   if (return_lse) lse = at::empty({T, q.size(1)}, unit.options());
   if (T) {
     if (!chosen.has_value() && max_q * G > prompt_rows(c.D)) {
-      const int64_t B = seq_lens.size(0), splits = kv4_prompt_splits(T, B, c.H, G, c.D, max_q, table.size(1), window);
+      const auto [whole, splits, floats] = kv4_prompt_plan(T, seq_lens.size(0), c.H, G, c.D, max_q, table.size(1), window);
       optional<Tensor> part;
-      if (splits > 1) part = workspace(pages, kv4_prompt_workspace(T, B, c.H, G, c.D, max_q, splits), 0).first;
-      kv4_prompt_launch(q, cu_q, seq_lens, table, pages, scale, max_q, window, k_exp, v_exp, out, lse, splits, part, status);
+      if (floats) part = workspace(pages, floats, 0).first;
+      kv4_prompt_launch(q, cu_q, seq_lens, table, pages, scale, max_q, window, k_exp, v_exp, out, lse, whole, splits, part,
+                        status);
     } else {
       const auto [floats, ints] = kv4_attend_workspace(G, c.D, max_q, chosen.has_value());
       auto [part, split] = workspace(pages, floats, ints);
