@@ -280,7 +280,8 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
         const float raw = top;
         top *= cs;
         const bool move = m == -INFINITY ? top > -INFINITY : top > m + 8.f;
-        if (__any_sync(0xffffffffu, move)) {
+        const bool moves = __any_sync(0xffffffffu, move);
+        if (moves) {
           const float f = !move ? 1.f : m == -INFINITY ? 0.f : pr::exp2_fast(m - top);
           if (move) m = top, rest = __fmaf_rn(raw, cs, -top);
           l *= f;
@@ -316,6 +317,12 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
           pr::st16(s_at + c * 16, pk);       // P takes the columns of the scores
         }
         l += s0 + s1;
+        // Every phase of pv_done is waited for in turn, here where it is long past: a wait by parity for a
+        // later phase would take an earlier one for it (the output would be read before the last products).
+        if (i > 0 && !moves) {
+          ok = tc::mbar_wait(&sm.pv_done[t], (i - 1) & 1);
+          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        }
         pr::wait_st();
         tc::fence_before();
         pr::arrive(&sm.p_full[t]);

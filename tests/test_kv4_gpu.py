@@ -317,6 +317,34 @@ def test_attend_over_chosen_pages(KV4Cache, lens, news, H, G, D, dtype):
     check(out, lse, x.oracle(0.09, pages=pages), 320)
 
 
+@pytest.mark.parametrize("D,T,n", [(128, 1024, 6000), (64, 700, 5000), (256, 600, 4000)])
+def test_long_prompts_are_whole_and_the_same_every_time(KV4Cache, D, T, n):
+    """Every row of many tiles, some whole and some with their keys split, against f32 on the GPU, over and over:
+    an output read before its last products shows in some rows of some runs."""
+    H, G = 8, 4
+    g = torch.Generator(device=DEV).manual_seed(D)
+    k = (torch.randn(n, H, D, generator=g, device=DEV) * 1.3 + 0.3).bfloat16()
+    v = torch.randn(n, H, D, generator=g, device=DEV).bfloat16()
+    q = (torch.randn(T, H * G, D, generator=g, device=DEV) * 1.5).bfloat16()
+    pages = -(-n // 64)
+    c = KV4Cache(pages, H, D, device=DEV)
+    table = torch.randperm(pages, generator=g, device=DEV).int()[None]
+    j = torch.arange(n, device=DEV)
+    slots = table[0, j // 64].long() * 64 + j % 64
+    c.append(k, v, slots)
+    hk, hv = (x.float() for x in c.read(slots))
+    s = torch.einsum("thgd,nhd->htgn", q.float().unflatten(1, (H, G)), hk) * D ** -0.5
+    s.masked_fill_((j > torch.arange(n - T, n, device=DEV)[:, None])[None, :, None], -math.inf)
+    want = torch.einsum("htgn,nhd->thgd", torch.softmax(s, -1), hv).flatten(1, 2)
+    cu = torch.tensor([0, T], dtype=torch.int32, device=DEV)
+    lens = torch.tensor([n], dtype=torch.int32, device=DEV)
+    first = c.attend(q, cu, lens, table, D ** -0.5)
+    assert float((first.float() - want).abs().max()) <= 2.0 ** -8 * float(want.abs().max()) + 2.0 ** -9
+    for _ in range(30):
+        assert torch.equal(c.attend(q, cu, lens, table, D ** -0.5), first)
+    c.check()
+
+
 def test_many_sequences(KV4Cache):
     """More sequences than threads of a block, most of them short, tiles split over blocks."""
     g = torch.Generator().manual_seed(14)
