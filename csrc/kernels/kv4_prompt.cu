@@ -52,7 +52,7 @@ template <int D> struct PromptSmem {
   uint8_t k[2][C::kKBytes];
   uint8_t v[2][C::kKBytes];
   float row_scale[C::TILES * 128];
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2], pv_done[2];
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2], pv_done[2], o_full[2];
   uint32_t tmem;
 };
 
@@ -191,6 +191,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
       tc::mbar_init(&sm.s_full[i][1], 1);
       tc::mbar_init(&sm.p_full[i], 128);
       tc::mbar_init(&sm.pv_done[i], 1);
+      tc::mbar_init(&sm.o_full[i], 1);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -280,12 +281,13 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
         const float raw = top;
         top *= cs;
         const bool move = m == -INFINITY ? top > -INFINITY : top > m + 8.f;
-        const bool moves = __any_sync(0xffffffffu, move);
-        if (moves) {
+        if (__any_sync(0xffffffffu, move)) {
           const float f = !move ? 1.f : m == -INFINITY ? 0.f : pr::exp2_fast(m - top);
           if (move) m = top, rest = __fmaf_rn(raw, cs, -top);
           l *= f;
-          if (i > 0) {                       // once the product before is in O
+          // Once the product before is in O.  A wait by parity is right only if the phase before has ended:
+          // these scores were issued after the product of two steps ago.
+          if (i > 0) {
             ok = tc::mbar_wait(&sm.pv_done[t], (i - 1) & 1);
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             tc::fence_after();
@@ -317,19 +319,13 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
           pr::st16(s_at + c * 16, pk);       // P takes the columns of the scores
         }
         l += s0 + s1;
-        // Every phase of pv_done is waited for in turn, here where it is long past: a wait by parity for a
-        // later phase would take an earlier one for it (the output would be read before the last products).
-        if (i > 0 && !moves) {
-          ok = tc::mbar_wait(&sm.pv_done[t], (i - 1) & 1);
-          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-        }
         pr::wait_st();
         tc::fence_before();
         pr::arrive(&sm.p_full[t]);
       }
       // ---- output
       if (nkb > 0 && ok) {
-        ok = tc::mbar_wait(&sm.pv_done[t], (steps - 1) & 1);
+        ok = tc::mbar_wait(&sm.o_full[t], 0);      // its own barrier: pv_done may still be two phases back
         if (!__all_sync(0xffffffffu, ok)) ok = false;
       }
       if (ok) {
@@ -522,6 +518,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
       for (int k = 0; k < C::SK / 16; k++)
         pr::mma_ts(lead, tm + C::kOCol + t * D, tm + t * 128 + (n & 1) * C::SK + k * 8, va + k * 16, id_o, n > 0 || k > 0);
       pr::commit(lead, &sm.pv_done[t]);
+      if (n == steps - 1) pr::commit(lead, &sm.o_full[t]);
       if (t == ntile - 1 && half == C::HALVES - 1) pr::commit(lead, &sm.v_empty[st]);
     };
     if (steps > 0) {
