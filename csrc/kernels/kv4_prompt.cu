@@ -52,7 +52,7 @@ template <int D> struct PromptSmem {
   uint8_t k[2][C::kKBytes];
   uint8_t v[2][C::kKBytes];
   float row_scale[C::TILES * 128];
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2], pv_done[2], o_full[2];
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], pv_done[2], o_full[2];
   uint32_t tmem;
 };
 
@@ -189,7 +189,8 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
       tc::mbar_init(&sm.v_empty[i], 1);
       tc::mbar_init(&sm.s_full[i][0], 1);
       tc::mbar_init(&sm.s_full[i][1], 1);
-      tc::mbar_init(&sm.p_full[i], 128);
+      tc::mbar_init(&sm.p_full[i][0], 128);
+      tc::mbar_init(&sm.p_full[i][1], 128);
       tc::mbar_init(&sm.pv_done[i], 1);
       tc::mbar_init(&sm.o_full[i], 1);
     }
@@ -321,7 +322,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
         l += s0 + s1;
         pr::wait_st();
         tc::fence_before();
-        pr::arrive(&sm.p_full[t]);
+        pr::arrive(&sm.p_full[t][i & 1]);   // one per buffer: a warp may end its next step before the last warp ends this one
       }
       // ---- output
       if (nkb > 0 && ok) {
@@ -537,7 +538,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
           tc::fence_after();
           scores(t, nx);
         }
-        ok = tc::mbar_wait(&sm.p_full[t], n & 1);
+        ok = tc::mbar_wait(&sm.p_full[t][n & 1], (n >> 1) & 1);
         if (!ok) break;
         tc::fence_after();
         outputs(t, n);

@@ -345,6 +345,41 @@ def test_long_prompts_are_whole_and_the_same_every_time(KV4Cache, D, T, n):
     c.check()
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_prompt_rows_that_fall_behind(KV4Cache, D):
+    """The rows of one warp in four see scores that rise without end (their outputs are rescaled again and again),
+    the other rows see equal scores: the slow warp's neighbours may be a whole step ahead of it."""
+    H, G, T, n = 8, 4, 512, 6000
+    g = torch.Generator(device=DEV).manual_seed(D)
+    j = torch.arange(n, device=DEV)
+    ramp = 3.0 * (j + 64) / n
+    k = (ramp[:, None] * (1 + torch.arange(D, device=DEV) // 16 / 16.0)).bfloat16()[:, None].expand(n, H, D)
+    v = torch.randn(n, H, D, generator=g, device=DEV).bfloat16()
+    sign = 1.0 - 2.0 * (torch.arange(D, device=DEV) % 2)
+    steep = (torch.arange(T, device=DEV) // 8 % 4 == 1)[:, None]         # 8 tokens x 4 rows: a warp's rows
+    q = torch.where(steep, torch.full_like(sign, 2048.0 / D), sign).bfloat16()[:, None].expand(T, H * G, D)
+    pages = -(-n // 64)
+    c = KV4Cache(pages, H, D, device=DEV)
+    table = torch.randperm(pages, generator=g, device=DEV).int()[None]
+    slots = table[0, j // 64].long() * 64 + j % 64
+    c.append(k, v, slots)
+    hk, hv = (x.double() for x in c.read(slots))
+    scale = 1.0 / 8
+    want = torch.empty(T, H * G, D, dtype=torch.float64, device=DEV)
+    for h in range(H):
+        s = torch.einsum("tgd,nd->tgn", q[:, h * G:(h + 1) * G].double(), hk[:, h]) * scale
+        s.masked_fill_((j > torch.arange(n - T, n, device=DEV)[:, None])[:, None], -math.inf)
+        want[:, h * G:(h + 1) * G] = torch.softmax(s, -1) @ hv[:, h]
+    cu = torch.tensor([0, T], dtype=torch.int32, device=DEV)
+    lens = torch.tensor([n], dtype=torch.int32, device=DEV)
+    first = c.attend(q, cu, lens, table, scale)
+    # half an ulp of bf16, P in f16, and exp2 of differences between scores (sums of few-bit values: exact) near 2^11
+    assert float((first.double() - want).abs().max()) <= (2.0 ** -9 + 2.0 ** -10 + 2.0 ** -11) * float(hv.abs().max())
+    for _ in range(30):
+        assert torch.equal(c.attend(q, cu, lens, table, scale), first)
+    c.check()
+
+
 def test_many_sequences(KV4Cache):
     """More sequences than threads of a block, most of them short, tiles split over blocks."""
     g = torch.Generator().manual_seed(14)
