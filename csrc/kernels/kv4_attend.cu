@@ -20,6 +20,11 @@
 // its part (maxima, sums, unnormalised outputs), and kv4_join_kernel adds the parts up in
 // block order.  A split tile is named by the block in which it begins, so the join needs no
 // counters and its grid is the first one's.
+//
+// B200: 32 sequences with 362 k positions together, 8 heads of 128, 8 rows each: 92 us, 4.5 TB/s (69 % of the
+// measured copy rate); not the bytes but the instructions of the conversion bound it there (IPC 2.2 of
+// 4, ALU pipe 49 %, tensor 22 %, DRAM 46 %).  One sequence of 1000 positions: 8 us, a chain of
+// schedule, page look-up, one page per warp and join.
 #include "kv4.cuh"
 #include "tcgen05.cuh"
 #include "torch_glue.h"
@@ -98,6 +103,8 @@ struct Unit {
 
 // A tile's queries, join and output take a block as long as about this many of its pages;
 // counted as empty units in front of them, so that many short tiles do not all fall to one block.
+// B200, 32 sequences, one of them of two positions: without it the block that got its eight one-page
+// tiles ended after 120 us, the others after 87.
 constexpr int kTileCost = 8;
 
 // A unit is one page of a tile.  Its keys and its values are two copies, each into a slot of
@@ -697,7 +704,8 @@ static int sm_count() {
   return n;
 }
 
-// query rows of a tile / 8: the fewest that hold a sequence's rows, as the registers allow
+// query rows of a tile / 8: the fewest that hold a sequence's rows, as the registers allow.  B200, 8 sequences
+// of 30000, 8 heads of 128, 24 rows: 209 us in two tiles of 16, which convert every page twice, 124 in one of 24.
 static int row_tiles(int64_t rows, int D) {
   return rows <= 8 ? 1 : (rows <= 16 || D == 256) ? 2 : rows <= 24 ? 3 : 4;
 }

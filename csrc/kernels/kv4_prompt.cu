@@ -16,6 +16,13 @@
 // in the no-swizzle core-matrix order; the orders of values (depth of S, columns of O) are the
 // ones the cache's pieces give, so every 16-byte store of the conversion is one core-matrix row
 // and a warp's stores fill whole matrices without bank conflicts.
+//
+// B200, 2048 x 4 rows, 8 heads of 128, 16384 keys: 540 us for the kernel (568 with the join and the launches,
+// 910 TFLOP/s, 55 % of the measured bf16 rate).  The tensor path is busy 61 % of the time (64 keys a step
+// read Q and K from shared memory at three quarters of the product's own rate), exp2 46 %, the ALU
+// 34 %; the rest is the chain score, softmax, product of a step.  Measured and not taken: a warp per tile that
+// issues the products (570 us), eight warps that convert (586), 128 keys a step with one S
+// buffer per tile (601), two threads per row (748).
 #include "kv4.cuh"
 #include "tcgen05.cuh"
 #include "torch_glue.h"

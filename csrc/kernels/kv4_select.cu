@@ -12,8 +12,12 @@
 // [hi | lo]; a warp holds 16 pages' bounds as A fragments (16-byte loads, straight from
 // memory: each byte is used by one block per token tile) and walks over the rows' B fragments
 // in shared memory.  Bound by the bounds' bytes (2 D per page and head) in a decode step, by
-// the int8 product in a prompt chunk.  Choice: a block per (token, head) finds the threshold
-// by four passes of a radix search over the ordered bits and writes the pages in order.
+// the int8 product in a prompt chunk.  Choice: a warp (long rows: a block) per (token, head) finds
+// the threshold over the ordered bits and writes the pages in order.
+//
+// B200, 8 heads of 128: 1024 tokens x 8 rows over 512 pages, scores 68 us (252 int8 TOP/s: the per-token
+// maximum, in 32-bit integers and floats, costs as much issue as the products); 32 tokens x 8 rows over
+// 1.1 M positions, scores 14 us (its 35 MB of bounds are 2.5 TB/s: three dependent loads, then one wave).
 #include "kv4.cuh"
 #include "torch_glue.h"
 
@@ -253,6 +257,7 @@ MOET_DEVICE Pick pick_row(const SelectArgs& a, int tok, int h, int tid, int thre
 
 // A warp per (token, head), its keys in registers: up to 32 K pages.  The threshold is found bit by
 // bit from the highest bit in which the keys differ, and stops as soon as just `want` keys reach it.
+// Bound by the chain of votes (a step per bit over the warp's keys).
 template <int K>
 __global__ void __launch_bounds__(128) kv4_pick_warp_kernel(SelectArgs a) {
   pdl_entry();
@@ -317,8 +322,8 @@ __global__ void __launch_bounds__(128) kv4_pick_warp_kernel(SelectArgs a) {
 
 constexpr int kPickThreads = 128;
 
-// A block per (token, head) for longer rows: four passes of a radix search over the row in memory.
-
+// A block per (token, head) for longer rows, or few of them: four passes of a radix search over the row in memory, which L2
+// holds.  8 tokens x 8 heads over 2048 pages: 6 us (B200), the passes one after the other.
 __global__ void __launch_bounds__(kPickThreads) kv4_pick_kernel(SelectArgs a) {
   pdl_entry();
   __shared__ uint32_t hist[256];
@@ -415,7 +420,9 @@ void kv4_select_launch(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_le
   a.tpc = kScoreRows / a.gp;
   a.tiles = (int)((std::min<int64_t>(max_q, a.T) + a.tpc - 1) / a.tpc);
   a.chunks = (a.W + kScoreWarps * 16 - 1) / (kScoreWarps * 16);
-  // As many chunks per block as leave four blocks per SM: a block converts its rows once per span.
+  // As many chunks per block as leave four blocks per SM: a block converts its rows once per span.  us with
+  // 2 / 4 / 8 per SM, cold, choice included: 32 tokens over 1.1 M positions 36 / 34 / 36, 1024 tokens over
+  // 512 pages 89 / 89 / 99.
   const int64_t per_chunk = (int64_t)a.B * a.tiles * a.H;
   a.span = (int)std::max<int64_t>(1, std::min<int64_t>(a.chunks, per_chunk * a.chunks / (4 * 148)));
   const int64_t blocks = (int64_t)a.B * a.tiles * ((a.chunks + a.span - 1) / a.span);
@@ -442,9 +449,13 @@ void kv4_select_launch(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_le
     else go(std::integral_constant<int, 256>{});
   }
   const dim3 warps((unsigned)(((int64_t)a.T * a.H + 3) / 4)), four(128);
+  // A warp per row, except for more than 512 pages (32 keys a lane) with fewer than two rows per SM, where the
+  // latency of one row counts.  us of a whole choice, warp / block, 8 heads, back to back on B200: 32 tokens, 400
+  // pages 18.9 / 19.5, 700 pages 26.1 / 22.0; 64 tokens, 700 pages 36.6 / 37.6; 512 tokens, 1000 pages 156 / 165.
+  const bool few = a.W > 512 && (int64_t)a.T * a.H < 2 * 148;
   if (a.W <= 256) launch_k(kv4_pick_warp_kernel<8>, warps, four, 0, stream, a);
   else if (a.W <= 512) launch_k(kv4_pick_warp_kernel<16>, warps, four, 0, stream, a);
-  else if (a.W <= 1024) launch_k(kv4_pick_warp_kernel<32>, warps, four, 0, stream, a);
+  else if (a.W <= 1024 && !few) launch_k(kv4_pick_warp_kernel<32>, warps, four, 0, stream, a);
   else launch_k(kv4_pick_kernel, dim3((unsigned)((int64_t)a.T * a.H)), dim3(kPickThreads), 0, stream, a);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
