@@ -532,6 +532,27 @@ def test_select_of_long_rows(KV4Cache, width):
             assert got[r, 0].tolist() == [0] + sorted(order) + [width - 2, width - 1]
 
 
+@pytest.mark.parametrize("width", [500, 600, 1000])
+def test_select_of_many_rows_is_the_choice_of_each(KV4Cache, width):
+    """Many rows at once and a few at a time are chosen for in different ways: the choices are the same, ties too."""
+    g = torch.Generator().manual_seed(width)
+    T, H, D, n = 160, 2, 64, 400
+    c = KV4Cache(n, H, D, device=DEV)
+    c.bounds.copy_(torch.randint(-3, 4, c.bounds.shape, generator=g).to(torch.int8))
+    c.unit.copy_(2.0 ** torch.randint(-2, 3, c.unit.shape, generator=g).float())
+    q = torch.randn(T, H * 2, D, generator=g).bfloat16()
+    q[::3] = torch.round(q[::3])                                      # with ties
+    table = torch.randint(0, n, (T, width), generator=g).int().to(DEV)
+    sl = torch.randint(width * 32, width * 64 + 1, (T,), generator=g).int().to(DEV)
+    q, cu = q.to(DEV), torch.arange(T + 1).int().to(DEV)
+    for budget in (5, 64, 300):
+        all_rows = c.select(q, cu, sl, table, budget, max_q=1)
+        for i in range(0, T, 20):
+            part = c.select(q[i:i + 20], cu[:21], sl[i:i + 20], table[i:i + 20], budget, max_q=1)
+            assert torch.equal(part, all_rows[i:i + 20])
+    c.check()
+
+
 def test_chosen_pages_hold_the_best_key(KV4Cache):
     """The score is an upper bound: a page with a key far above the others is always taken."""
     x = Batch([64 * 40], [1], 2, 4, 128, seed=21)
