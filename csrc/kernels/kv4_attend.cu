@@ -547,6 +547,7 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, NT>()) kv4_atten
             }
           }
         } else if (st == kPage / TS - 1) {
+          __syncwarp();             // every lane has read the slot's start, which the next unit overwrites
           issue();
         }
       }

@@ -661,3 +661,23 @@ def test_demo_layer_from_prompt_to_decode():
     assert got["bytes_per_position"] * 32 == got["bf16_bytes_per_position"] * 9
     assert got["all_pages_rel_err"] < 0.2
     assert abs(got["chosen_pages_rel_err"] - got["all_pages_rel_err"]) < 2e-3      # 64 pages hold every position
+
+
+# --------------------------------------------------------------------- units that carry no page
+@pytest.mark.parametrize("G,D", [(4, 128), (12, 64), (5, 256)])
+def test_pages_between_empty_places(KV4Cache, G, D):
+    """Choices with a page in every third place: a warp passes over the empty ones, whose ring slots are taken again
+    at once.  The same as the choice without gaps up to rounding, and the same bits every time."""
+    H, n, m = 2, 2000, 3
+    x = Batch([n], [m], H, G, D, seed=31)
+    c = x.cache(KV4Cache)
+    some = torch.arange(0, 30, 2, dtype=torch.int32)
+    gaps = torch.full((m, H, 3 * some.numel()), -1, dtype=torch.int32)
+    gaps[..., 1::3] = some
+    gaps = gaps.to(DEV)
+    out, lse = c.attend(*x.args(), 0.1, max_q=m, pages=gaps, return_lse=True)
+    check(out, lse, x.oracle(0.1, pages=gaps.cpu()), 64 * some.numel())
+    for _ in range(100):
+        again, l2 = c.attend(*x.args(), 0.1, max_q=m, pages=gaps, return_lse=True)
+        assert torch.equal(again, out) and torch.equal(l2, lse)
+    c.check()
