@@ -45,6 +45,7 @@ struct AttendArgs {
   void* out; float* lse;                                // [T, H * G, D], [T, H * G] or null
   float* part; int* split;                              // parts: two per block; split: kSplitInts per block
   int min_units;
+  uint32_t tries;                                       // of a wait for a copy, before it gives up
   int* status;
 };
 // What a block notes of the tile that begins in it and goes on past it:
@@ -337,13 +338,19 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, NT>()) kv4_atten
 #pragma unroll 1
   for (int k = 0; k < NSLOT; k++) issue();
   int slot = 0;                          // the half that comes next
-  auto arrived = [&](int k) {            // wait for slot k; false: the copy did not come in time
+  // Wait for half x (of this warp's halves, in order).  If its copy does not come in time the warp computes
+  // nothing more, and waits here for what it has in flight: a copy must not outlive the block's shared memory.
+  auto arrived = [&](int k, int x) {     // k: the half's slot
     if (dead) return;
-    if (!tc::mbar_wait(&sm.bar[warp][k], (phase >> k) & 1)) {
-      set_status(a.status, kTimeout);
-      dead = true;
+    if (tc::mbar_wait(&sm.bar[warp][k], (phase >> k) & 1, a.tries)) {
+      phase ^= 1u << k;
+      return;
     }
-    phase ^= 1u << k;
+    set_status(a.status, kTimeout);
+    dead = true;
+    for (; x < next; x++)
+      if (sm.start[warp][x % NSLOT] >= 0) tc::mbar_wait(&sm.bar[warp][x % NSLOT], (phase >> x % NSLOT) & 1);
+    __syncwarp();
   };
 
   int i = 0;                             // next own unit
@@ -415,7 +422,7 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, NT>()) kv4_atten
     for (; u0 + warp + kWarps * i < seg_end; i++) {
       const int ks = slot, vs_ = ks + 1 == NSLOT ? 0 : ks + 1, start = sm.start[warp][ks];
       slot = vs_ + 1 == NSLOT ? 0 : vs_ + 1;
-      if (start >= 0) arrived(ks);
+      if (start >= 0) arrived(ks, 2 * i);
       const uint8_t *keys = sm.ring[warp][ks], *values = sm.ring[warp][vs_];
 #pragma unroll 1
       for (int st = 0; st < kPage / TS; st++) {
@@ -506,7 +513,7 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, NT>()) kv4_atten
             __syncwarp();           // every lane has read the keys
             issue();
           }
-          if (st == 0) arrived(vs_);
+          if (st == 0) arrived(vs_, 2 * i + 1);
           // O^T += V^T P^T
 #pragma unroll
           for (int mt = 0; mt < MT; mt++) {
@@ -639,9 +646,6 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, NT>()) kv4_atten
     tl = after;
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
-  if (dead) {        // copies that are still in flight must not outlive the block's shared memory
-    for (int k = 0; k < NSLOT; k++) tc::mbar_wait(&sm.bar[warp][k], (phase >> k) & 1);
-  }
 }
 
 // Joins the tile that begins in block blockIdx.x and goes on: 32 columns per block, the parts
@@ -726,7 +730,8 @@ std::tuple<int64_t, int64_t> kv4_attend_workspace(int64_t G, int64_t D, int64_t 
 void kv4_attend_launch(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_lens, torch::Tensor table,
                        torch::Tensor pages, c10::optional<torch::Tensor> sel, double scale, int64_t max_q,
                        int64_t window, int64_t k_exp, int64_t v_exp, torch::Tensor out,
-                       c10::optional<torch::Tensor> lse, torch::Tensor part, torch::Tensor split, torch::Tensor status) {
+                       c10::optional<torch::Tensor> lse, torch::Tensor part, torch::Tensor split, int64_t tries,
+                       torch::Tensor status) {
   const int T = (int)q.size(0), H = (int)pages.size(1), D = (int)(pages.size(2) / 72), G = (int)(q.size(1) / H);
   const int B = (int)seq_lens.size(0), W = (int)table.size(1);
   const bool chosen = sel.has_value() && sel->defined();
@@ -744,6 +749,7 @@ void kv4_attend_launch(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_le
   a.out = out.data_ptr(); a.lse = (float*)opt_ptr(lse);
   a.part = (float*)part.data_ptr(); a.split = (int*)split.data_ptr();
   a.min_units = kWarps;
+  a.tries = (uint32_t)tries;
   a.status = (int*)status.data_ptr();
   // the unit line is counted in 32 bits
   const int64_t line = chosen ? (int64_t)T * H * ((G + 8 * nt - 1) / (8 * nt)) * (a.budget + kTileCost)

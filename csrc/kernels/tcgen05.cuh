@@ -93,9 +93,10 @@ MOET_DEVICE bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
                : "=r"(ok) : "r"(smem_addr(bar)), "r"(parity) : "memory");
   return ok != 0;
 }
-// Bounded wait (about a second at most); false on timeout.
-MOET_DEVICE bool mbar_wait(uint64_t* bar, uint32_t parity) {
-  for (uint32_t it = 0; it < (1u << 22); it++)
+// Bounded wait (about a second at most, with the full number of tries); false on timeout.
+constexpr uint32_t kWaitTries = 1u << 22;
+MOET_DEVICE bool mbar_wait(uint64_t* bar, uint32_t parity, uint32_t tries = kWaitTries) {
+  for (uint32_t it = 0; it < tries; it++)
     if (mbar_try_wait(bar, parity)) return true;
   return false;
 }

@@ -20,7 +20,7 @@ void kv4_select_launch(Tensor q, Tensor cu_q, Tensor seq_lens, Tensor table, Ten
 std::tuple<int64_t, int64_t> kv4_attend_workspace(int64_t G, int64_t D, int64_t max_q, bool chosen);
 void kv4_attend_launch(Tensor q, Tensor cu_q, Tensor seq_lens, Tensor table, Tensor pages, optional<Tensor> sel,
                        double scale, int64_t max_q, int64_t window, int64_t k_exp, int64_t v_exp, Tensor out,
-                       optional<Tensor> lse, Tensor part, Tensor split, Tensor status);
+                       optional<Tensor> lse, Tensor part, Tensor split, int64_t tries, Tensor status);
 void kv4_prompt_launch(Tensor q, Tensor cu_q, Tensor seq_lens, Tensor table, Tensor pages, double scale, int64_t max_q,
                        int64_t window, int64_t k_exp, int64_t v_exp, Tensor out, optional<Tensor> lse, int64_t whole,
                        int64_t splits, optional<Tensor> part, Tensor status);
@@ -161,8 +161,9 @@ int64_t prompt_rows(int64_t D) { return D == 64 ? 64 : 32; }
 std::tuple<Tensor, optional<Tensor>> kv4_attend(Tensor q, Tensor cu_q, Tensor seq_lens, Tensor table, double scale,
                                                 int64_t max_q, int64_t window, optional<Tensor> chosen, bool return_lse,
                                                 Tensor pages, Tensor bounds, Tensor unit, Tensor status, int64_t k_exp,
-                                                int64_t v_exp) {
+                                                int64_t v_exp, int64_t tries) {
   const Cache c = check_cache(pages, bounds, unit, status, k_exp, v_exp);
+  TORCH_CHECK(tries >= 0 && tries <= 1 << 22, "kv4: a wait takes 0 to 2^22 tries");
   const c10::cuda::CUDAGuard guard(pages.device());
   const int64_t G = check_batch(q, cu_q, seq_lens, table, pages, c, max_q);
   TORCH_CHECK(window >= 0 && window < (int64_t)1 << 31, "kv4: window must be >= 0");
@@ -185,7 +186,7 @@ std::tuple<Tensor, optional<Tensor>> kv4_attend(Tensor q, Tensor cu_q, Tensor se
       const auto [floats, ints] = kv4_attend_workspace(G, c.D, max_q, chosen.has_value());
       auto [part, split] = workspace(pages, floats, ints);
       kv4_attend_launch(q, cu_q, seq_lens, table, pages, chosen, scale, max_q, window, k_exp, v_exp, out, lse, part, split,
-                        status);
+                        tries, status);
     }
   }
   return {out, lse};

@@ -681,3 +681,25 @@ def test_pages_between_empty_places(KV4Cache, G, D):
         again, l2 = c.attend(*x.args(), 0.1, max_q=m, pages=gaps, return_lse=True)
         assert torch.equal(again, out) and torch.equal(l2, lse)
     c.check()
+
+
+# --------------------------------------------------------------------------- waits that run out
+@pytest.mark.parametrize("G,D,pages", [(4, 128, False), (12, 64, True), (5, 256, False), (2, 256, True)])
+def test_a_wait_that_runs_out_is_reported(KV4Cache, G, D, pages):
+    """A copy that does not come in time (no try is made): the call ends with a status, and what was in flight has
+    landed before the block leaves, so the calls after it are whole."""
+    x = Batch([3000, 70], [2, 1], 2, G, D, seed=32)
+    c = x.cache(KV4Cache)
+    chosen = c.select(*x.args(), 9, max_q=2) if pages else None
+    ref = c.attend(*x.args(), 0.1, max_q=2, pages=chosen)
+    c.check()
+    for _ in range(5):
+        c._tries = 0
+        c.attend(*x.args(), 0.1, max_q=2, pages=chosen)
+        assert int(c.status) == 2
+        with pytest.raises(RuntimeError, match="wait"):
+            c.check()
+        c.status.zero_()
+        c._tries = KV4Cache._tries
+        assert torch.equal(c.attend(*x.args(), 0.1, max_q=2, pages=chosen), ref)
+        c.check()

@@ -41,6 +41,8 @@ class KV4Cache:
     ``k_exp`` / ``v_exp``: an element is e2m1 * e4m3 scale * 2^exp; the default reaches 42 in
     steps fine enough for normalised keys and values.  Larger values saturate."""
 
+    _tries = 1 << 22        # of a wait on the device (about a second) before the kernel gives up and sets the status
+
     def __init__(self, num_pages: int, num_kv_heads: int, head_dim: int, device="cuda", k_exp: int = -6,
                  v_exp: int = -6):
         if head_dim not in HEAD_DIMS:
@@ -106,5 +108,6 @@ class KV4Cache:
         none), as :meth:`select` gives them.  A row that sees nothing is zeros.  ``return_lse``:
         also the natural log-sum-exp [rows, heads] f32 (-inf for a row that sees nothing)."""
         out, lse = self._C.kv4_attend(q, cu_q, seq_lens, block_table, scale, -1 if max_q is None else max_q, window, pages,
-                                      return_lse, self.pages, self.bounds, self.unit, self.status, self.k_exp, self.v_exp)
+                                      return_lse, self.pages, self.bounds, self.unit, self.status, self.k_exp, self.v_exp,
+                                      self._tries)
         return (out, lse) if return_lse else out
