@@ -342,7 +342,8 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, NT>()) kv4_atten
   // nothing more, and waits here for what it has in flight: a copy must not outlive the block's shared memory.
   auto arrived = [&](int k, int x) {     // k: the half's slot
     if (dead) return;
-    if (tc::mbar_wait(&sm.bar[warp][k], (phase >> k) & 1, a.tries)) {
+    // one answer for the warp: its lanes go on to matrix instructions and shuffles, or none does
+    if (__all_sync(0xffffffffu, tc::mbar_wait(&sm.bar[warp][k], (phase >> k) & 1, a.tries))) {
       phase ^= 1u << k;
       return;
     }

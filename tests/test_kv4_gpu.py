@@ -703,3 +703,22 @@ def test_a_wait_that_runs_out_is_reported(KV4Cache, G, D, pages):
         c._tries = KV4Cache._tries
         assert torch.equal(c.attend(*x.args(), 0.1, max_q=2, pages=chosen), ref)
         c.check()
+
+
+@pytest.mark.parametrize("tries", [1, 2])
+def test_a_warp_gives_up_as_one(KV4Cache, tries):
+    """Waits that end about when the copy comes: lanes may see either, the warp takes one answer.  The call ends, and it
+    is whole or has set the status."""
+    x = Batch([2500, 900], [1, 1], 2, 8, 128, seed=33)
+    c = x.cache(KV4Cache)
+    ref = c.attend(*x.args(), 0.1, max_q=1)
+    for _ in range(20):
+        c._tries = tries
+        out = c.attend(*x.args(), 0.1, max_q=1)
+        assert int(c.status) in (0, 2)
+        if int(c.status) == 0:
+            assert torch.equal(out, ref)
+        c.status.zero_()
+        c._tries = KV4Cache._tries
+        assert torch.equal(c.attend(*x.args(), 0.1, max_q=1), ref)
+    c.check()
