@@ -30,6 +30,13 @@
 #include <algorithm>
 #include <tuple>
 
+// Tries of a bounded wait, and of the wait for the softmax's weights.  Constants (as an argument they cost the kernel
+// 3 %: registers); the test of waits that run out builds this file with its own.
+#ifndef MOET_KV4_TRIES
+#define MOET_KV4_TRIES tc::kWaitTries
+#define MOET_KV4_P_TRIES tc::kWaitTries
+#endif
+
 namespace moet {
 namespace kv4 {
 
@@ -59,7 +66,7 @@ template <int D> struct PromptSmem {
   uint8_t k[2][C::kKBytes];
   uint8_t v[2][C::kKBytes];
   float row_scale[C::TILES * 128];
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], pv_done[2], o_full[2];
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], pv_done[2], o_full[2], done;
   uint32_t tmem;
 };
 
@@ -201,6 +208,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
       tc::mbar_init(&sm.pv_done[i], 1);
       tc::mbar_init(&sm.o_full[i], 1);
     }
+    tc::mbar_init(&sm.done, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   for (int it = tid; it < TILES * 128 * 4; it += C::kWarps * 32) {   // kWarps * 32 is a multiple of 4: lanes stay together
@@ -267,7 +275,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
         const int j0 = kb0 * BK + i * SK;
         const uint32_t s_at = tmem + lanes + t * 128 + (i & 1) * SK;
         const bool edge = j0 + SK - 1 > pt_first || (a.window > 0 && j0 <= pt_last - a.window);
-        ok = tc::mbar_wait(&sm.s_full[t][i & 1], (i >> 1) & 1);
+        ok = tc::mbar_wait(&sm.s_full[t][i & 1], (i >> 1) & 1, MOET_KV4_TRIES);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         tc::fence_after();
         uint32_t u[SK / 32][32];
@@ -296,7 +304,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
           // Once the product before is in O.  A wait by parity is right only if the phase before has ended:
           // these scores were issued after the product of two steps ago.
           if (i > 0) {
-            ok = tc::mbar_wait(&sm.pv_done[t], (i - 1) & 1);
+            ok = tc::mbar_wait(&sm.pv_done[t], (i - 1) & 1, MOET_KV4_TRIES);
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             tc::fence_after();
 #pragma unroll 1
@@ -333,7 +341,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
       }
       // ---- output
       if (nkb > 0 && ok) {
-        ok = tc::mbar_wait(&sm.o_full[t], 0);      // its own barrier: pv_done may still be two phases back
+        ok = tc::mbar_wait(&sm.o_full[t], 0, MOET_KV4_TRIES);      // its own barrier: pv_done may still be two phases back
         if (!__all_sync(0xffffffffu, ok)) ok = false;
       }
       if (ok) {
@@ -449,7 +457,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
     fetch_v(kb0);
     for (int i = 0; i < nkb && ok; i++) {
       const int st = i & 1;
-      if (i >= 2) ok = tc::mbar_wait(&sm.k_empty[st], ((i >> 1) - 1) & 1);
+      if (i >= 2) ok = tc::mbar_wait(&sm.k_empty[st], ((i >> 1) - 1) & 1, MOET_KV4_TRIES);
       if (!ok) break;
 #pragma unroll
       for (int x = 0; x < KI; x++) {
@@ -470,7 +478,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
       for (int x = 0; x < KP; x++) page[x] = ahead[x];
       fetch_k(kb0 + i + 1);
       look_up(kb0 + i + 2, ahead);
-      if (i >= 2) ok = tc::mbar_wait(&sm.v_empty[st], ((i >> 1) - 1) & 1);
+      if (i >= 2) ok = tc::mbar_wait(&sm.v_empty[st], ((i >> 1) - 1) & 1, MOET_KV4_TRIES);
       if (!ok) break;
       // values: a thread has 8 tokens of its piece: per value one 16-byte row of a core matrix
       uint8_t* dst = sm.v[st] + vsl * (L::SD / 8) * kVSbo + vo * 128 + vg * 16;
@@ -530,27 +538,32 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
       if (t == ntile - 1 && half == C::HALVES - 1) pr::commit(lead, &sm.v_empty[st]);
     };
     if (steps > 0) {
-      ok = tc::mbar_wait(&sm.k_full[0], 0);
+      ok = tc::mbar_wait(&sm.k_full[0], 0, MOET_KV4_TRIES);
       tc::fence_after();
       for (int t = 0; t < ntile && ok; t++) scores(t, 0);
     }
     for (int n = 0; n < steps && ok; n++) {
       const int nx = n + 1, kb = n / C::HALVES, kx = nx / C::HALVES;
-      if (nx < steps && nx % C::HALVES == 0) ok = tc::mbar_wait(&sm.k_full[kx & 1], (kx >> 1) & 1);
-      if (ok && n % C::HALVES == 0) ok = tc::mbar_wait(&sm.v_full[kb & 1], (kb >> 1) & 1);
+      if (nx < steps && nx % C::HALVES == 0) ok = tc::mbar_wait(&sm.k_full[kx & 1], (kx >> 1) & 1, MOET_KV4_TRIES);
+      if (ok && n % C::HALVES == 0) ok = tc::mbar_wait(&sm.v_full[kb & 1], (kb >> 1) & 1, MOET_KV4_TRIES);
       for (int t = 0; t < ntile && ok; t++) {
         if (nx < steps) {                      // under this tile's softmax; its P of two steps before has been read
-          if (n > 0) ok = tc::mbar_wait(&sm.pv_done[t], (n - 1) & 1);
+          if (n > 0) ok = tc::mbar_wait(&sm.pv_done[t], (n - 1) & 1, MOET_KV4_TRIES);
           if (!ok) break;
           tc::fence_after();
           scores(t, nx);
         }
-        ok = tc::mbar_wait(&sm.p_full[t][n & 1], (n >> 1) & 1);
+        ok = tc::mbar_wait(&sm.p_full[t][n & 1], (n >> 1) & 1, MOET_KV4_P_TRIES);
         if (!ok) break;
         tc::fence_after();
         outputs(t, n);
       }
     }
+    // Where a wait ran out (here or in another warp) nobody has waited for the last products: none may still read
+    // shared memory or write tensor memory when the block gives them back.  With the full limit; it costs no time.
+    __syncwarp();
+    pr::commit(lead, &sm.done);
+    if (!tc::mbar_wait(&sm.done, 0)) ok = false;
   }
   __syncwarp();
   if (!ok) set_status(a.status, kTimeout);

@@ -722,3 +722,21 @@ def test_a_warp_gives_up_as_one(KV4Cache, tries):
         c._tries = KV4Cache._tries
         assert torch.equal(c.attend(*x.args(), 0.1, max_q=1), ref)
     c.check()
+
+
+@pytest.mark.parametrize("D,G,new", [(64, 8, 40), (128, 4, 200), (256, 2, 90)])
+def test_a_wait_that_runs_out_in_a_prompt(KV4Cache, D, G, new):
+    """The prompt kernel built with short waits: it gives up with products in flight, reports it, and none of them is
+    left when the block gives its tensor memory back, so the calls after it are whole."""
+    import moet_testkit       # test-only extension (tests/csrc)
+    x = Batch([4000, 300], [new, new], 2, G, D, seed=34)
+    c = x.cache(KV4Cache)
+    args = x.args()
+    ref = c.attend(*args, 0.1, max_q=new)
+    c.check()
+    for _ in range(5):
+        moet_testkit.kv4_prompt_wait_test(*args, c.pages, new, torch.empty_like(ref), c.status)
+        assert int(c.status) == 2
+        c.status.zero_()
+        assert torch.equal(c.attend(*args, 0.1, max_q=new), ref)
+        c.check()
