@@ -67,6 +67,7 @@ template <int D> struct PromptSmem {
   uint8_t v[2][C::kKBytes];
   float row_scale[C::TILES * 128];
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], pv_done[2], o_full[2], done;
+  uint32_t gone[16];                   // of step n's page, in place n & 15: it is not in the pool
   uint32_t tmem;
 };
 
@@ -274,19 +275,21 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
         constexpr int SK = C::SK;
         const int j0 = kb0 * BK + i * SK;
         const uint32_t s_at = tmem + lanes + t * 128 + (i & 1) * SK;
-        const bool edge = j0 + SK - 1 > pt_first || (a.window > 0 && j0 <= pt_last - a.window);
         ok = tc::mbar_wait(&sm.s_full[t][i & 1], (i >> 1) & 1, MOET_KV4_TRIES);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         tc::fence_after();
         uint32_t u[SK / 32][32];
 #pragma unroll
         for (int c = 0; c < SK / 32; c++) pr::ld32(s_at + c * 32, u[c]);
+        // a page that is not there is seen by no row; the look-up is at most four key blocks ahead of this step
+        const bool gone = sm.gone[i & 15];
+        const bool edge = gone || j0 + SK - 1 > pt_first || (a.window > 0 && j0 <= pt_last - a.window);
         tc::tmem_wait_ld();
         // the row's largest score; where it exceeds the reference by 2^8 (or there is none yet) the reference moves
         float top = -INFINITY, top1 = -INFINITY;
 #pragma unroll
         for (int c = 0; c < SK / 32; c++) {
-          if (edge) hide<32>(u[c], j0 + c * 32, p, a.window);
+          if (edge) hide<32>(u[c], j0 + c * 32, gone ? -1 : p, a.window);
 #pragma unroll
           for (int k = 0; k < 32; k += 4) {
             top = pr::max3(top, __uint_as_float(u[c][k]), __uint_as_float(u[c][k + 1]));
@@ -404,19 +407,32 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
     const int vg = dt & 7, vo = (dt >> 3) % OCT, vsl = (dt >> 3) / OCT;
     uint32_t kc[KI][W], vc[4][W];
     uint16_t ks[KI], vs[4];                                  // scales as they are held: converting waits for the load
-    // pages of a key block, looked up two blocks ahead (the look-up is a load of its own): -1 for none
+    // pages of a key block, looked up two blocks ahead (the look-up is a load of its own)
     constexpr int KP = BK / kPage;
+    // pages that some row of the tile sees; the others are neither looked at nor reported
+    auto seen = [&](int kb, int i) {
+      const int x = (kb * KP + i) * kPage;
+      return kb < kb1 && kb * KP + i < a.W && x <= p_last && (a.window == 0 || x + kPage > p_first - a.window + 1);
+    };
     int ahead[KP], page[KP];                                 // of the block after the next one, of the next one
-    auto look_up = [&](int kb, int (&to)[KP]) {
+    auto look_up = [&](int kb) {
+#pragma unroll
+      for (int i = 0; i < KP; i++) ahead[i] = seen(kb, i) ? a.table[(long long)b * a.W + kb * KP + i] : 0;
+    };
+    // the pages of block n (kb = kb0 + n) as looked up, -1 where there is nothing to load; whoever is missing is reported
+    auto take = [&](int n) {
 #pragma unroll
       for (int i = 0; i < KP; i++) {
-        const int x = kb * KP + i;
-        to[i] = kb < kb1 && x < a.W && x * kPage <= p_last ? a.table[(long long)b * a.W + x] : -1;
+        const bool want = seen(kb0 + n, i), there = (uint32_t)ahead[i] < (uint32_t)a.n_pages;
+        page[i] = want && there ? ahead[i] : -1;
+        if (dt == 0) {
+          sm.gone[n * KP + i & 15] = want && !there;
+          if (want && !there) set_status(a.status, kBadIndex);
+        }
       }
     };
     auto at = [&](int phys) -> const uint8_t* {
-      if (phys >= a.n_pages || phys < -1) set_status(a.status, kBadIndex);
-      return phys < 0 || phys >= a.n_pages ? nullptr : a.pages + ((long long)phys * a.H + h) * L::kPageBytes;
+      return phys < 0 ? nullptr : a.pages + ((long long)phys * a.H + h) * L::kPageBytes;
     };
     auto fetch_k = [&](int kb) {
 #pragma unroll
@@ -451,8 +467,9 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
         }
       }
     };
-    look_up(kb0, page);
-    look_up(kb0 + 1, ahead);
+    look_up(kb0);
+    take(0);
+    look_up(kb0 + 1);
     fetch_k(kb0);
     fetch_v(kb0);
     for (int i = 0; i < nkb && ok; i++) {
@@ -474,10 +491,9 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
       }
       tc::fence_proxy_async_smem();
       pr::arrive(&sm.k_full[st]);
-#pragma unroll
-      for (int x = 0; x < KP; x++) page[x] = ahead[x];
+      take(i + 1);
       fetch_k(kb0 + i + 1);
-      look_up(kb0 + i + 2, ahead);
+      look_up(kb0 + i + 2);
       if (i >= 2) ok = tc::mbar_wait(&sm.v_empty[st], ((i >> 1) - 1) & 1, MOET_KV4_TRIES);
       if (!ok) break;
       // values: a thread has 8 tokens of its piece: per value one 16-byte row of a core matrix

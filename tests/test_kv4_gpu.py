@@ -740,3 +740,42 @@ def test_a_wait_that_runs_out_in_a_prompt(KV4Cache, D, G, new):
         c.status.zero_()
         assert torch.equal(c.attend(*args, 0.1, max_q=new), ref)
         c.check()
+
+
+# ------------------------------------------------------------- pages that are not there, both kernels
+@pytest.mark.parametrize("entry", [-1, -7, None, 2 ** 31 - 1])             # None: one past the pool
+@pytest.mark.parametrize("lens,news,H,G,D,dtype,window,bad", [
+    ([300, 90], [2, 1], 2, 4, 128, torch.float16, 0, 1),
+    ([300, 90], [40, 30], 1, 2, 128, torch.bfloat16, 0, 2),
+    ([200], [70], 2, 2, 256, torch.float16, 0, 0),
+    ([2500], [60], 1, 2, 64, torch.float16, 0, 17),                        # a tile's keys split over blocks
+    ([640], [3], 1, 5, 64, torch.bfloat16, 200, 8),
+    ([640], [70], 1, 3, 128, torch.float16, 200, 7),
+])
+def test_a_bad_page_is_left_out_by_both_kernels(KV4Cache, lens, news, H, G, D, dtype, window, bad, entry):
+    x = Batch(lens, news, H, G, D, dtype, seed=41)
+    c = x.cache(KV4Cache)
+    q, cu, sl, tb = x.args()
+    tb[0, bad] = x.n_pages if entry is None else entry
+    seen = torch.arange(-(-max(lens) // 64), dtype=torch.int32).expand(sum(news), H, -1).clone()
+    seen[:news[0]][seen[:news[0]] == bad] = -1
+    want = x.oracle(0.1, window, seen)
+    for max_q in (max(news), 40 * max(news)):
+        out, lse = c.attend(q, cu, sl, tb, 0.1, max_q=max_q, window=window, return_lse=True)
+        assert int(c.status) == 1
+        c.status.zero_()
+        check(out, lse, want, max(lens))
+
+
+@pytest.mark.parametrize("max_q", [3, 200])
+def test_pages_before_the_window_may_be_gone(KV4Cache, max_q):
+    """A sliding window's pages are given back as the window leaves them: what no row sees is not looked at."""
+    x = Batch([900], [3], 1, 4, 128, seed=42)
+    c = x.cache(KV4Cache)
+    q, cu, sl, tb = x.args()
+    want = x.oracle(0.1, 150)
+    first = (900 - 3 - 150 + 1) // 64                                      # 748: page 11
+    tb[0, :first] = torch.tensor([-1, -9, x.n_pages, 2 ** 31 - 1] * 3, dtype=torch.int32, device=DEV)[:first]
+    out, lse = c.attend(q, cu, sl, tb, 0.1, max_q=max_q, window=150, return_lse=True)
+    c.check()
+    check(out, lse, want, 900)
