@@ -102,6 +102,13 @@ MOET_DEVICE void grid_prefetch(const void* p, long long bytes) {
   if (at < bytes) prefetch_l2(static_cast<const uint8_t*>(p) + at);
 }
 
+// Positions of a sequence that a table of W pages can hold: a length out of range is taken as the nearest in range,
+// and reported (once a call).
+MOET_DEVICE int held_length(int len, int W) { return max(0, min(len, W * kPage)); }
+MOET_DEVICE void check_length(int len, int W, int* status) {
+  if (len != held_length(len, W)) set_status(status, kBadIndex);
+}
+
 MOET_DEVICE float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }   // -126 <= e <= 127
 
 // Smallest e >= -100 with amax <= 127 * 2^e; 0 for amax = 0 (finite amax >= 0).

@@ -141,7 +141,7 @@ MOET_DEVICE int row_start(const AttendArgs& a, int b) { return max(0, min(a.cu_q
 template <int D, int NT>
 MOET_DEVICE void seq_units(const AttendArgs& a, int b, int& tiles, int& n, int& page0) {
   const int nq = max(0, row_start(a, b + 1) - row_start(a, b));
-  const int len = max(0, min(a.seq_lens[b], a.W * kPage));
+  const int len = held_length(a.seq_lens[b], a.W);
   tiles = (nq * a.G + 8 * NT - 1) / (8 * NT);
   page0 = a.window > 0 ? max(0, len - nq - a.window + 1) / kPage : 0;
   n = max(1, (len + kPage - 1) / kPage - page0) + kTileCost;      // an empty sequence's rows are still written
@@ -167,7 +167,7 @@ MOET_DEVICE Unit find_unit(const AttendArgs& a, const int* pre, int u) {
     r.b = lo;
     r.row0 = chunk * RT;
     r.rows = a.G;
-    r.p0 = r.tok0 < pre[lo + 1] ? min(a.seq_lens[lo], a.W * kPage) - pre[lo + 1] + r.tok0 : -1;   // -1: no sequence's
+    r.p0 = r.tok0 < pre[lo + 1] ? held_length(a.seq_lens[lo], a.W) - pre[lo + 1] + r.tok0 : -1;   // -1: no sequence's
     r.page = r.x - kTileCost;
     return r;
   }
@@ -186,7 +186,7 @@ MOET_DEVICE Unit find_unit(const AttendArgs& a, const int* pre, int u) {
   r.row0 = tile * RT;
   r.rows = nq * a.G;
   r.tok0 = c0;
-  r.p0 = min(a.seq_lens[lo], a.W * kPage) - nq;
+  r.p0 = held_length(a.seq_lens[lo], a.W) - nq;
   r.page = page0 + r.x - kTileCost;
   return r;
 }
@@ -277,6 +277,8 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, NT>()) kv4_atten
   const int u0 = (int)min((long long)blockIdx.x * per, (long long)total), u1 = min(u0 + per, total);
   int* split = a.split + blockIdx.x * kSplitInts;
   if (tid == 0) split[0] = 0;
+  if (blockIdx.x == gridDim.x - 1)       // the last block, which has the least to do
+    for (int b = tid; b < a.B; b += kWarps * 32) check_length(a.seq_lens[b], a.W, a.status);
   if (u0 >= u1) return;
 
   // ---- queries come by way of shared memory, a tile ahead

@@ -50,7 +50,7 @@ MOET_DEVICE void mma_s8_16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2
 MOET_DEVICE void seq_rows(const SelectArgs& a, int b, int& c0, int& nq, int& p0) {
   c0 = max(0, min(a.cu_q[b], a.T));
   nq = max(0, max(0, min(a.cu_q[b + 1], a.T)) - c0);
-  p0 = min(a.seq_lens[b], a.W * kPage) - nq;
+  p0 = held_length(a.seq_lens[b], a.W) - nq;
 }
 // pages of a row at position p that compete for a place: [first, n - last), n = p / 64 + 1
 MOET_DEVICE int rivals_end(const SelectArgs& a, int p) { return p < 0 ? 0 : p / kPage + 1 - a.last; }
@@ -231,6 +231,10 @@ struct Pick {
   int n, end, want;         // pages; rivals are [first, end), `want` of them are taken (more than that: n > budget)
   int* out;
 };
+MOET_DEVICE void check_lengths(const SelectArgs& a) {      // by the last block
+  if (blockIdx.x == gridDim.x - 1)
+    for (int b = threadIdx.x; b < a.B; b += blockDim.x) check_length(a.seq_lens[b], a.W, a.status);
+}
 MOET_DEVICE Pick pick_row(const SelectArgs& a, int tok, int h, int tid, int threads) {
   int lo = 0, hi = a.B;
   while (hi - lo > 1) {
@@ -261,6 +265,7 @@ MOET_DEVICE Pick pick_row(const SelectArgs& a, int tok, int h, int tid, int thre
 template <int K>
 __global__ void __launch_bounds__(128) kv4_pick_warp_kernel(SelectArgs a) {
   pdl_entry();
+  check_lengths(a);
   const int lane = threadIdx.x & 31;
   const long long id = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (id >= (long long)a.T * a.H) return;
@@ -326,6 +331,7 @@ constexpr int kPickThreads = 128;
 // holds.  8 tokens x 8 heads over 2048 pages: 6 us (B200), the passes one after the other.
 __global__ void __launch_bounds__(kPickThreads) kv4_pick_kernel(SelectArgs a) {
   pdl_entry();
+  check_lengths(a);
   __shared__ uint32_t hist[256];
   __shared__ int scan[kPickThreads / 32][2];
   __shared__ uint32_t prefix_s;

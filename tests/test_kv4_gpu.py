@@ -779,3 +779,31 @@ def test_pages_before_the_window_may_be_gone(KV4Cache, max_q):
     out, lse = c.attend(q, cu, sl, tb, 0.1, max_q=max_q, window=150, return_lse=True)
     c.check()
     check(out, lse, want, 900)
+
+
+# ------------------------------------------------------------------- lengths out of range
+@pytest.mark.parametrize("length", [64 * 12 + 1, 2 ** 31 - 1, -1, -2 ** 31])
+@pytest.mark.parametrize("max_q", [3, 200])
+def test_a_length_out_of_range_is_reported(KV4Cache, length, max_q):
+    """More positions than the table holds, or fewer than none; the other sequences are what they were."""
+    x = Batch([700, 150, 400], [3, 2, 3], 2, 4, 128, seed=50, width=12)
+    c = x.cache(KV4Cache)
+    q, cu, sl, tb = x.args()
+    tb.clamp_(min=0)
+    ref = c.attend(q, cu, sl, tb, 0.1, max_q=max_q)
+    ref_pages = c.select(q, cu, sl, tb, 4, max_q=max_q)
+    ref_chosen = c.attend(q, cu, sl, tb, 0.1, max_q=max_q, pages=ref_pages)
+    c.check()
+    sl[1] = length
+    rest = [0, 1, 2, 5, 6, 7]
+    for call, want in ((lambda: c.attend(q, cu, sl, tb, 0.1, max_q=max_q), ref),
+                       (lambda: c.attend(q, cu, sl, tb, 0.1, max_q=max_q, window=300), None),
+                       (lambda: c.select(q, cu, sl, tb, 4, max_q=max_q), ref_pages),
+                       (lambda: c.select(q, cu, sl, tb, 12, max_q=max_q), None),
+                       (lambda: c.attend(q, cu, sl, tb, 0.1, max_q=max_q, pages=ref_pages), ref_chosen)):
+        got = call()
+        assert int(c.status) == 1
+        c.status.zero_()
+        if want is not None:
+            got, want = got[rest].float(), want[rest].float()
+            assert torch.allclose(got, want, rtol=2.0 ** -7, atol=2.0 ** -9 * 6)      # split elsewhere: a rounding apart
