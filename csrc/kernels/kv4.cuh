@@ -102,11 +102,13 @@ MOET_DEVICE void grid_prefetch(const void* p, long long bytes) {
   if (at < bytes) prefetch_l2(static_cast<const uint8_t*>(p) + at);
 }
 
-// Positions of a sequence that a table of W pages can hold: a length out of range is taken as the nearest in range,
-// and reported (once a call).
+// Positions of a sequence that a table of W pages can hold: a length out of range is taken as the nearest in range.
 MOET_DEVICE int held_length(int len, int W) { return max(0, min(len, W * kPage)); }
-MOET_DEVICE void check_length(int len, int W, int* status) {
-  if (len != held_length(len, W)) set_status(status, kBadIndex);
+// Sequence b of a batch with T rows: reports a length out of range, and row offsets that are out of range or order
+// (they are pulled back into the rows).  Once a call.
+MOET_DEVICE void check_sequence(const int* cu_q, const int* seq_lens, int b, int T, int W, int* status) {
+  const int c0 = cu_q[b], c1 = cu_q[b + 1], len = seq_lens[b];
+  if (c0 < 0 || c1 < c0 || c1 > T || len != held_length(len, W)) set_status(status, kBadIndex);
 }
 
 MOET_DEVICE float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }   // -126 <= e <= 127

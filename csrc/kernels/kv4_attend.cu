@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, NT>()) kv4_atten
   int* split = a.split + blockIdx.x * kSplitInts;
   if (tid == 0) split[0] = 0;
   if (blockIdx.x == gridDim.x - 1)       // the last block, which has the least to do
-    for (int b = tid; b < a.B; b += kWarps * 32) check_length(a.seq_lens[b], a.W, a.status);
+    for (int b = tid; b < a.B; b += kWarps * 32) check_sequence(a.cu_q, a.seq_lens, b, a.T, a.W, a.status);
   if (u0 >= u1) return;
 
   // ---- queries come by way of shared memory, a tile ahead

@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
   const int rows = nq * a.G, p0 = held_length(a.seq_lens[b], a.W) - nq;
   const int ntiles_seq = (rows + TILES * 128 - 1) / (TILES * 128);
   const int tile = ntiles_seq - 1 - back;
-  if (h == 0 && back == 0 && split == 0 && tid == 0) check_length(a.seq_lens[b], a.W, a.status);
+  if (h == 0 && back == 0 && split == 0 && tid == 0) check_sequence(a.cu_q, a.seq_lens, b, a.T, a.W, a.status);
   if (tile < 0) return;
   const int row0 = tile * TILES * 128, live = min(rows - row0, TILES * 128);
   const int p_first = p0 + row0 / a.G, p_last = p0 + (row0 + live - 1) / a.G;

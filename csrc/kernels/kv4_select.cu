@@ -231,9 +231,9 @@ struct Pick {
   int n, end, want;         // pages; rivals are [first, end), `want` of them are taken (more than that: n > budget)
   int* out;
 };
-MOET_DEVICE void check_lengths(const SelectArgs& a) {      // by the last block
+MOET_DEVICE void check_batch(const SelectArgs& a) {      // by the last block
   if (blockIdx.x == gridDim.x - 1)
-    for (int b = threadIdx.x; b < a.B; b += blockDim.x) check_length(a.seq_lens[b], a.W, a.status);
+    for (int b = threadIdx.x; b < a.B; b += blockDim.x) check_sequence(a.cu_q, a.seq_lens, b, a.T, a.W, a.status);
 }
 MOET_DEVICE Pick pick_row(const SelectArgs& a, int tok, int h, int tid, int threads) {
   int lo = 0, hi = a.B;
@@ -265,7 +265,7 @@ MOET_DEVICE Pick pick_row(const SelectArgs& a, int tok, int h, int tid, int thre
 template <int K>
 __global__ void __launch_bounds__(128) kv4_pick_warp_kernel(SelectArgs a) {
   pdl_entry();
-  check_lengths(a);
+  check_batch(a);
   const int lane = threadIdx.x & 31;
   const long long id = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (id >= (long long)a.T * a.H) return;
@@ -331,7 +331,7 @@ constexpr int kPickThreads = 128;
 // holds.  8 tokens x 8 heads over 2048 pages: 6 us (B200), the passes one after the other.
 __global__ void __launch_bounds__(kPickThreads) kv4_pick_kernel(SelectArgs a) {
   pdl_entry();
-  check_lengths(a);
+  check_batch(a);
   __shared__ uint32_t hist[256];
   __shared__ int scan[kPickThreads / 32][2];
   __shared__ uint32_t prefix_s;

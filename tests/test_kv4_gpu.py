@@ -807,3 +807,20 @@ def test_a_length_out_of_range_is_reported(KV4Cache, length, max_q):
         if want is not None:
             got, want = got[rest].float(), want[rest].float()
             assert torch.allclose(got, want, rtol=2.0 ** -7, atol=2.0 ** -9 * 6)      # split elsewhere: a rounding apart
+
+
+# ------------------------------------------------------------------------ row offsets out of range
+@pytest.mark.parametrize("cu", [[0, 3, 9, 8], [-1, 3, 5, 8], [0, 5, 3, 8]])
+@pytest.mark.parametrize("max_q", [8, 200])
+def test_offsets_out_of_range_are_reported(KV4Cache, cu, max_q):
+    x = Batch([700, 150, 400], [3, 2, 3], 2, 4, 128, seed=51)
+    c = x.cache(KV4Cache)
+    q, _, sl, tb = x.args()
+    tb.clamp_(min=0)
+    cu = torch.tensor(cu, dtype=torch.int32, device=DEV)
+    pages = torch.zeros(8, 2, 3, dtype=torch.int32, device=DEV)
+    for call in (lambda: c.attend(q, cu, sl, tb, 0.1, max_q=max_q), lambda: c.attend(q, cu, sl, tb, 0.1, max_q=max_q, pages=pages),
+                 lambda: c.select(q, cu, sl, tb, 4, max_q=max_q), lambda: c.select(q, cu, sl, tb, 400, max_q=max_q)):
+        call()
+        assert int(c.status) == 1
+        c.status.zero_()

@@ -18,8 +18,8 @@ the rows' own (append first), ``block_table`` int32 [B, W] page per 64 positions
 sequence's n sits at position ``seq_len - n + i`` and sees the positions up to its own.
 
 All calls run on the current CUDA stream, never synchronise and can be captured in a CUDA
-graph.  Errors that only the device can see (a slot, page or length out of range, a value
-that is not finite) set ``cache.status``, as the engine's other kernels do; ``cache.check()`` raises.
+graph.  Errors that only the device can see (a slot, page, length or row
+offset out of range, a value that is not finite) set ``cache.status``, as the engine's other kernels do; ``cache.check()`` raises.
 """
 from __future__ import annotations
 
@@ -31,7 +31,7 @@ from . import native
 
 PAGE = 64
 HEAD_DIMS = (64, 128, 256)
-_STATUS = {1: "a slot, page or length out of range", 2: "a wait on the device ran out", 3: "bad size",
+_STATUS = {1: "a slot, page, length or row offset out of range", 2: "a wait on the device ran out", 3: "bad size",
            4: "a key or value that is not finite (NaN is held as 0, infinities as the largest value)"}
 
 
