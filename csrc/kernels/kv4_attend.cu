@@ -167,7 +167,7 @@ MOET_DEVICE Unit find_unit(const AttendArgs& a, const int* pre, int u) {
     r.b = lo;
     r.row0 = chunk * RT;
     r.rows = a.G;
-    r.p0 = r.tok0 < pre[lo + 1] ? held_length(a.seq_lens[lo], a.W) - pre[lo + 1] + r.tok0 : -1;   // -1: no sequence's
+    r.p0 = r.tok0 >= pre[lo] && r.tok0 < pre[lo + 1] ? held_length(a.seq_lens[lo], a.W) - pre[lo + 1] + r.tok0 : -1;   // -1: no sequence's
     r.page = r.x - kTileCost;
     return r;
   }
@@ -240,6 +240,8 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, NT>()) kv4_atten
   grid_prefetch(a.q, ((long long)(a.T - 1) * a.q_tok + (a.H * a.G - 1ll) * a.q_head + D) * 2);
   pdl_entry();
 
+  const int rows0 = a.cu_q[0], rows1 = a.cu_q[a.B];
+
   // the line of units: prefix sums over the sequences (all pages), or over nothing (chosen pages)
   int total;
   if (a.sel) {
@@ -279,6 +281,7 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, NT>()) kv4_atten
   if (tid == 0) split[0] = 0;
   if (blockIdx.x == gridDim.x - 1)       // the last block, which has the least to do
     for (int b = tid; b < a.B; b += kWarps * 32) check_sequence(a.cu_q, a.seq_lens, b, a.T, a.W, a.status);
+  if (!a.sel) blank_rows(rows0, rows1, a.T, a.out, a.lse, a.H * a.G, D);     // chosen pages: such a row is a tile that sees nothing
   if (u0 >= u1) return;
 
   // ---- queries come by way of shared memory, a tile ahead

@@ -183,6 +183,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
   const int rows = nq * a.G, p0 = held_length(a.seq_lens[b], a.W) - nq;
   const int ntiles_seq = (rows + TILES * 128 - 1) / (TILES * 128);
   const int tile = ntiles_seq - 1 - back;
+  blank_rows(a.cu_q[0], a.cu_q[a.B], a.T, a.out, a.lse, a.H * a.G, D);
   if (h == 0 && back == 0 && split == 0 && tid == 0) check_sequence(a.cu_q, a.seq_lens, b, a.T, a.W, a.status);
   if (tile < 0) return;
   const int row0 = tile * TILES * 128, live = min(rows - row0, TILES * 128);

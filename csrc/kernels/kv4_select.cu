@@ -243,7 +243,7 @@ MOET_DEVICE Pick pick_row(const SelectArgs& a, int tok, int h, int tid, int thre
   }
   int c0, nq, p0;
   seq_rows(a, lo, c0, nq, p0);
-  const int p = tok - c0 < nq ? p0 + tok - c0 : -1;
+  const int p = tok >= c0 && tok - c0 < nq ? p0 + tok - c0 : -1;       // -1: no sequence's
   Pick r;
   r.n = p < 0 ? 0 : p / kPage + 1;
   r.out = a.pages + ((long long)tok * a.H + h) * a.budget;

@@ -824,3 +824,54 @@ def test_offsets_out_of_range_are_reported(KV4Cache, cu, max_q):
         call()
         assert int(c.status) == 1
         c.status.zero_()
+
+
+# -------------------------------------------------------------------- rows that belong to no sequence
+def poison(*shapes):
+    """NaN into the blocks that the allocator gives out next for these sizes."""
+    x = [torch.full(s, math.nan, dtype=d, device=DEV) for s, d in shapes for _ in range(3)]
+    torch.cuda.synchronize()
+    del x
+
+
+@pytest.mark.parametrize("before,after", [(0, 3), (2, 0), (5, 700)])
+@pytest.mark.parametrize("news,max_q,G,D,dtype", [([2, 1], 2, 4, 128, torch.float16), ([2, 1], 400, 4, 128, torch.bfloat16),
+                                                  ([50, 3], 50, 2, 64, torch.float16), ([3, 70], 70, 3, 256, torch.bfloat16)])
+def test_rows_of_no_sequence_are_zeros(KV4Cache, news, max_q, G, D, dtype, before, after):
+    """A batch padded to a captured size: rows in front of cu_q[0] and past cu_q[B]."""
+    H = 2
+    x = Batch([700, 64 * 9], news, H, G, D, dtype, seed=43)
+    c = x.cache(KV4Cache)
+    q, cu, sl, tb = x.args()
+    n = sum(news)
+    wide = torch.randn(before + n + after, H * G, D, device=DEV).to(dtype)
+    wide[before:before + n] = q
+    cu = cu + before
+    ref_pages = c.select(q, cu - before, sl, tb, 5, max_q=max_q)
+    for chosen in (False, True):
+        pages = None
+        if chosen:
+            pages = c.select(wide, cu, sl, tb, 5, max_q=max_q)
+            assert torch.equal(pages[before:before + n], ref_pages)
+            assert (pages[:before] == -1).all() and (pages[before + n:] == -1).all()
+            pages[:before], pages[before + n:] = ref_pages[0], ref_pages[0]          # and whatever they ask for
+        want = x.oracle(0.1, pages=ref_pages.cpu() if chosen else None)
+        poison((wide.shape, dtype), (wide.shape[:2], torch.float32))
+        out, lse = c.attend(wide, cu, sl, tb, 0.1, max_q=max_q, pages=pages, return_lse=True)
+        check(out[before:before + n], lse[before:before + n], want, 700)
+        assert (out[:before] == 0).all() and (out[before + n:] == 0).all()
+        assert (lse[:before] == -math.inf).all() and (lse[before + n:] == -math.inf).all()
+    c.check()
+
+
+@pytest.mark.parametrize("max_q", [1, 100])
+def test_a_batch_without_sequence_rows(KV4Cache, max_q):
+    x = Batch([100, 0], [0, 0], 1, 2, 64, seed=44)
+    c = x.cache(KV4Cache)
+    _, cu, sl, tb = x.args()
+    q = torch.randn(5, 2, 64, device=DEV).bfloat16()
+    poison((q.shape, q.dtype), (q.shape[:2], torch.float32))
+    out, lse = c.attend(q, cu, sl, tb, 0.1, max_q=max_q, return_lse=True)
+    assert (out == 0).all() and (lse == -math.inf).all()
+    assert (c.select(q, cu, sl, tb, 3, max_q=max_q) == -1).all()
+    c.check()
