@@ -110,17 +110,18 @@ MOET_DEVICE void check_sequence(const int* cu_q, const int* seq_lens, int b, int
   const int c0 = cu_q[b], c1 = cu_q[b + 1], len = seq_lens[b];
   if (c0 < 0 || c1 < c0 || c1 > T || len != held_length(len, W)) set_status(status, kBadIndex);
 }
+MOET_DEVICE void blank_row(long long row, void* out, float* lse, int heads, int D) {
+  uint4* p = static_cast<uint4*>(out) + row * heads * (D / 8);
+  for (int e = threadIdx.x; e < heads * (D / 8); e += blockDim.x) p[e] = make_uint4(0, 0, 0, 0);
+  if (lse)
+    for (int e = threadIdx.x; e < heads; e += blockDim.x) lse[row * heads + e] = -INFINITY;
+}
 // Output rows of no sequence, in front of the first offset and past the last (a batch padded to a captured size): zeros,
 // and a log-sum-exp of -inf.  The grid's blocks share them out; the first rows go to the last blocks.
 MOET_DEVICE void blank_rows(int first, int last, int T, void* out, float* lse, int heads, int D) {
   first = max(0, min(first, T)), last = max(first, min(last, T));
-  for (int i = gridDim.x - 1 - blockIdx.x; i < first + T - last; i += gridDim.x) {
-    const long long row = (long long)(i < first ? i : last + i - first) * heads;
-    uint4* p = static_cast<uint4*>(out) + row * (D / 8);
-    for (int e = threadIdx.x; e < heads * (D / 8); e += blockDim.x) p[e] = make_uint4(0, 0, 0, 0);
-    if (lse)
-      for (int e = threadIdx.x; e < heads; e += blockDim.x) lse[row + e] = -INFINITY;
-  }
+  for (int i = gridDim.x - 1 - blockIdx.x; i < first + T - last; i += gridDim.x)
+    blank_row(i < first ? i : last + i - first, out, lse, heads, D);
 }
 
 MOET_DEVICE float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }   // -126 <= e <= 127

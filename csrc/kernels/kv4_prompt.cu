@@ -42,7 +42,7 @@ namespace kv4 {
 
 struct PromptArgs {
   const void* q; long long q_tok; int q_head;
-  const int *cu_q, *seq_lens, *table; int B, W, T, H, G, window;
+  const int *cu_q, *seq_lens, *table; int B, W, T, H, G, max_q, window;
   const uint8_t* pages; int n_pages;
   float scale_log2, v_mul;
   void* out; float* lse;
@@ -179,12 +179,19 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
   const int split = (int)blockIdx.x < a.whole ? 0 : (int)(blockIdx.x - a.whole) % a.splits;
   const int splits = (int)blockIdx.x < a.whole ? 1 : a.splits;
   const int b = entry % a.B, h = entry / a.B % a.H, back = entry / (a.B * a.H);
-  const int c0 = max(0, min(a.cu_q[b], a.T)), nq = max(0, max(0, min(a.cu_q[b + 1], a.T)) - c0);
-  const int rows = nq * a.G, p0 = held_length(a.seq_lens[b], a.W) - nq;
+  const int c0 = max(0, min(a.cu_q[b], a.T)), all = max(0, max(0, min(a.cu_q[b + 1], a.T)) - c0);
+  const int nq = min(all, a.max_q);                        // the tiles that there are: rows past them are reported
+  const int rows = nq * a.G, p0 = held_length(a.seq_lens[b], a.W) - all;
   const int ntiles_seq = (rows + TILES * 128 - 1) / (TILES * 128);
   const int tile = ntiles_seq - 1 - back;
   blank_rows(a.cu_q[0], a.cu_q[a.B], a.T, a.out, a.lse, a.H * a.G, D);
-  if (h == 0 && back == 0 && split == 0 && tid == 0) check_sequence(a.cu_q, a.seq_lens, b, a.T, a.W, a.status);
+  if (h == 0 && back == 0 && split == 0) {
+    if (tid == 0) check_sequence(a.cu_q, a.seq_lens, b, a.T, a.W, a.status);
+    if (all > nq) {
+      if (tid == 0) set_status(a.status, kBadSize);
+      for (int i = nq; i < all; i++) blank_row(c0 + i, a.out, a.lse, a.H * a.G, D);
+    }
+  }
   if (tile < 0) return;
   const int row0 = tile * TILES * 128, live = min(rows - row0, TILES * 128);
   const int p_first = p0 + row0 / a.G, p_last = p0 + (row0 + live - 1) / a.G;
@@ -601,7 +608,7 @@ __global__ void __launch_bounds__(256) kv4_prompt_join_kernel(PromptArgs a) {
   pdl_entry();
   const int entry = a.whole + blockIdx.y, b = entry % a.B, h = entry / a.B % a.H, back = entry / (a.B * a.H);
   const int it = blockIdx.x * 256 + threadIdx.x, r = it / (D / 8), d = it % (D / 8) * 8;
-  const int c0 = max(0, min(a.cu_q[b], a.T)), nq = max(0, max(0, min(a.cu_q[b + 1], a.T)) - c0);
+  const int c0 = max(0, min(a.cu_q[b], a.T)), nq = min(a.max_q, max(0, max(0, min(a.cu_q[b + 1], a.T)) - c0));
   const int tile = (nq * a.G + RT - 1) / RT - 1 - back, row = tile * RT + r;
   if (tile < 0 || row >= nq * a.G) return;
   const float* p = a.part + prompt_part<D>(a, blockIdx.y, 0);
@@ -673,7 +680,7 @@ void kv4_prompt_launch(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_le
   a.B = (int)seq_lens.size(0); a.W = (int)table.size(1);
   a.q = q.data_ptr(); a.q_tok = q.stride(0); a.q_head = (int)q.stride(1);
   a.cu_q = (const int*)cu_q.data_ptr(); a.seq_lens = (const int*)seq_lens.data_ptr();
-  a.table = (const int*)table.data_ptr(); a.window = (int)window;
+  a.table = (const int*)table.data_ptr(); a.max_q = (int)std::min<int64_t>(max_q, a.T); a.window = (int)window;
   a.pages = (const uint8_t*)pages.data_ptr(); a.n_pages = (int)pages.size(0);
   a.scale_log2 = (float)(scale * 1.4426950408889634 * std::ldexp(1.0, (int)k_exp));
   a.v_mul = std::ldexp(1.f, (int)v_exp);

@@ -28,7 +28,7 @@ namespace kv4 {
 
 struct SelectArgs {
   const void* q; long long q_tok; int q_head;
-  const int *cu_q, *seq_lens, *table; int B, W, T, H, G;
+  const int *cu_q, *seq_lens, *table; int B, W, T, H, G, max_q;
   int gp, tpc;                        // rows reserved per token (a power of two or a multiple of 8), tokens per block
   int tiles, chunks, span;            // token tiles per sequence; chunks of 128 pages, in spans of so many per block
   const int8_t* bounds; const float* unit; int n_pages;
@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(kScoreWarps * 32) kv4_score_kernel(SelectArgs 
   const int b = bt / a.tiles, tile = bt % a.tiles;
   int c0, nq, p0;
   seq_rows(a, b, c0, nq, p0);
-  const int i0 = tile * a.tpc, ntok = min(a.tpc, nq - i0);
+  const int i0 = tile * a.tpc, ntok = min(a.tpc, min(nq, a.max_q) - i0);
   if (ntok <= 0) return;
   const int end = rivals_end(a, p0 + i0 + ntok - 1);       // the last token's
   if (chunk0 * kChunk >= end) return;
@@ -253,6 +253,11 @@ MOET_DEVICE Pick pick_row(const SelectArgs& a, int tok, int h, int tid, int thre
     for (int i = tid; i < a.budget; i += threads) r.out[i] = i < r.n ? i : -1;
     return r;
   }
+  if (tok - c0 >= a.max_q) {         // its scores were not computed
+    for (int i = tid; i < a.budget; i += threads) r.out[i] = -1;
+    if (tid == 0) set_status(a.status, kBadSize);
+    return r;
+  }
   r.want = a.budget - a.first - a.last;
   for (int i = tid; i < a.first; i += threads) r.out[i] = i;
   for (int i = tid; i < a.last; i += threads) r.out[a.budget - a.last + i] = r.end + i;
@@ -424,7 +429,8 @@ void kv4_select_launch(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_le
   while (a.gp < a.G && a.gp < 8) a.gp *= 2;
   if (a.G > 8) a.gp = (a.G + 7) / 8 * 8;
   a.tpc = kScoreRows / a.gp;
-  a.tiles = (int)((std::min<int64_t>(max_q, a.T) + a.tpc - 1) / a.tpc);
+  a.max_q = (int)std::min<int64_t>(max_q, a.T);
+  a.tiles = (a.max_q + a.tpc - 1) / a.tpc;
   a.chunks = (a.W + kScoreWarps * 16 - 1) / (kScoreWarps * 16);
   // As many chunks per block as leave four blocks per SM: a block converts its rows once per span.  us with
   // 2 / 4 / 8 per SM, cold, choice included: 32 tokens over 1.1 M positions 36 / 34 / 36, 1024 tokens over

@@ -875,3 +875,28 @@ def test_a_batch_without_sequence_rows(KV4Cache, max_q):
     assert (out == 0).all() and (lse == -math.inf).all()
     assert (c.select(q, cu, sl, tb, 3, max_q=max_q) == -1).all()
     c.check()
+
+
+# ----------------------------------------------------------------------------- max_q below the rows
+@pytest.mark.parametrize("news,max_q,G,D", [([200, 9], 40, 8, 128), ([90, 200], 64, 4, 64), ([200, 20], 33, 2, 256)])
+def test_more_rows_than_max_q_are_reported(KV4Cache, news, max_q, G, D):
+    """The rows up to max_q are whole; those past it are zeros (no pages), and the status says so."""
+    x = Batch([900, 700], news, 2, G, D, seed=45)
+    c = x.cache(KV4Cache)
+    args = x.args()
+    ref, ref_lse = c.attend(*args, 0.1, max_q=max(news), return_lse=True)
+    ref_pages = c.select(*args, 5, max_q=max(news))
+    c.check()
+    some = torch.cat([torch.arange(n) < max_q for n in news]).to(DEV)
+    poison((ref.shape, ref.dtype), (ref.shape[:2], torch.float32))
+    out, lse = c.attend(*args, 0.1, max_q=max_q, return_lse=True)
+    assert int(c.status) == 3
+    c.status.zero_()
+    assert torch.isfinite(out).all() and (out[~some] == 0).all() and (lse[~some] == -math.inf).all()
+    # another plan may cut a tile's keys elsewhere: P in f16 and one rounding of the output apart
+    assert torch.allclose(out[some].float(), ref[some].float(), rtol=2.0 ** -7, atol=2.0 ** -9 * 6)
+    assert torch.allclose(lse[some], ref_lse[some], rtol=0, atol=2.0 ** -11)
+    pages = c.select(*args, 5, max_q=max_q)
+    assert int(c.status) == 3
+    assert torch.equal(pages[some], ref_pages[some])
+    assert (pages[~some] == -1).all()

@@ -31,7 +31,7 @@ from . import native
 
 PAGE = 64
 HEAD_DIMS = (64, 128, 256)
-_STATUS = {1: "a slot, page, length or row offset out of range", 2: "a wait on the device ran out", 3: "bad size",
+_STATUS = {1: "a slot, page, length or row offset out of range", 2: "a wait on the device ran out", 3: "a sequence with more rows than max_q",
            4: "a key or value that is not finite (NaN is held as 0, infinities as the largest value)"}
 
 
@@ -92,7 +92,8 @@ class KV4Cache:
 
         The first ``first`` and the last ``last`` (>= 1) pages up to the row's own are always taken; the
         others compete by an upper bound on their logits that is computed exactly, so equal inputs give
-        equal choices on every rank, and ties go to the lowest page.  Needs the rows' own positions
+        equal choices on every rank, and ties go to the lowest page.  A row past ``max_q`` of its sequence may
+        get no page, which sets the status.  Needs the rows' own positions
         appended: pages before a row's last one must be complete."""
         return self._C.kv4_select(q, cu_q, seq_lens, block_table, budget, first, last, -1 if max_q is None else max_q,
                                   self.pages, self.bounds, self.unit, self.status)
@@ -102,7 +103,8 @@ class KV4Cache:
                return_lse: bool = False) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
         """softmax(scale * q k^T) v for every row of the batch -> [rows, heads, head_dim] in q's type.
 
-        ``max_q``: the most rows of one sequence (default: all rows).  ``window`` > 0: only the last
+        ``max_q``: the most rows of one sequence (default: all rows); it sizes the work, so give it where it
+        is known.  Rows past it may come out as zeros, which sets the status.  ``window`` > 0: only the last
         ``window`` positions up to the row's own.  ``pages`` int32 [rows, K/V heads, n]: only the
         positions of these pages of the row's sequence (logical indices, each at most once, -1 for
         none), as :meth:`select` gives them.  A row that sees nothing is zeros.  ``return_lse``:
