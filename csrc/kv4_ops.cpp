@@ -167,6 +167,7 @@ std::tuple<Tensor, optional<Tensor>> kv4_attend(Tensor q, Tensor cu_q, Tensor se
   const c10::cuda::CUDAGuard guard(pages.device());
   const int64_t G = check_batch(q, cu_q, seq_lens, table, pages, c, max_q);
   TORCH_CHECK(window >= 0 && window < (int64_t)1 << 31, "kv4: window must be >= 0");
+  if (window >= table.size(1) * 64) window = 0;     // hides nothing; so position - window stays well within 32 bits
   const int64_t T = q.size(0);
   if (chosen.has_value())
     TORCH_CHECK(chosen->device() == pages.device() && chosen->scalar_type() == at::kInt && chosen->is_contiguous() &&

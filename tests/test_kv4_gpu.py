@@ -900,3 +900,19 @@ def test_more_rows_than_max_q_are_reported(KV4Cache, news, max_q, G, D):
     assert int(c.status) == 3
     assert torch.equal(pages[some], ref_pages[some])
     assert (pages[~some] == -1).all()
+
+
+# ------------------------------------------------------------------------------------ huge windows
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 5, 64 * 5, 64 * 5 - 1])
+@pytest.mark.parametrize("max_q", [20, 200])
+def test_a_window_past_the_table_hides_nothing(KV4Cache, window, max_q):
+    """With sequences that are shorter than their rows: positions below zero take part in the window's arithmetic."""
+    x = Batch([5, 300], [20, 7], 1, 1, 64, seed=46)
+    c = x.cache(KV4Cache)
+    args = x.args()
+    out, lse = c.attend(*args, 0.2, max_q=max_q, window=window, return_lse=True)
+    check(out, lse, x.oracle(0.2, window), 300)
+    pages = torch.arange(5, dtype=torch.int32, device=DEV).expand(27, 1, 5).contiguous()
+    out, lse = c.attend(*args, 0.2, max_q=max_q, window=window, pages=pages, return_lse=True)
+    check(out, lse, x.oracle(0.2, window), 300)
+    c.check()
