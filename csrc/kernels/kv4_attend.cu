@@ -9,8 +9,8 @@
 // the block's e4m3 scale: exact, kv4.cuh) straight into the A fragments; P goes from the
 // accumulator layout to a B fragment by one 8x8 transpose per tile.  Queries are held as f16:
 // bf16 rows are scaled by a power of two to at most 512 first, which leaves their 8
-// significant bits whole down to 2^-23 of the row's maximum.  P <= 1 is rounded to f16 (11
-// bits, three more than a bf16 output has); maxima, sums and outputs stay in 32 bits.
+// significant bits whole down to 2^-23 of the row's maximum.  P <= 2^14 is rounded to f16 (11
+// bits, three more than a bf16 output has); references, sums and outputs stay in 32 bits.
 //
 // What bounds it is the cache's bytes (a long context), so each warp streams its own units
 // (pages) through a private ring of bulk copies, one for a page's keys and one for its
@@ -81,6 +81,10 @@ MOET_DEVICE float fast_exp2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// What a row's weights exp2(s - reference) refer to: 14 below its largest score, so that the weights use f16's range up to
+// 2^14 and those of a long tail, down to 2^-28 of the largest, keep all their bits.  Scores that are too large for
+// the difference to be near 14 in f32 refer to the largest itself.
+MOET_DEVICE float reference(float top) { return fabsf(top) < 1048576.f ? top - 14.f : top; }
 MOET_DEVICE void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(tc::smem_addr(bar)), "r"(bytes) : "memory");
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
@@ -471,7 +475,7 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, NT>()) kv4_atten
           uint32_t pf[MT][NT][2];
 #pragma unroll
           for (int n = 0; n < NT; n++) {
-            float mx[2] = {m[n][0], m[n][1]};
+            float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
             for (int mt = 0; mt < MT; mt++) {
               mul2(s[mt][n][0], s[mt][n][1], cs[n][0], cs[n][1]);
@@ -494,6 +498,7 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, NT>()) kv4_atten
             for (int c = 0; c < 2; c++) {
 #pragma unroll
               for (int off = 4; off < 32; off <<= 1) mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], off));
+              mx[c] = fmaxf(m[n][c], reference(mx[c]));
             }
             const float ref0 = mx[0] == -INFINITY ? 0.f : mx[0], ref1 = mx[1] == -INFINITY ? 0.f : mx[1];
             if (__any_sync(0xffffffffu, mx[0] != m[n][0] || mx[1] != m[n][1])) {

@@ -11,8 +11,10 @@
 // softmax, 64 keys at a step; one warp issues the products.  Each tile has two S buffers, so its
 // next scores are computed under its softmax; the order of issue is S0' PV0 S1' PV1 (' = next step).
 //
-// The running maximum is only moved when a row's scores exceed it by 2^8 (P <= 256 in f16, sums
-// in f32): O is rescaled a few times per row, not per block.  Operands are
+// The running maximum is only moved when a row's scores exceed it by 2^8: O is rescaled a few times
+// per row, not per block.  Weights are P = 2^7 exp2(score - maximum) <= 2^15 in f16: a weight of a long
+// tail is off by at most 2^-32 of the row's largest (2^-11 of itself down to 2^-21 of that); sums stay in
+// f32.  A chunk of 2048 rows over 16384 keys takes 579 us so, 588 if the maximum moves at 2^6 and 607 at 2^4.  Operands are
 // in the no-swizzle core-matrix order; the orders of values (depth of S, columns of O) are the
 // ones the cache's pieces give, so every 16-byte store of the conversion is one core-matrix row
 // and a warp's stores fill whole matrices without bank conflicts.
@@ -150,6 +152,8 @@ template <typename T16> MOET_DEVICE uint32_t down2(float a, float b);
 template <> MOET_DEVICE uint32_t down2<__half>(float a, float b) { return f16x2(a, b); }
 template <> MOET_DEVICE uint32_t down2<__nv_bfloat16>(float a, float b) { return pack_bf16x2(a, b); }
 }  // namespace pr
+
+constexpr float kSlack = 8.f, kLift = 7.f;       // in powers of two; together 15, as f16 holds
 
 // where the part of one stretch of a tile's keys lies: rows x D outputs, then the rows' maxima and sums
 template <int D> MOET_DEVICE long long prompt_part(const PromptArgs& a, int entry, int split) {
@@ -294,7 +298,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
         const bool gone = sm.gone[i & 15];
         const bool edge = gone || j0 + SK - 1 > pt_first || (a.window > 0 && j0 <= pt_last - a.window);
         tc::tmem_wait_ld();
-        // the row's largest score; where it exceeds the reference by 2^8 (or there is none yet) the reference moves
+        // the row's largest score; where it exceeds the reference by kSlack (or there is none yet) the reference moves
         float top = -INFINITY, top1 = -INFINITY;
 #pragma unroll
         for (int c = 0; c < SK / 32; c++) {
@@ -308,7 +312,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
         top = fmaxf(top, top1);
         const float raw = top;
         top *= cs;
-        const bool move = m == -INFINITY ? top > -INFINITY : top > m + 8.f;
+        const bool move = m == -INFINITY ? top > -INFINITY : top > m + kSlack;
         if (__any_sync(0xffffffffu, move)) {
           const float f = !move ? 1.f : m == -INFINITY ? 0.f : pr::exp2_fast(m - top);
           if (move) m = top, rest = __fmaf_rn(raw, cs, -top);
@@ -339,7 +343,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
           for (int k = 0; k < 32; k += 2) {
             float x = __uint_as_float(u[c][k]), y = __uint_as_float(u[c][k + 1]);
             pr::fma2(x, y, cs, -ref);
-            pr::add2(x, y, -rest, -rest);
+            pr::add2(x, y, kLift - rest, kLift - rest);
             x = pr::exp2_fast(x), y = pr::exp2_fast(y);
             pr::add2(s0, s1, x, y);
             pk[k / 2] = pr::f16x2(x, y);
@@ -403,7 +407,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
               }
             }
           }
-        if (on && a.lse && !part) a.lse[at] = l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.6931471805599453f;
+        if (on && a.lse && !part) a.lse[at] = l == 0.f ? -INFINITY : (m + (__log2f(l) - kLift)) * 0.6931471805599453f;
       }
     }
   } else if (warp < C::kSoftWarps + 4) {
@@ -631,7 +635,7 @@ __global__ void __launch_bounds__(256) kv4_prompt_join_kernel(PromptArgs a) {
   *reinterpret_cast<uint4*>((T16*)a.out + at * D + d) =
       make_uint4(pr::down2<T16>(x[0] * inv, x[1] * inv), pr::down2<T16>(x[2] * inv, x[3] * inv),
                  pr::down2<T16>(x[4] * inv, x[5] * inv), pr::down2<T16>(x[6] * inv, x[7] * inv));
-  if (a.lse && d == 0) a.lse[at] = sum == 0.f ? -INFINITY : (M + __log2f(sum)) * 0.6931471805599453f;
+  if (a.lse && d == 0) a.lse[at] = sum == 0.f ? -INFINITY : (M + (__log2f(sum) - kLift)) * 0.6931471805599453f;
 }
 
 static int64_t prompt_tiles(int64_t T, int64_t G, int64_t D, int64_t max_q) {

@@ -916,3 +916,37 @@ def test_a_window_past_the_table_hides_nothing(KV4Cache, window, max_q):
     out, lse = c.attend(*args, 0.2, max_q=max_q, window=window, pages=pages, return_lse=True)
     check(out, lse, x.oracle(0.2, window), 300)
     c.check()
+
+
+# -------------------------------------------------------------------------------- long flat tails
+@pytest.mark.parametrize("bits", [25.05, 24.5, 20.3])
+@pytest.mark.parametrize("mode", ["step", "prompt", "chosen"])
+@pytest.mark.parametrize("D", [64, 256])
+def test_small_weights_of_a_long_tail_count(KV4Cache, D, mode, bits):
+    """One key takes nearly all; 131071 others weigh 2^-bits of it each.  In f16 beside a weight of 1 they would be
+    subnormal or nothing.  Enough rows that a warp has many of a row's pages.  Bound: half an ulp of f16, 2^-11 for a
+    weight in f16, 2^-12 for the sum and the exponent; in a prompt the largest weight is held as 2^7 at least, so each
+    weight is off by half a subnormal step, 2^-25 / 2^7 of it, at most."""
+    n, G, H = 131072, 2, 8
+    B, m = (1, 40) if mode == "prompt" else (64, 1)
+    k = torch.zeros(n, H, D, dtype=torch.float16, device=DEV)
+    v = torch.full((n, H, D), 1.5, dtype=torch.float16, device=DEV)
+    k[70], v[70] = 1.5, 0                                             # 1.5 = 6 * 0.25: held as it is
+    c = KV4Cache(n // 64, H, D, device=DEV)
+    c.append(k, v, torch.arange(n, device=DEV))
+    rk, rv = c.read(torch.tensor([70, 71], device=DEV), torch.float16)
+    assert (rk[0] == 1.5).all() and (rk[1] == 0).all() and (rv[1] == 1.5).all()
+    q = torch.full((B * m, H * G, D), 0.5, dtype=torch.float16, device=DEV)
+    scale = bits * math.log(2) / (D * 0.75)
+    cu = torch.arange(B + 1, dtype=torch.int32, device=DEV) * m
+    sl = torch.full((B,), n, dtype=torch.int32, device=DEV)
+    table = torch.arange(n // 64, dtype=torch.int32, device=DEV).expand(B, -1).contiguous()
+    pages = table[:, None].expand(B, H, -1).contiguous() if mode == "chosen" else None
+    out, lse = c.attend(q, cu, sl, table, scale, max_q=1 if mode != "prompt" else 80, pages=pages, return_lse=True)
+    for i in range(B * m):
+        tail = (n - m + i % m) * 2.0 ** -bits                         # the positions up to the row's own, less the one
+        want = 1.5 * tail / (1 + tail)
+        bound = (2.0 ** -11 + 2.0 ** -11 + 2.0 ** -12) * want + (1.5 * n * 2.0 ** -32 if mode == "prompt" else 0)
+        assert ((out[i].double() - want).abs() <= bound).all(), (out[i, 0, 0], want)
+        assert ((lse[i].double() - (bits * math.log(2) + math.log1p(tail))).abs() <= 2.0 ** -11).all()
+    c.check()
