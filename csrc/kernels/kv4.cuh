@@ -22,6 +22,8 @@
 #include "common.cuh"
 #include <cuda_fp16.h>
 
+#include <cmath>
+
 namespace moet {
 namespace kv4 {
 
@@ -125,6 +127,20 @@ MOET_DEVICE void blank_rows(int first, int last, int T, void* out, float* lse, i
 }
 
 MOET_DEVICE float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }   // -126 <= e <= 127
+
+// What a product of a query and a key is multiplied by (scale * log2(e) * 2^k_exp), as a factor and a power of two:
+// with a row's own power, 2^-118 to 2^119, either may leave f32's range while their product is in it.
+struct ScoreScale {
+  float factor; int exp;
+};
+inline ScoreScale score_scale(double scale, int k_exp) {
+  int e = 0;
+  const double f = std::frexp(scale * 1.4426950408889634, &e);
+  return {(float)f, e + k_exp};
+}
+MOET_DEVICE float row_factor(const ScoreScale& s, int row_exp) {
+  return pow2f(max(-126, min(127, s.exp + row_exp))) * s.factor;
+}
 
 // Smallest e >= -100 with amax <= 127 * 2^e; 0 for amax = 0 (finite amax >= 0).
 MOET_DEVICE int exp_for_127(float amax) {

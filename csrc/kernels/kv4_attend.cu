@@ -40,7 +40,7 @@ struct AttendArgs {
   const int* sel; int budget;                           // [T, H, budget] or null
   int T, H, G, window;
   const uint8_t* pages; int n_pages;
-  float scale_log2;                                     // scale * log2(e) * 2^k_exp
+  ScoreScale scale;
   float v_mul;                                          // 2^v_exp
   void* out; float* lse;                                // [T, H * G, D], [T, H * G] or null
   float* part; int* split;                              // parts: two per block; split: kSplitInts per block
@@ -393,12 +393,13 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, NT>()) kv4_atten
           amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
         }
       }
-      float mul = 1.f, back = 1.f;
+      float mul = 1.f;
+      int e = 0;                            // queries are held times 2^-e
       if (sizeof(T16) == 2 && !std::is_same<T16, __half>::value) {
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        const int e = amax > 0.f ? max(-110, min(110, (int)(__float_as_uint(amax) >> 23) - 127 - 8)) : 0;
-        mul = pow2f(-e), back = pow2f(e);
+        e = amax > 0.f ? max(-110, min(119, (int)(__float_as_uint(amax) >> 23) - 127 - 8)) : 0;
+        mul = pow2f(-e);
       }
 #pragma unroll
       for (int w = 0; w < KW; w++)
@@ -410,7 +411,7 @@ __global__ void __launch_bounds__(kWarps * 32, blocks_per_sm<D, NT>()) kv4_atten
         }
 #pragma unroll
       for (int c = 0; c < 2; c++) {
-        cs[n][c] = __shfl_sync(0xffffffffu, back, (2 * t + c) * 4) * a.scale_log2;
+        cs[n][c] = row_factor(a.scale, __shfl_sync(0xffffffffu, e, (2 * t + c) * 4));
         const int rc = min(tl.row0 + n * 8 + 2 * t + c, tl.rows - 1);
         pc[n][c] = tl.p0 + (a.sel ? 0 : rc / a.G);
       }
@@ -755,7 +756,7 @@ void kv4_attend_launch(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_le
   a.budget = chosen ? (int)sel->size(2) : 0;
   a.T = T; a.H = H; a.G = G; a.window = (int)window;
   a.pages = (const uint8_t*)pages.data_ptr(); a.n_pages = (int)pages.size(0);
-  a.scale_log2 = (float)(scale * 1.4426950408889634 * std::ldexp(1.0, (int)k_exp));
+  a.scale = score_scale(scale, (int)k_exp);
   a.v_mul = std::ldexp(1.f, (int)v_exp);
   a.out = out.data_ptr(); a.lse = (float*)opt_ptr(lse);
   a.part = (float*)part.data_ptr(); a.split = (int*)split.data_ptr();

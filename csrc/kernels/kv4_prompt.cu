@@ -46,7 +46,8 @@ struct PromptArgs {
   const void* q; long long q_tok; int q_head;
   const int *cu_q, *seq_lens, *table; int B, W, T, H, G, max_q, window;
   const uint8_t* pages; int n_pages;
-  float scale_log2, v_mul;
+  ScoreScale scale;
+  float v_mul;
   void* out; float* lse;
   int whole, splits;                  // tiles that a block takes whole, stretches of keys of each of the others
   float* part;                        // the stretches' outputs, maxima and sums
@@ -244,17 +245,18 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
           amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
         }
       }
-    float mul = 1.f, back = 1.f;
+    float mul = 1.f;
+    int e = 0;                                             // the row is held times 2^-e
     if (!std::is_same<T16, __half>::value) {
       const uint32_t quad = 0xFu << (lane & 28);
       amax = fmaxf(amax, __shfl_xor_sync(quad, amax, 1));
       amax = fmaxf(amax, __shfl_xor_sync(quad, amax, 2));
-      const int e = amax > 0.f ? max(-110, min(110, (int)(__float_as_uint(amax) >> 23) - 127 - 8)) : 0;
-      mul = pow2f(-e), back = pow2f(e);
+      e = amax > 0.f ? max(-110, min(119, (int)(__float_as_uint(amax) >> 23) - 127 - 8)) : 0;
+      mul = pow2f(-e);
     }
     // the scale's sign goes to the row, so that scores only grow; above 0, so that -inf stays what it is
-    if (t == 0) sm.row_scale[r] = fmaxf(back * fabsf(a.scale_log2), 1e-30f);
-    mul = copysignf(mul, a.scale_log2);
+    if (t == 0) sm.row_scale[r] = fmaxf(fabsf(row_factor(a.scale, e)), 1e-30f);
+    mul = copysignf(mul, a.scale.factor);
     uint8_t* dst = sm.q[r >> 7] + ((r & 127) >> 3) * kQSbo + (r & 7) * 16;
 #pragma unroll
     for (int sl = 0; sl < L::NS; sl++)
@@ -686,7 +688,7 @@ void kv4_prompt_launch(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_le
   a.cu_q = (const int*)cu_q.data_ptr(); a.seq_lens = (const int*)seq_lens.data_ptr();
   a.table = (const int*)table.data_ptr(); a.max_q = (int)std::min<int64_t>(max_q, a.T); a.window = (int)window;
   a.pages = (const uint8_t*)pages.data_ptr(); a.n_pages = (int)pages.size(0);
-  a.scale_log2 = (float)(scale * 1.4426950408889634 * std::ldexp(1.0, (int)k_exp));
+  a.scale = score_scale(scale, (int)k_exp);
   a.v_mul = std::ldexp(1.f, (int)v_exp);
   a.out = out.data_ptr(); a.lse = (float*)opt_ptr(lse);
   a.status = (int*)status.data_ptr();

@@ -950,3 +950,18 @@ def test_small_weights_of_a_long_tail_count(KV4Cache, D, mode, bits):
         assert ((out[i].double() - want).abs() <= bound).all(), (out[i, 0, 0], want)
         assert ((lse[i].double() - (bits * math.log(2) + math.log1p(tail))).abs() <= 2.0 ** -11).all()
     c.check()
+
+
+# ------------------------------------------------------------------------------- the largest queries
+@pytest.mark.parametrize("max_q", [2, 500])
+def test_bf16_queries_up_to_the_type_s_largest(KV4Cache, max_q):
+    x = Batch([300], [2], 1, 4, 64, seed=48)
+    x.k = (x.k.float() * 2.0 ** -6).to(torch.bfloat16)
+    x.q[0, 1] = (x.q[0, 1].float() * 2.0 ** 124).clamp(-3.38e38, 3.38e38).to(torch.bfloat16)
+    x.q[1, 3, ::2] = -3.3895314e38                                     # the type's lowest value
+    x.q[1, 3, 1::2] = 3.3895314e38
+    assert torch.isfinite(x.q).all()
+    c = x.cache(KV4Cache)
+    scale = 2.0 ** -121
+    out, lse = c.attend(*x.args(), scale, max_q=max_q, return_lse=True)
+    check(out, lse, x.oracle(scale), 300)
