@@ -83,7 +83,7 @@ template <typename T16> MOET_DEVICE uint32_t scale_of(const uint32_t (&w)[8], fl
 #pragma unroll
     for (int i = 0; i < 16; i++) {
       const float y = __fmul_rn(x[i], r);
-      x[i] = __fmaf_rn(__fmaf_rn(-y, s, x[i]), r, y);
+      x[i] = copysignf(__fmaf_rn(__fmaf_rn(-y, s, x[i]), r, y), x[i]);      // -0 stays -0
     }
   }
   return s8;

@@ -77,3 +77,16 @@ def test_cache_refuses_what_it_cannot_hold():
                      ((4, 2, 64), {"v_exp": -15}), ((4, 2, 64), {"device": "cpu"})):
         with pytest.raises(ValueError):
             KV4Cache(*args, **kw)
+
+
+def test_the_sign_of_zero_is_kept():
+    """As the format says, and as the kernel that writes the cache has it."""
+    x = torch.zeros(3, 64)
+    x[0] = -0.0
+    x[1, ::2] = -0.0
+    x[2, :4] = torch.tensor([-0.0, 6.0, -1e-9, 0.0])
+    codes, s8 = kv4.quantise(x)
+    assert (codes[0] == 8).all() and not s8[0].any()
+    assert (codes[1, ::2] == 8).all() and (codes[1, 1::2] == 0).all()
+    assert codes[2, :4].tolist() == [8, 7, 8, 0]
+    assert torch.equal(kv4.values(codes, s8)[:2], torch.zeros(2, 64))

@@ -965,3 +965,17 @@ def test_bf16_queries_up_to_the_type_s_largest(KV4Cache, max_q):
     scale = 2.0 ** -121
     out, lse = c.attend(*x.args(), scale, max_q=max_q, return_lse=True)
     check(out, lse, x.oracle(scale), 300)
+
+
+# --------------------------------------------------------------------------------- negative zeros
+@pytest.mark.parametrize("D,dtype", [(64, torch.float16), (128, torch.bfloat16)])
+def test_negative_zeros_keep_their_sign(KV4Cache, D, dtype):
+    g = torch.Generator().manual_seed(49)
+    k = torch.randn(64, 1, D, generator=g).to(dtype)
+    k[:, :, ::3] = -0.0
+    k[5] = -0.0
+    k[6] = 0.0
+    c = KV4Cache(1, 1, D, device=DEV)
+    c.append(k.to(DEV), k.to(DEV), torch.arange(64, device=DEV))
+    codes, s8 = kv4.quantise(k[:, 0])
+    assert torch.equal(c.pages[0, 0].cpu(), kv4.pack_page(codes, s8, codes, s8))

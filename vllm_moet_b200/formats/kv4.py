@@ -29,7 +29,7 @@ def quantise(x: torch.Tensor, exp: int = -6) -> Tuple[torch.Tensor, torch.Tensor
     a = y.abs()
     code = ((a > 0.25 * s).int() + (a >= 0.75 * s) + (a > 1.25 * s) + (a >= 1.75 * s) + (a > 2.5 * s)
             + (a >= 3.5 * s) + (a > 5 * s))
-    code = torch.where(s > 0, code, 0) + 8 * (y < 0)
+    code = torch.where(s > 0, code, 0) + 8 * torch.signbit(y)
     return code.to(torch.uint8).flatten(-2), s8.view(torch.uint8)
 
 
