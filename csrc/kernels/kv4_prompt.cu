@@ -70,8 +70,8 @@ template <int D> struct PromptSmem {
   uint8_t v[2][C::kKBytes];
   float row_scale[C::TILES * 128];
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], pv_done[2], o_full[2], done;
-  uint32_t gone[16];                   // of step n's page, in place n & 15: it is not in the pool
   uint32_t tmem;
+  const int* holes;                    // the sequence's table row where a page is missing, else null
 };
 
 namespace pr {
@@ -208,6 +208,16 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
   const int nkb = kb1 - kb0;
   const int steps = nkb > 0 ? min(p_last / C::SK + 1, kb1 * C::HALVES) - kb0 * C::HALVES : 0;   // softmax steps
 
+  // ---- pages of this stretch that some row sees and that are not in the pool: reported, and hidden step by step.  Looked
+  // for once, in front: flags that the conversion passes on with every step cost D = 256 14 %, D = 128 1 %.
+  constexpr int KP = BK / kPage;
+  const int page0 = max(kb0 * KP, a.window > 0 ? max(0, p_first - a.window + 1) / kPage : 0);
+  const int page1 = nkb > 0 ? min(kb1 * KP, p_last / kPage + 1) : 0;
+  auto in_pool = [&](int phys) { return (uint32_t)phys < (uint32_t)a.n_pages; };
+  bool missing = false;
+  for (int x = page0 + tid; x < page1; x += C::kWarps * 32) missing |= !in_pool(a.table[(long long)b * a.W + x]);
+  if (tid == 0) sm.holes = nullptr;
+
   // ---- queries as f16 operands (bf16 rows scaled to at most 512), barriers, tensor memory
   if (warp == 0) tc::tmem_alloc(&sm.tmem, 512);
   if (tid == 0) {
@@ -270,7 +280,14 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
   }
   tc::fence_proxy_async_smem();
   tc::fence_before();
-  __syncthreads();
+  const bool holes = __syncthreads_or(missing);
+  if (holes) {
+    if (tid == 0) {
+      sm.holes = a.table + (long long)b * a.W;
+      set_status(a.status, kBadIndex);
+    }
+    __syncthreads();
+  }
   tc::fence_after();
   const uint32_t tmem = sm.tmem;
   bool ok = true;
@@ -281,7 +298,8 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t o_at = tmem + lanes + C::kOCol + t * D;
     const int row = row0 + r, p = p0 + min(row, rows - 1) / a.G;
-    const int pt_first = p0 + (row0 + t * 128) / a.G, pt_last = p0 + min(row0 + t * 128 + 127, rows - 1) / a.G;
+    const int pt_first = holes ? -1 : p0 + (row0 + t * 128) / a.G;     // with holes, every step is looked at key by key
+    const int pt_last = p0 + min(row0 + t * 128 + 127, rows - 1) / a.G;
     const float cs = sm.row_scale[r];
     // the reference is the product m + rest, exactly: the largest score's own difference is 0 at any size
     float m = -INFINITY, rest = 0.f, l = 0.f;
@@ -296,15 +314,15 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
         uint32_t u[SK / 32][32];
 #pragma unroll
         for (int c = 0; c < SK / 32; c++) pr::ld32(s_at + c * 32, u[c]);
-        // a page that is not there is seen by no row; the look-up is at most four key blocks ahead of this step
-        const bool gone = sm.gone[i & 15];
-        const bool edge = gone || j0 + SK - 1 > pt_first || (a.window > 0 && j0 <= pt_last - a.window);
+        const bool edge = j0 + SK - 1 > pt_first || (a.window > 0 && j0 <= pt_last - a.window);
         tc::tmem_wait_ld();
         // the row's largest score; where it exceeds the reference by kSlack (or there is none yet) the reference moves
         float top = -INFINITY, top1 = -INFINITY;
+        int pe = p;
+        if (edge && sm.holes && !in_pool(sm.holes[j0 / kPage])) pe = -1;     // nobody sees a page that is not there
 #pragma unroll
         for (int c = 0; c < SK / 32; c++) {
-          if (edge) hide<32>(u[c], j0 + c * 32, gone ? -1 : p, a.window);
+          if (edge) hide<32>(u[c], j0 + c * 32, pe, a.window);
 #pragma unroll
           for (int k = 0; k < 32; k += 4) {
             top = pr::max3(top, __uint_as_float(u[c][k]), __uint_as_float(u[c][k + 1]));
@@ -422,32 +440,17 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
     const int vg = dt & 7, vo = (dt >> 3) % OCT, vsl = (dt >> 3) / OCT;
     uint32_t kc[KI][W], vc[4][W];
     uint16_t ks[KI], vs[4];                                  // scales as they are held: converting waits for the load
-    // pages of a key block, looked up two blocks ahead (the look-up is a load of its own)
-    constexpr int KP = BK / kPage;
-    // pages that some row of the tile sees; the others are neither looked at nor reported
-    auto seen = [&](int kb, int i) {
-      const int x = (kb * KP + i) * kPage;
-      return kb < kb1 && kb * KP + i < a.W && x <= p_last && (a.window == 0 || x + kPage > p_first - a.window + 1);
-    };
+    // pages of a key block, looked up two blocks ahead (the look-up is a load of its own): -1 for none
     int ahead[KP], page[KP];                                 // of the block after the next one, of the next one
-    auto look_up = [&](int kb) {
-#pragma unroll
-      for (int i = 0; i < KP; i++) ahead[i] = seen(kb, i) ? a.table[(long long)b * a.W + kb * KP + i] : 0;
-    };
-    // the pages of block n (kb = kb0 + n) as looked up, -1 where there is nothing to load; whoever is missing is reported
-    auto take = [&](int n) {
+    auto look_up = [&](int kb, int (&to)[KP]) {
 #pragma unroll
       for (int i = 0; i < KP; i++) {
-        const bool want = seen(kb0 + n, i), there = (uint32_t)ahead[i] < (uint32_t)a.n_pages;
-        page[i] = want && there ? ahead[i] : -1;
-        if (dt == 0) {
-          sm.gone[n * KP + i & 15] = want && !there;
-          if (want && !there) set_status(a.status, kBadIndex);
-        }
+        const int x = kb * KP + i;
+        to[i] = x >= page0 && x < page1 ? a.table[(long long)b * a.W + x] : -1;
       }
     };
     auto at = [&](int phys) -> const uint8_t* {
-      return phys < 0 ? nullptr : a.pages + ((long long)phys * a.H + h) * L::kPageBytes;
+      return in_pool(phys) ? a.pages + ((long long)phys * a.H + h) * L::kPageBytes : nullptr;
     };
     auto fetch_k = [&](int kb) {
 #pragma unroll
@@ -482,9 +485,8 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
         }
       }
     };
-    look_up(kb0);
-    take(0);
-    look_up(kb0 + 1);
+    look_up(kb0, page);
+    look_up(kb0 + 1, ahead);
     fetch_k(kb0);
     fetch_v(kb0);
     for (int i = 0; i < nkb && ok; i++) {
@@ -506,9 +508,10 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
       }
       tc::fence_proxy_async_smem();
       pr::arrive(&sm.k_full[st]);
-      take(i + 1);
+#pragma unroll
+      for (int x = 0; x < KP; x++) page[x] = ahead[x];
       fetch_k(kb0 + i + 1);
-      look_up(kb0 + i + 2);
+      look_up(kb0 + i + 2, ahead);
       if (i >= 2) ok = tc::mbar_wait(&sm.v_empty[st], ((i >> 1) - 1) & 1, MOET_KV4_TRIES);
       if (!ok) break;
       // values: a thread has 8 tokens of its piece: per value one 16-byte row of a core matrix
