@@ -49,7 +49,7 @@ struct PromptArgs {
   ScoreScale scale;
   float v_mul;
   void* out; float* lse;
-  int whole, splits;                  // tiles that a block takes whole, stretches of keys of each of the others
+  int whole, splits;                  // tiles that a block takes whole; stretches of keys of each of the others, at most
   float* part;                        // the stretches' outputs, maxima and sums
   int* status;
 };
@@ -154,12 +154,40 @@ template <> MOET_DEVICE uint32_t down2<__half>(float a, float b) { return f16x2(
 template <> MOET_DEVICE uint32_t down2<__nv_bfloat16>(float a, float b) { return pack_bf16x2(a, b); }
 }  // namespace pr
 
+// Keys of a stretch, at least.  us with 128 / 256 / 512, 8 K/V heads, 4 rows per token, B200: 128 tokens of 1000 keys,
+// D = 128: 26.4 / 25.9 / 28.9, D = 64: 20.8 / 19.5 / 22.2; 70 tokens, D = 256: 24.4 / 24.0 / 27.8; 4 sequences of 40
+// tokens and 700 keys, D = 64: 17.7 / 18.1 / 20.4.
+constexpr int kMinStretch = 256;
 constexpr float kSlack = 8.f, kLift = 7.f;       // in powers of two; together 15, as f16 holds
 
 // where the part of one stretch of a tile's keys lies: rows x D outputs, then the rows' maxima and sums
 template <int D> MOET_DEVICE long long prompt_part(const PromptArgs& a, int entry, int split) {
   return ((long long)entry * a.splits + split) * (PromptCfg<D>::TILES * 128 * (D + 2));
 }
+
+// Entry of the grid's order: a row tile of a sequence and K/V head, the last rows (the longest stretches of keys) of every
+// sequence and head first.
+template <int D> struct PromptTile {
+  int b, h, back;                     // back: tiles of the sequence behind this one
+  int c0, all, nq, p0;                // first row, rows, rows within max_q, position of the first row
+  int rows, tile, row0, live;         // query rows; tile (< 0: none), its first row and rows
+  int p_first, p_last;                // positions of its first and last row
+  int from, to, splits;               // its key blocks [from, to), and the stretches they are shared out over
+  MOET_DEVICE PromptTile(const PromptArgs& a, int entry) {
+    constexpr int RT = PromptCfg<D>::TILES * 128, BK = PromptCfg<D>::BK;
+    b = entry % a.B, h = entry / a.B % a.H, back = entry / (a.B * a.H);
+    c0 = max(0, min(a.cu_q[b], a.T)), all = max(0, max(0, min(a.cu_q[b + 1], a.T)) - c0);
+    nq = min(all, a.max_q);                                // the tiles that there are: rows past them are reported
+    p0 = held_length(a.seq_lens[b], a.W) - all;
+    rows = nq * a.G;
+    tile = (rows + RT - 1) / RT - 1 - back;
+    row0 = tile * RT, live = min(rows - row0, RT);
+    p_first = p0 + row0 / a.G, p_last = p0 + (row0 + live - 1) / a.G;
+    from = a.window > 0 ? max(0, p_first - a.window + 1) / BK : 0;
+    to = p_last < 0 ? from : p_last / BK + 1;
+    splits = entry < a.whole ? 1 : max(1, min(a.splits, (to - from) * BK / kMinStretch));
+  }
+};
 
 // scores of keys j0 .. that the row at position p does not see -> -inf
 template <int N> MOET_DEVICE void hide(uint32_t (&u)[N], int j0, int p, int window) {
@@ -179,32 +207,23 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_entry();
 
-  // tiles in order: the longest stretches of keys (a sequence's last rows) of every sequence and head first
   const int entry = (int)blockIdx.x < a.whole ? blockIdx.x : a.whole + (int)(blockIdx.x - a.whole) / a.splits;
   const int split = (int)blockIdx.x < a.whole ? 0 : (int)(blockIdx.x - a.whole) % a.splits;
-  const int splits = (int)blockIdx.x < a.whole ? 1 : a.splits;
-  const int b = entry % a.B, h = entry / a.B % a.H, back = entry / (a.B * a.H);
-  const int c0 = max(0, min(a.cu_q[b], a.T)), all = max(0, max(0, min(a.cu_q[b + 1], a.T)) - c0);
-  const int nq = min(all, a.max_q);                        // the tiles that there are: rows past them are reported
-  const int rows = nq * a.G, p0 = held_length(a.seq_lens[b], a.W) - all;
-  const int ntiles_seq = (rows + TILES * 128 - 1) / (TILES * 128);
-  const int tile = ntiles_seq - 1 - back;
+  const PromptTile<D> tl(a, entry);
+  const int b = tl.b, h = tl.h, c0 = tl.c0, rows = tl.rows, p0 = tl.p0, splits = tl.splits;
   blank_rows(a.cu_q[0], a.cu_q[a.B], a.T, a.out, a.lse, a.H * a.G, D);
-  if (h == 0 && back == 0 && split == 0) {
+  if (h == 0 && tl.back == 0 && split == 0) {
     if (tid == 0) check_sequence(a.cu_q, a.seq_lens, b, a.T, a.W, a.status);
-    if (all > nq) {
+    if (tl.all > tl.nq) {
       if (tid == 0) set_status(a.status, kBadSize);
-      for (int i = nq; i < all; i++) blank_row(c0 + i, a.out, a.lse, a.H * a.G, D);
+      for (int i = tl.nq; i < tl.all; i++) blank_row(c0 + i, a.out, a.lse, a.H * a.G, D);
     }
   }
-  if (tile < 0) return;
-  const int row0 = tile * TILES * 128, live = min(rows - row0, TILES * 128);
-  const int p_first = p0 + row0 / a.G, p_last = p0 + (row0 + live - 1) / a.G;
+  if (tl.tile < 0 || split >= splits) return;
+  const int row0 = tl.row0, live = tl.live, p_first = tl.p_first, p_last = tl.p_last;
   const int ntile = (live + 127) / 128;
-  const int from = a.window > 0 ? max(0, p_first - a.window + 1) / BK : 0;
-  const int to = p_last < 0 ? from : p_last / BK + 1;              // the tile's key blocks [from, to), shared out evenly
-  const int per = (to - from + splits - 1) / splits;
-  const int kb0 = min(to, from + split * per), kb1 = min(to, kb0 + per);
+  const int per = (tl.to - tl.from + splits - 1) / splits;
+  const int kb0 = min(tl.to, tl.from + split * per), kb1 = min(tl.to, kb0 + per);
   const int nkb = kb1 - kb0;
   const int steps = nkb > 0 ? min(p_last / C::SK + 1, kb1 * C::HALVES) - kb0 * C::HALVES : 0;   // softmax steps
 
@@ -615,18 +634,17 @@ template <int D, typename T16>
 __global__ void __launch_bounds__(256) kv4_prompt_join_kernel(PromptArgs a) {
   constexpr int RT = PromptCfg<D>::TILES * 128;
   pdl_entry();
-  const int entry = a.whole + blockIdx.y, b = entry % a.B, h = entry / a.B % a.H, back = entry / (a.B * a.H);
+  const PromptTile<D> tl(a, a.whole + blockIdx.y);
   const int it = blockIdx.x * 256 + threadIdx.x, r = it / (D / 8), d = it % (D / 8) * 8;
-  const int c0 = max(0, min(a.cu_q[b], a.T)), nq = min(a.max_q, max(0, max(0, min(a.cu_q[b + 1], a.T)) - c0));
-  const int tile = (nq * a.G + RT - 1) / RT - 1 - back, row = tile * RT + r;
-  if (tile < 0 || row >= nq * a.G) return;
+  const int row = tl.row0 + r;
+  if (tl.tile < 0 || row >= tl.rows || tl.splits == 1) return;      // one stretch: its block has written the rows
   const float* p = a.part + prompt_part<D>(a, blockIdx.y, 0);
   constexpr int PF = RT * (D + 2);
   float M = -INFINITY;
-  for (int s = 0; s < a.splits; s++) M = fmaxf(M, p[s * PF + RT * D + r]);
+  for (int s = 0; s < tl.splits; s++) M = fmaxf(M, p[s * PF + RT * D + r]);
   float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, sum = 0.f;
 #pragma unroll 2
-  for (int s = 0; s < a.splits; s++) {
+  for (int s = 0; s < tl.splits; s++) {
     const float m = p[s * PF + RT * D + r], l = p[s * PF + RT * (D + 1) + r];
     if (m == -INFINITY && l == 0.f) continue;          // a stretch of which the row saw nothing
     const float w = m == -INFINITY ? 1.f : pr::exp2_fast(m - M);   // NaN sums have no maximum
@@ -636,7 +654,7 @@ __global__ void __launch_bounds__(256) kv4_prompt_join_kernel(PromptArgs a) {
     sum += w * l;
   }
   const float inv = sum > 0.f ? __fdividef(a.v_mul, sum) : sum;
-  const long long at = (long long)(c0 + row / a.G) * a.H * a.G + h * a.G + row % a.G;
+  const long long at = (long long)(tl.c0 + row / a.G) * a.H * a.G + tl.h * a.G + row % a.G;
   *reinterpret_cast<uint4*>((T16*)a.out + at * D + d) =
       make_uint4(pr::down2<T16>(x[0] * inv, x[1] * inv), pr::down2<T16>(x[2] * inv, x[3] * inv),
                  pr::down2<T16>(x[4] * inv, x[5] * inv), pr::down2<T16>(x[6] * inv, x[7] * inv));
@@ -656,27 +674,28 @@ using namespace moet::kv4;
 
 // {tiles taken whole, stretches of keys of each of the others, floats of `part`}.  Tiles that fill all SMs
 // are taken whole.  The rest (all, where there are fewer tiles than SMs) would leave SMs idle: its keys
-// are split so that the last wave is even, into stretches of at least 512 keys (below that a stretch's
-// set-up, about 5 us, outweighs its keys), unless four or more waves come before it.
+// are split so that the last wave is even, unless four or more waves come before it.  The number of stretches
+// comes from the table's width (or the window) and is the most there can be; each tile takes as many as its own
+// keys fill with kMinStretch keys or more, and the blocks of the others leave at once.
 // 2048 x 4 rows, 8 heads, 16384 keys: 256 tiles, 556 us whole, 550 us with the last 108 in
 // quarters; with D = 256 (512 tiles) 1289 and 1092 us.
 std::tuple<int64_t, int64_t, int64_t> kv4_prompt_plan(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t max_q,
                                                       int64_t W, int64_t window) {
   constexpr int64_t kSms = 148;
   const int64_t n = prompt_tiles(T, G, D, max_q) * H * B, rest = n % kSms;
-  const int64_t keys = window > 0 ? std::min(W * kPage, window + max_q) : W * kPage;
+  const int64_t rt = D == 256 ? 128 : 256, keys = window > 0 ? std::min(W * kPage, window + (rt + G - 1) / G) : W * kPage;
   if (rest == 0 || n >= 4 * kSms) return {n, 1, 0};
   int64_t best = 1;
   if (n < kSms) {
-    best = std::min<int64_t>({kSms / n, keys / 512, 64});
+    best = std::min<int64_t>({kSms / n, keys / kMinStretch, 64});
   } else {
-    for (int64_t s = 2; s <= std::min<int64_t>(keys / 512, 8); s++) {       // waves of stretches / s, 3 % for a split
+    for (int64_t s = 2; s <= std::min<int64_t>(keys / kMinStretch, 8); s++) {       // waves of stretches / s, 3 % for a split
       const auto cost = [&](int64_t x) { return (double)((rest * x + kSms - 1) / kSms) / x + 0.03 * (x - 1); };
       if (cost(s) < cost(best)) best = s;
     }
   }
   if (best <= 1) return {n, 1, 0};
-  return {n - rest, best, rest * best * (D == 256 ? 128 : 256) * (D + 2)};
+  return {n - rest, best, rest * best * rt * (D + 2)};
 }
 
 void kv4_prompt_launch(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_lens, torch::Tensor table,

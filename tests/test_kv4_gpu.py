@@ -979,3 +979,25 @@ def test_negative_zeros_keep_their_sign(KV4Cache, D, dtype):
     c.append(k.to(DEV), k.to(DEV), torch.arange(64, device=DEV))
     codes, s8 = kv4.quantise(k[:, 0])
     assert torch.equal(c.pages[0, 0].cpu(), kv4.pack_page(codes, s8, codes, s8))
+
+
+# ----------------------------------------------------------------------- tables wider than the sequences
+@pytest.mark.parametrize("lens,news,H,G,D,dtype,window", [
+    ([1000], [40], 1, 2, 128, torch.float16, 0),
+    ([300, 1500], [33, 60], 2, 2, 64, torch.bfloat16, 0),
+    ([2000, 100], [70, 100], 1, 2, 256, torch.float16, 0),
+    ([1800], [50], 1, 4, 128, torch.bfloat16, 700),
+    ([3, 1100], [40, 40], 1, 1, 128, torch.float16, 1090),
+])
+def test_a_table_padded_to_the_longest_length(KV4Cache, lens, news, H, G, D, dtype, window):
+    """As a server has it.  A tile's keys are split by what it has, not by what the table could hold: the same bits
+    whether the table is as wide as two or as sixty-four stretches, and whole."""
+    got = []
+    for width in (2048, 512):
+        x = Batch(lens, news, H, G, D, dtype, seed=52, width=width)
+        c = x.cache(KV4Cache)
+        out, lse = c.attend(*x.args(), 0.1, max_q=64 // G + max(news), window=window, return_lse=True)
+        c.check()
+        check(out, lse, x.oracle(0.1, window), max(lens))
+        got.append((out, lse))
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
