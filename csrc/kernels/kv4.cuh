@@ -38,6 +38,14 @@ template <int D> struct Lay {
   static constexpr int kSlabBytes = kPage * SD / 2;  // codes of a slab
 };
 
+// SMs of the current device: grids, plans and the rules that choose between forms go by it
+inline int sm_count() {
+  int dev = 0, n = 0;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  return n > 0 ? n : 148;
+}
+
 // four bytes of two e2m1 codes each -> four f16x2 (low code in the low half)
 MOET_DEVICE void e2m1x8_to_f16(uint32_t w, uint32_t (&r)[4]) {
   asm("{\n.reg .b8 b0, b1, b2, b3;\nmov.b32 {b0, b1, b2, b3}, %4;\n"

@@ -711,16 +711,6 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(AttendArgs a) {
   if (blockIdx.y == 0 && it % 8 == 0) store_lse(a, h, row0 + r, tok0, fm[r], fl[r]);
 }
 
-static int sm_count() {
-  static int n = [] {
-    int dev = 0, v = 0;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev);
-    return v > 0 ? v : 148;
-  }();
-  return n;
-}
-
 // query rows of a tile / 8: the fewest that hold a sequence's rows, as the registers allow.  B200, 8 sequences
 // of 30000, 8 heads of 128, 24 rows: 209 us in two tiles of 16, which convert every page twice, 124 in one of 24.
 static int row_tiles(int64_t rows, int D) {

@@ -399,7 +399,7 @@ void kv4_read_launch(torch::Tensor slots, torch::Tensor pages, int64_t k_exp, in
   const long long threads = (long long)T * H * (D / 8);
   // Four rows a thread where one row each would be two or more full waves (32768 rows x 8 heads: 41 us with
   // one, 37 with four, cold); below that more threads hide the same latency (1574 rows, D = 64: 8.1 and 8.3).
-  const int per = threads >= 2ll * 148 * 2048 ? 4 : 1;
+  const int per = threads >= 2ll * sm_count() * 2048 ? 4 : 1;
   const dim3 grid((unsigned)((threads + 256 * per - 1) / (256 * per)));
   auto launch = [&](auto dim, auto t, auto u) {
     launch_k(kv4_read_kernel<decltype(dim)::value, decltype(t), decltype(u)::value>, grid, dim3(256), 0, stream, a);

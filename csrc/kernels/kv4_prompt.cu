@@ -681,16 +681,16 @@ using namespace moet::kv4;
 // quarters; with D = 256 (512 tiles) 1289 and 1092 us.
 std::tuple<int64_t, int64_t, int64_t> kv4_prompt_plan(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t max_q,
                                                       int64_t W, int64_t window) {
-  constexpr int64_t kSms = 148;
-  const int64_t n = prompt_tiles(T, G, D, max_q) * H * B, rest = n % kSms;
+  const int64_t sms = sm_count();
+  const int64_t n = prompt_tiles(T, G, D, max_q) * H * B, rest = n % sms;
   const int64_t rt = D == 256 ? 128 : 256, keys = window > 0 ? std::min(W * kPage, window + (rt + G - 1) / G) : W * kPage;
-  if (rest == 0 || n >= 4 * kSms) return {n, 1, 0};
+  if (rest == 0 || n >= 4 * sms) return {n, 1, 0};
   int64_t best = 1;
-  if (n < kSms) {
-    best = std::min<int64_t>({kSms / n, keys / kMinStretch, 64});
+  if (n < sms) {
+    best = std::min<int64_t>({sms / n, keys / kMinStretch, 64});
   } else {
     for (int64_t s = 2; s <= std::min<int64_t>(keys / kMinStretch, 8); s++) {       // waves of stretches / s, 3 % for a split
-      const auto cost = [&](int64_t x) { return (double)((rest * x + kSms - 1) / kSms) / x + 0.03 * (x - 1); };
+      const auto cost = [&](int64_t x) { return (double)((rest * x + sms - 1) / sms) / x + 0.03 * (x - 1); };
       if (cost(s) < cost(best)) best = s;
     }
   }
@@ -726,7 +726,7 @@ void kv4_prompt_launch(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_le
     const dim3 grid((unsigned)(whole + rest * splits));
     moet_allow_max_smem(kv4_prompt_kernel<DD, T16>);
     launch_k(kv4_prompt_kernel<DD, T16>, grid, dim3(C::kWarps * 32), sizeof(PromptSmem<DD>), stream, a);
-    if (rest > 0)         // fewer than 148 tiles
+    if (rest > 0)         // fewer tiles than SMs
       launch_k(kv4_prompt_join_kernel<DD, T16>, dim3(C::TILES * 128 * DD / 8 / 256, (unsigned)rest), dim3(256), 0, stream, a);
   };
   auto by_type = [&](auto dim) {

@@ -436,7 +436,7 @@ void kv4_select_launch(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_le
   // 2 / 4 / 8 per SM, cold, choice included: 32 tokens over 1.1 M positions 36 / 34 / 36, 1024 tokens over
   // 512 pages 89 / 89 / 99.
   const int64_t per_chunk = (int64_t)a.B * a.tiles * a.H;
-  a.span = (int)std::max<int64_t>(1, std::min<int64_t>(a.chunks, per_chunk * a.chunks / (4 * 148)));
+  a.span = (int)std::max<int64_t>(1, std::min<int64_t>(a.chunks, per_chunk * a.chunks / (4 * sm_count())));
   const int64_t blocks = (int64_t)a.B * a.tiles * ((a.chunks + a.span - 1) / a.span);
   TORCH_CHECK(blocks < (int64_t)1 << 31 && (int64_t)a.T * a.H < (int64_t)1 << 31, "kv4: too much work for one call");
   auto stream = at::cuda::getCurrentCUDAStream();
@@ -464,7 +464,7 @@ void kv4_select_launch(torch::Tensor q, torch::Tensor cu_q, torch::Tensor seq_le
   // A warp per row, except for more than 512 pages (32 keys a lane) with fewer than two rows per SM, where the
   // latency of one row counts.  us of a whole choice, warp / block, 8 heads, back to back on B200: 32 tokens, 400
   // pages 18.9 / 19.5, 700 pages 26.1 / 22.0; 64 tokens, 700 pages 36.6 / 37.6; 512 tokens, 1000 pages 156 / 165.
-  const bool few = a.W > 512 && (int64_t)a.T * a.H < 2 * 148;
+  const bool few = a.W > 512 && (int64_t)a.T * a.H < 2 * sm_count();
   if (a.W <= 256) launch_k(kv4_pick_warp_kernel<8>, warps, four, 0, stream, a);
   else if (a.W <= 512) launch_k(kv4_pick_warp_kernel<16>, warps, four, 0, stream, a);
   else if (a.W <= 1024 && !few) launch_k(kv4_pick_warp_kernel<32>, warps, four, 0, stream, a);
