@@ -162,11 +162,9 @@ struct BoundsArgs {
   const uint8_t* pages; int8_t* bounds; float* unit; float k_mul;     // k_mul = 2^k_exp
 };
 
-// A warp per touched page and head.  The block looks at `win` slots (64 in a prompt, where a run in
-// one page is long; 2 where every slot may be a page of its own) and lists the last of each run in one
+// A warp per touched page and head.  The block looks at `win` slots and lists the last of each run in one
 // page; max and min are taken in f16, where the held values are exact.  Bound by the page's own latency
-// (its keys are read once more, out of L2).  B200, 8 heads of 128: 32 pages 3 us, 8183 rows (131 pages)
-// 9 us; all of a write and read back with win = 2 / 64: 32 decode rows 13 / 48 us, 8183 rows 62 / 32 us.
+// (its keys are read once more, out of L2).  B200, 8 heads of 128: 32 pages 3 us, 8183 rows (131 pages) 9 us.
 template <int D>
 __global__ void __launch_bounds__(64) kv4_bounds_kernel(BoundsArgs a) {
   using L = Lay<D>;
@@ -375,7 +373,12 @@ void kv4_append_launch(torch::Tensor k, torch::Tensor v, torch::Tensor slots, to
     using T16 = decltype(t);
     if (vec) launch_k(kv4_append_kernel<DD, T16, true>, grid, dim3(256), 0, stream, a);
     else launch_k(kv4_append_kernel<DD, T16, false>, grid, dim3(256), 0, stream, a);
-    BoundsArgs c{a.slots, T, H, a.n_slots, T >= 4096 ? 64 : 2, a.pages, (int8_t*)bounds.data_ptr(),
+    // Long runs in one page (prompts) want a long window, pages of one row each (decode steps) a short one, and the
+    // call does not say which it has: few rows may be either, more than 4096 are prompts.  us of an append with win =
+    // 2 / 8 / 64, 8 heads of 128, cold, B200: one prompt's rows, 256: 11.4 / 11.4 / 11.3, 1024: 15.3 / 13.4 / 13.4, 2048: 21.5 /
+    // 15.4 / 15.4, 8183: 54.4 / 29.8 / 25.6; rows of a page each, 32: 13 / 19.5 / 48, 512: 19.5 / 23.6 / 87, 2048: 42 / 44 / 118.
+    const int win = T > 4096 ? 64 : T >= 1024 ? 8 : 2;
+    BoundsArgs c{a.slots, T, H, a.n_slots, win, a.pages, (int8_t*)bounds.data_ptr(),
                  (float*)unit.data_ptr(), std::ldexp(1.f, (int)k_exp)};
     launch_k(kv4_bounds_kernel<DD>, dim3((T + c.win - 1) / c.win, H), dim3(64), 0, stream, c);
   };

@@ -1001,3 +1001,28 @@ def test_a_table_padded_to_the_longest_length(KV4Cache, lens, news, H, G, D, dty
         check(out, lse, x.oracle(0.1, window), max(lens))
         got.append((out, lse))
     assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+
+
+# ------------------------------------------------------------------------------- rows in one call or in several
+@pytest.mark.parametrize("T", [1023, 1024, 4096, 4097])
+@pytest.mark.parametrize("order", ["runs", "scattered", "mixed"])
+def test_one_append_is_what_several_are(KV4Cache, T, order):
+    """The bounds are looked for in other ways for few rows than for many: bytes, bounds and units are the same."""
+    g = torch.Generator().manual_seed(T)
+    P, H, D = 160, 2, 64
+    perm = torch.randperm(P, generator=g)
+    j = torch.arange(T)
+    runs = perm[j // 64] * 64 + j % 64
+    slots = {"runs": runs, "scattered": torch.randperm(P * 64, generator=g)[:T],
+             "mixed": torch.cat([runs[:T // 2], (perm[T // 128 + 1:, None] * 64 + torch.randperm(64, generator=g)).flatten()[:T - T // 2]])}[order]
+    assert len(slots.unique()) == T
+    k, v = ((torch.randn(T, H, D, generator=g) * 2).bfloat16().to(DEV) for _ in range(2))
+    slots = slots.to(DEV)
+    one, many = KV4Cache(P, H, D, device=DEV), KV4Cache(P, H, D, device=DEV)
+    one.append(k, v, slots)
+    for i in range(0, T, 300):
+        many.append(k[i:i + 300], v[i:i + 300], slots[i:i + 300])
+    assert torch.equal(one.pages, many.pages) and torch.equal(one.bounds, many.bounds) and torch.equal(one.unit, many.unit)
+    page = int(slots[T // 3]) // 64
+    want, unit = kv4.bounds(one.read(torch.arange(page * 64, page * 64 + 64, device=DEV), torch.float16)[0][:, 1].float().cpu())
+    assert torch.equal(one.bounds[page, 1].cpu(), want) and float(one.unit[page, 1]) == unit
