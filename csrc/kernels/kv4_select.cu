@@ -1,12 +1,14 @@
 // Choosing the pages that a query attends to, per token and K/V head.
 //
-// The score of a page is an upper bound on the logits of the head's query rows against the
-// page's keys, from the page bounds that kv4_cache.cu keeps (hi, lo in units e):
+// The score of a page estimates the largest product of the head's query rows with the page's
+// keys, from the page bounds that kv4_cache.cu keeps (hi, lo in units e):
 //   score = max over the head's rows of f e sum_d (max(r_d, 0) hi_d + min(r_d, 0) lo_d),
-// r = round(q / f), f the smallest power of two with max |q| <= 127 f.  The sum is an integer
-// below 2^24 (D <= 256 products of 7-bit numbers), f and e are powers of two: the score is
-// exact in f32 whatever the order of the additions, so every rank and every replay of a step
-// makes the same choice.  Ties go to the lowest page.
+// r = round(q / f), f the smallest power of two with max |q| <= 127 f.  It is an upper bound for
+// the rounded query f r; a product of q itself lies at most f / 2 sum_d max |k_d| above it (with
+// pages of equal keys and D = 128, one random query in ten does).  The scale is taken as positive.
+// The sum is an integer below 2^24 (D <= 256 products of 7-bit numbers), f and e are powers of two:
+// the score is exact in f32 whatever the order of the additions (queries between 2^-90 and 2^100),
+// so every rank and every replay of a step makes the same choice.  Ties go to the lowest page.
 //
 // Two launches.  Scores: the sum over d is one int8 matrix product of depth 2 D, [r+ | r-] by
 // [hi | lo]; a warp holds 16 pages' bounds as A fragments (16-byte loads, straight from

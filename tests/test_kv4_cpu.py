@@ -90,3 +90,21 @@ def test_the_sign_of_zero_is_kept():
     assert (codes[1, ::2] == 8).all() and (codes[1, 1::2] == 0).all()
     assert codes[2, :4].tolist() == [8, 7, 8, 0]
     assert torch.equal(kv4.values(codes, s8)[:2], torch.zeros(2, 64))
+
+
+def test_a_page_s_score_bounds_the_rounded_query():
+    """The score by which pages are chosen is an upper bound for the query rounded to 127 steps; a product of the query
+    itself lies at most half a step times sum |k| above it, and some do (pages of equal keys, nothing else to hide it)."""
+    g = torch.Generator().manual_seed(7)
+    above = 0
+    for _ in range(200):
+        k = kv4.values(*kv4.quantise(torch.randn(1, 128, generator=g))).double().expand(64, 128)
+        q = torch.randn(128, generator=g).double()
+        (hi, lo), e = kv4.bounds(k)
+        f = kv4.bounds(q[None])[1]
+        r = torch.round(q / f)
+        score = f * e * float(r.clamp(min=0) @ hi.double() + r.clamp(max=0) @ lo.double())
+        assert float(f * r @ k[0]) <= score
+        assert float(q @ k[0]) <= score + f / 2 * float(k[0].abs().sum())
+        above += float(q @ k[0]) > score
+    assert 0 < above < 60

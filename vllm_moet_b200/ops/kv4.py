@@ -1,7 +1,7 @@
 """4-bit paged K/V cache for layers with K/V heads of their own (grouped-query attention).
 
 The engine's NVFP4 cache row (``formats/kv_nvfp4.py``) is the MLA latent; this cache holds
-full K and V rows of grouped-query layers, such as drafters trained beside an MLA target, in
+full K and V rows of grouped-query layers that a user brings (the engine's own layers are MLA), in
 4.5 bits a value: e2m1 codes with one e4m3 scale per 16 values (``formats/kv4.py`` has the
 byte layout and the golden encoder).  It can be read whole or by chosen pages:
 
@@ -69,7 +69,7 @@ class KV4Cache:
         return self.num_kv_heads * 72 * self.head_dim // PAGE
 
     def check(self) -> None:
-        """Raise if a kernel has reported an error (synchronises)."""
+        """Raise if a kernel has reported an error (synchronises).  The first error stays until ``status`` is zeroed."""
         s = int(self.status)
         if s:
             raise RuntimeError(f"kv4: {_STATUS.get(s, f'status {s}')}")
@@ -77,7 +77,8 @@ class KV4Cache:
     # ------------------------------------------------------------------ operators
     def append(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
         """Quantise rows k, v [T, num_kv_heads, head_dim] (bf16 or f16, inner stride 1) into slots
-        ``page * 64 + offset``; a negative slot skips its row.  The bounds of every page touched
+        ``page * 64 + offset``; a negative slot skips its row.  Finite values past 2688 * 2^exp (42 by default) are
+        held as the largest value without a report; NaN and infinities set the status.  The bounds of every page touched
         are recomputed.  Rows may come in any order, but no slot twice in one call."""
         self._C.kv4_append(k, v, slots, self.pages, self.bounds, self.unit, self.status, self.k_exp, self.v_exp)
 
@@ -91,10 +92,12 @@ class KV4Cache:
         logical page indices in ascending order, -1 after the last where a row has fewer pages.
 
         The first ``first`` and the last ``last`` (>= 1) pages up to the row's own are always taken; the
-        others compete by an upper bound on their logits that is computed exactly, so equal inputs give
-        equal choices on every rank, and ties go to the lowest page.  A row past ``max_q`` of its sequence may
-        get no page, which sets the status.  Needs the rows' own positions
-        appended: pages before a row's last one must be complete."""
+        others compete by an estimate of their largest logit for a positive scale: the upper bound that
+        the page's bounds give for the query rounded to 8 bits.  It is computed exactly, so equal inputs give
+        equal choices on every rank, and ties go to the lowest page.  Where the table is wider than ``budget``,
+        rows * K/V heads * W floats of workspace are taken: give a table as wide as the longest sequence.
+        A row past ``max_q`` of its sequence may get no page, which sets the status.  Needs the rows' own
+        positions appended: pages before a row's last one must be complete."""
         return self._C.kv4_select(q, cu_q, seq_lens, block_table, budget, first, last, -1 if max_q is None else max_q,
                                   self.pages, self.bounds, self.unit, self.status)
 
@@ -103,9 +106,10 @@ class KV4Cache:
                return_lse: bool = False) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
         """softmax(scale * q k^T) v for every row of the batch -> [rows, heads, head_dim] in q's type.
 
-        ``max_q``: the most rows of one sequence (default: all rows); it sizes the work, so give it where it
-        is known.  Rows past it may come out as zeros, which sets the status.  ``window`` > 0: only the last
-        ``window`` positions up to the row's own.  ``pages`` int32 [rows, K/V heads, n]: only the
+        ``max_q``: the most rows of one sequence (default: all rows); it sizes the work and chooses between
+        two kernels for the whole batch, so give it where it is known, and serve long prompt chunks and decode
+        rows in calls of their own.  Rows past it may come out as zeros, which sets the status.  ``window`` > 0:
+        only the last ``window`` positions up to the row's own.  ``pages`` int32 [rows, K/V heads, n]: only the
         positions of these pages of the row's sequence (logical indices, each at most once, -1 for
         none), as :meth:`select` gives them.  A row that sees nothing is zeros.  ``return_lse``:
         also the natural log-sum-exp [rows, heads] f32 (-inf for a row that sees nothing)."""

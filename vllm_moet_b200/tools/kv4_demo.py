@@ -3,7 +3,7 @@
     python -m vllm_moet_b200.tools.kv4_demo [--hidden 4096 --heads 32 --kv-heads 8 --head-dim 128]
         [--streams 8] [--prompt 8192] [--chunk 2048] [--tokens 32] [--budget 32]
 
-One attention layer of a drafter trained beside an MLA target (q / k / v projections, RMS-normed
+One grouped-query attention layer, as a drafter of a user's own may have it (q / k / v projections, RMS-normed
 q and k heads, RoPE, output projection; random weights) runs as such a layer runs in serving:
 each stream's prompt in chunks (append the chunk's rows, attend to the whole context), then one
 token per stream and step over all pages, and once more with ``--budget`` pages chosen per token
