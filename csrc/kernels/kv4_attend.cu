@@ -10,7 +10,8 @@
 // accumulator layout to a B fragment by one 8x8 transpose per tile.  Queries are held as f16:
 // bf16 rows are scaled by a power of two to at most 512 first, which leaves their 8
 // significant bits whole down to 2^-23 of the row's maximum.  P <= 2^14 is rounded to f16 (11
-// bits, three more than a bf16 output has); references, sums and outputs stay in 32 bits.
+// bits, three more than a bf16 output has); references, sums and outputs stay in 32 bits.  exp2,
+// log2 and the division are the hardware's approximations (2^-21 or better, against P's 2^-11).
 //
 // What bounds it is the cache's bytes (a long context), so each warp streams its own units
 // (pages) through a private ring of bulk copies, one for a page's keys and one for its
@@ -21,7 +22,7 @@
 // block order.  A split tile is named by the block in which it begins, so the join needs no
 // counters and its grid is the first one's.
 //
-// B200: 32 sequences with 362 k positions together, 8 heads of 128, 8 rows each: 92 us, 4.5 TB/s (69 % of the
+// B200: 32 sequences with 362 k positions together, 8 heads of 128, 8 rows each: 94 us, 4.5 TB/s (68 % of the
 // measured copy rate); not the bytes but the instructions of the conversion bound it there (IPC 2.2 of
 // 4, ALU pipe 49 %, tensor 22 %, DRAM 46 %).  One sequence of 1000 positions: 8 us, a chain of
 // schedule, page look-up, one page per warp and join.

@@ -19,8 +19,8 @@
 // ones the cache's pieces give, so every 16-byte store of the conversion is one core-matrix row
 // and a warp's stores fill whole matrices without bank conflicts.
 //
-// B200, 2048 x 4 rows, 8 heads of 128, 16384 keys: 540 us for the kernel (568 with the join and the launches,
-// 910 TFLOP/s, 55 % of the measured bf16 rate).  The tensor path is busy 61 % of the time (64 keys a step
+// B200, 2048 x 4 rows, 8 heads of 128, 16384 keys: 551 us for the kernel (575 with the join and the launches,
+// 896 TFLOP/s, 54 % of the measured bf16 rate; 128 registers, 256 bytes of spills a thread).  The tensor path is busy 61 % of the time (64 keys a step
 // read Q and K from shared memory at three quarters of the product's own rate), exp2 46 %, the ALU
 // 34 %; the rest is the chain score, softmax, product of a step.  Measured and not taken: a warp per tile that
 // issues the products (570 us), eight warps that convert (586), 128 keys a step with one S
@@ -677,8 +677,8 @@ using namespace moet::kv4;
 // are split so that the last wave is even, unless four or more waves come before it.  The number of stretches
 // comes from the table's width (or the window) and is the most there can be; each tile takes as many as its own
 // keys fill with kMinStretch keys or more, and the blocks of the others leave at once.
-// 2048 x 4 rows, 8 heads, 16384 keys: 256 tiles, 556 us whole, 550 us with the last 108 in
-// quarters; with D = 256 (512 tiles) 1289 and 1092 us.
+// us whole / with the rest split, 8 heads x 4 rows, warm: 2048 tokens and 16384 keys (256 tiles), D = 64: 471 / 450, D = 128:
+// 551 / 542, D = 256 (512 tiles): 1190 / 1099; 1300 tokens, 8192 keys (168 tiles): 268 / 194; 1250 tokens, 32768 keys: 1112 / 674.
 std::tuple<int64_t, int64_t, int64_t> kv4_prompt_plan(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t max_q,
                                                       int64_t W, int64_t window) {
   const int64_t sms = sm_count();

@@ -5,7 +5,7 @@
 //   score = max over the head's rows of f e sum_d (max(r_d, 0) hi_d + min(r_d, 0) lo_d),
 // r = round(q / f), f the smallest power of two with max |q| <= 127 f.  It is an upper bound for
 // the rounded query f r; a product of q itself lies at most f / 2 sum_d max |k_d| above it (with
-// pages of equal keys and D = 128, one random query in ten does).  The scale is taken as positive.
+// pages of equal keys and D = 128, 6 random queries in 100 do).  The scale is taken as positive.
 // The sum is an integer below 2^24 (D <= 256 products of 7-bit numbers), f and e are powers of two:
 // the score is exact in f32 whatever the order of the additions (queries between 2^-90 and 2^100),
 // so every rank and every replay of a step makes the same choice.  Ties go to the lowest page.
