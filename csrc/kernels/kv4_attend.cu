@@ -24,7 +24,7 @@
 //
 // B200: 32 sequences with 362 k positions together, 8 heads of 128, 8 rows each: 94 us, 4.5 TB/s (68 % of the
 // measured copy rate); not the bytes but the instructions of the conversion bound it there (IPC 2.2 of
-// 4, ALU pipe 49 %, tensor 22 %, DRAM 46 %).  One sequence of 1000 positions: 8 us, a chain of
+// 4, ALU pipe 50 %, tensor 25 %, DRAM 55 %).  One sequence of 1000 positions: 8 us, a chain of
 // schedule, page look-up, one page per warp and join.
 #include "kv4.cuh"
 #include "tcgen05.cuh"

@@ -20,7 +20,7 @@
 // and a warp's stores fill whole matrices without bank conflicts.
 //
 // B200, 2048 x 4 rows, 8 heads of 128, 16384 keys: 551 us for the kernel (575 with the join and the launches,
-// 896 TFLOP/s, 54 % of the measured bf16 rate; 128 registers, 256 bytes of spills a thread).  The tensor path is busy 61 % of the time (64 keys a step
+// 896 TFLOP/s, 54 % of the measured bf16 rate; 128 registers, 256 bytes of spills a thread).  The tensor path is busy 60 % of the time (64 keys a step
 // read Q and K from shared memory at three quarters of the product's own rate), exp2 46 %, the ALU
 // 34 %; the rest is the chain score, softmax, product of a step.  Measured and not taken: a warp per tile that
 // issues the products (570 us), eight warps that convert (586), 128 keys a step with one S
