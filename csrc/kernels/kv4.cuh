@@ -81,6 +81,25 @@ MOET_DEVICE void join_pair(uint32_t a, uint32_t b, uint32_t& g0, uint32_t& g8) {
   g8 = ((a >> 4) & 0x0F0F0F0Fu) | (b & 0xF0F0F0F0u);
 }
 
+MOET_DEVICE uint32_t pack_f16x2(float a, float b) {
+  __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+MOET_DEVICE float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// two 16-bit values as floats, and back
+template <typename T16> MOET_DEVICE float2 unpack2(uint32_t v);
+template <> MOET_DEVICE float2 unpack2<__half>(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
+template <> MOET_DEVICE float2 unpack2<__nv_bfloat16>(uint32_t v) {
+  return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u));
+}
+template <typename T16> MOET_DEVICE uint32_t round2(float a, float b);
+template <> MOET_DEVICE uint32_t round2<__nv_bfloat16>(float a, float b) { return pack_bf16x2(a, b); }
+template <> MOET_DEVICE uint32_t round2<__half>(float a, float b) { return pack_f16x2(a, b); }
+
 template <typename T16> MOET_DEVICE float to_f32(T16 x);
 template <> MOET_DEVICE float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
 template <> MOET_DEVICE float to_f32(__half x) { return __half2float(x); }

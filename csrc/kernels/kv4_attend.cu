@@ -64,10 +64,6 @@ MOET_DEVICE uint32_t transpose_8x8(uint32_t x) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
   return d;
 }
-MOET_DEVICE uint32_t pack_f16x2(float a, float b) {
-  __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<uint32_t*>(&h);
-}
 // two f32 operations in one instruction
 MOET_DEVICE void mul2(float& x, float& y, float a, float b) {
   asm("{\n.reg .b64 u, v;\nmov.b64 u, {%0, %1};\nmov.b64 v, {%2, %3};\nmul.rn.ftz.f32x2 u, u, v;\nmov.b64 {%0, %1}, u;\n}\n"
@@ -76,11 +72,6 @@ MOET_DEVICE void mul2(float& x, float& y, float a, float b) {
 MOET_DEVICE void sub2(float& x, float& y, float a, float b) {
   asm("{\n.reg .b64 u, v;\nmov.b64 u, {%0, %1};\nmov.b64 v, {%2, %3};\nadd.rn.ftz.f32x2 u, u, v;\nmov.b64 {%0, %1}, u;\n}\n"
       : "+f"(x), "+f"(y) : "f"(-a), "f"(-b));
-}
-MOET_DEVICE float fast_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 // What a row's weights exp2(s - reference) refer to: 14 below its largest score, so that the weights use f16's range up to
 // 2^14 and those of a long tail, down to 2^-28 of the largest, keep all their bits.  Scores that are too large for
@@ -91,14 +82,6 @@ MOET_DEVICE void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t*
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                ::"r"(tc::smem_addr(dst)), "l"(src), "r"(bytes), "r"(tc::smem_addr(bar)) : "memory");
 }
-template <typename T16> MOET_DEVICE float2 unpack2(uint32_t v);
-template <> MOET_DEVICE float2 unpack2<__half>(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
-template <> MOET_DEVICE float2 unpack2<__nv_bfloat16>(uint32_t v) {
-  return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u));
-}
-template <typename T16> MOET_DEVICE uint32_t round2(float a, float b);
-template <> MOET_DEVICE uint32_t round2<__nv_bfloat16>(float a, float b) { return pack_bf16x2(a, b); }
-template <> MOET_DEVICE uint32_t round2<__half>(float a, float b) { return pack_f16x2(a, b); }
 
 // A unit of work: a page of one tile (sequence, row tile, head).
 struct Unit {

@@ -40,11 +40,6 @@ MOET_DEVICE void load16(const T16* p, uint32_t (&w)[8]) {
     for (int i = 0; i < 8; i++) w[i] = q[2 * i] | (uint32_t)q[2 * i + 1] << 16;
   }
 }
-template <typename T16> MOET_DEVICE float2 widen(uint32_t w);
-template <> MOET_DEVICE float2 widen<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
-template <> MOET_DEVICE float2 widen<__nv_bfloat16>(uint32_t w) {
-  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
-}
 template <typename T16> constexpr uint32_t kInf16 = std::is_same<T16, __half>::value ? 0x7C00u : 0x7F80u;
 
 // The scale byte of 16 values, and the values over the scale (what the codes are rounded from) in x.
@@ -54,11 +49,11 @@ template <typename T16> MOET_DEVICE uint32_t scale_of(const uint32_t (&w)[8], fl
 #pragma unroll
   for (int i = 0; i < 8; i++) {
     top = __vmaxu2(top, w[i] & 0x7FFF7FFFu);
-    const float2 f = widen<T16>(w[i]);
+    const float2 f = unpack2<T16>(w[i]);
     x[2 * i] = f.x, x[2 * i + 1] = f.y;
   }
   top = max(top >> 16, top & 0xFFFFu);
-  float amax = widen<T16>(top).x;
+  float amax = unpack2<T16>(top).x;
   if (top >= kInf16<T16>) {                              // NaN counts as 0, an infinity as a value past every scale
     bad = true;
     amax = 0.f;
@@ -262,7 +257,7 @@ MOET_DEVICE void values4(uint32_t w, int shift, uint32_t& a, uint32_t& b) {
 template <typename T16> MOET_DEVICE uint32_t out2(uint32_t v);
 template <> MOET_DEVICE uint32_t out2<__half>(uint32_t v) { return v; }
 template <> MOET_DEVICE uint32_t out2<__nv_bfloat16>(uint32_t v) {
-  const float2 f = widen<__half>(v);
+  const float2 f = unpack2<__half>(v);
   return pack_bf16x2(f.x, f.y);
 }
 // a scale times 2^exp, in both halves: every product with a code is exact in f16 (exp in [-14, 4])

@@ -121,11 +121,6 @@ MOET_DEVICE void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "
 MOET_DEVICE void arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc::smem_addr(bar)) : "memory");
 }
-MOET_DEVICE float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // x * c + b on a pair
 MOET_DEVICE void fma2(float& x, float& y, float c, float b) {
   asm("{\n.reg .b64 u, v, w;\nmov.b64 u, {%0, %1};\nmov.b64 v, {%2, %2};\nmov.b64 w, {%3, %3};\n"
@@ -140,18 +135,6 @@ MOET_DEVICE float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-template <typename T16> MOET_DEVICE float2 up2(uint32_t v);
-template <> MOET_DEVICE float2 up2<__half>(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
-template <> MOET_DEVICE float2 up2<__nv_bfloat16>(uint32_t v) {
-  return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u));
-}
-MOET_DEVICE uint32_t f16x2(float a, float b) {
-  __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<uint32_t*>(&h);
-}
-template <typename T16> MOET_DEVICE uint32_t down2(float a, float b);
-template <> MOET_DEVICE uint32_t down2<__half>(float a, float b) { return f16x2(a, b); }
-template <> MOET_DEVICE uint32_t down2<__nv_bfloat16>(float a, float b) { return pack_bf16x2(a, b); }
 }  // namespace pr
 
 // Keys of a stretch, at least.  us with 128 / 256 / 512, 8 K/V heads, 4 rows per token, B200: 128 tokens of 1000 keys,
@@ -269,7 +252,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
         const uint32_t w[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-          const float2 f = pr::up2<T16>(w[k]);
+          const float2 f = unpack2<T16>(w[k]);
           v[sl][8 * x + 2 * k] = f.x, v[sl][8 * x + 2 * k + 1] = f.y;
           amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
         }
@@ -293,7 +276,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
       for (int c = 0; c < E2 / 4; c++) {
         uint32_t w[4];
 #pragma unroll
-        for (int k = 0; k < 4; k++) w[k] = pr::f16x2(v[sl][4 * c + k] * mul, v[sl][E2 + 4 * c + k] * mul);
+        for (int k = 0; k < 4; k++) w[k] = pack_f16x2(v[sl][4 * c + k] * mul, v[sl][E2 + 4 * c + k] * mul);
         *reinterpret_cast<uint4*>(dst + (sl * (L::SD / 8) + t * (E2 / 4) + c) * 128) = make_uint4(w[0], w[1], w[2], w[3]);
       }
   }
@@ -353,7 +336,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
         top *= cs;
         const bool move = m == -INFINITY ? top > -INFINITY : top > m + kSlack;
         if (__any_sync(0xffffffffu, move)) {
-          const float f = !move ? 1.f : m == -INFINITY ? 0.f : pr::exp2_fast(m - top);
+          const float f = !move ? 1.f : m == -INFINITY ? 0.f : fast_exp2(m - top);
           if (move) m = top, rest = __fmaf_rn(raw, cs, -top);
           l *= f;
           // Once the product before is in O.  A wait by parity is right only if the phase before has ended:
@@ -383,9 +366,9 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
             float x = __uint_as_float(u[c][k]), y = __uint_as_float(u[c][k + 1]);
             pr::fma2(x, y, cs, -ref);
             pr::add2(x, y, kLift - rest, kLift - rest);
-            x = pr::exp2_fast(x), y = pr::exp2_fast(y);
+            x = fast_exp2(x), y = fast_exp2(y);
             pr::add2(s0, s1, x, y);
-            pk[k / 2] = pr::f16x2(x, y);
+            pk[k / 2] = pack_f16x2(x, y);
           }
           pr::st16(s_at + c * 16, pk);       // P takes the columns of the scores
         }
@@ -441,8 +424,8 @@ __global__ void __launch_bounds__(PromptCfg<D>::kWarps * 32, 1) kv4_prompt_kerne
 #pragma unroll
                 for (int k = 0; k < 8; k++) x[k] *= inv;
                 *reinterpret_cast<uint4*>((T16*)a.out + at * D + sl * L::SD + E * g + part_i * 8) =
-                    make_uint4(pr::down2<T16>(x[0], x[1]), pr::down2<T16>(x[2], x[3]), pr::down2<T16>(x[4], x[5]),
-                               pr::down2<T16>(x[6], x[7]));
+                    make_uint4(round2<T16>(x[0], x[1]), round2<T16>(x[2], x[3]), round2<T16>(x[4], x[5]),
+                               round2<T16>(x[6], x[7]));
               }
             }
           }
@@ -647,7 +630,7 @@ __global__ void __launch_bounds__(256) kv4_prompt_join_kernel(PromptArgs a) {
   for (int s = 0; s < tl.splits; s++) {
     const float m = p[s * PF + RT * D + r], l = p[s * PF + RT * (D + 1) + r];
     if (m == -INFINITY && l == 0.f) continue;          // a stretch of which the row saw nothing
-    const float w = m == -INFINITY ? 1.f : pr::exp2_fast(m - M);   // NaN sums have no maximum
+    const float w = m == -INFINITY ? 1.f : fast_exp2(m - M);   // NaN sums have no maximum
     const float4 y = *reinterpret_cast<const float4*>(p + s * PF + r * D + d), z = *reinterpret_cast<const float4*>(p + s * PF + r * D + d + 4);
     x[0] += w * y.x, x[1] += w * y.y, x[2] += w * y.z, x[3] += w * y.w;
     x[4] += w * z.x, x[5] += w * z.y, x[6] += w * z.z, x[7] += w * z.w;
@@ -656,8 +639,8 @@ __global__ void __launch_bounds__(256) kv4_prompt_join_kernel(PromptArgs a) {
   const float inv = sum > 0.f ? __fdividef(a.v_mul, sum) : sum;
   const long long at = (long long)(tl.c0 + row / a.G) * a.H * a.G + tl.h * a.G + row % a.G;
   *reinterpret_cast<uint4*>((T16*)a.out + at * D + d) =
-      make_uint4(pr::down2<T16>(x[0] * inv, x[1] * inv), pr::down2<T16>(x[2] * inv, x[3] * inv),
-                 pr::down2<T16>(x[4] * inv, x[5] * inv), pr::down2<T16>(x[6] * inv, x[7] * inv));
+      make_uint4(round2<T16>(x[0] * inv, x[1] * inv), round2<T16>(x[2] * inv, x[3] * inv),
+                 round2<T16>(x[4] * inv, x[5] * inv), round2<T16>(x[6] * inv, x[7] * inv));
   if (a.lse && d == 0) a.lse[at] = sum == 0.f ? -INFINITY : (M + (__log2f(sum) - kLift)) * 0.6931471805599453f;
 }
 

@@ -1026,3 +1026,19 @@ def test_one_append_is_what_several_are(KV4Cache, T, order):
     page = int(slots[T // 3]) // 64
     want, unit = kv4.bounds(one.read(torch.arange(page * 64, page * 64 + 64, device=DEV), torch.float16)[0][:, 1].float().cpu())
     assert torch.equal(one.bounds[page, 1].cpu(), want) and float(one.unit[page, 1]) == unit
+
+
+@pytest.mark.parametrize("max_q", [2, 100])
+@pytest.mark.parametrize("D,dtype", [(64, torch.float16), (128, torch.bfloat16), (256, torch.float16)])
+def test_unwritten_bytes_against_64_bits(KV4Cache, D, dtype, max_q):
+    """Pages of 0xFF (NaN scales) but for the sequences' own rows: outputs within the bound of every other case."""
+    x = Batch([70, 1, 190], [2, 1, 2], 1, 4, D, dtype, seed=53)
+    c = KV4Cache(x.n_pages, 1, D, device=DEV)
+    c.pages.fill_(0xFF)
+    c.append(x.k.to(DEV), x.v.to(DEV), x.slots.to(DEV))
+    out, lse = c.attend(*x.args(), 0.1, max_q=max_q, return_lse=True)
+    check(out, lse, x.oracle(0.1), 190)
+    pages = torch.tensor([[[1, 0]], [[0, 1]], [[0, -1]], [[2, 0]], [[1, 2]]], dtype=torch.int32)
+    out, lse = c.attend(*x.args(), 0.1, max_q=max_q, pages=pages.to(DEV), return_lse=True)
+    check(out, lse, x.oracle(0.1, pages=pages), 128)
+    c.check()
