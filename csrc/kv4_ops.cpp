@@ -40,8 +40,8 @@ std::string num(int64_t x) { return std::to_string(x); }
 Cache check_cache(const Tensor& pages, const Tensor& bounds, const Tensor& unit, const Tensor& status, int64_t k_exp,
                   int64_t v_exp) {
   TORCH_CHECK(pages.is_cuda() && pages.is_contiguous() && pages.scalar_type() == at::kByte && pages.dim() == 3 &&
-                  pages.size(0) >= 1 && pages.size(1) >= 1,
-              "kv4: pages must be a contiguous uint8 CUDA tensor [pages, kv_heads, 72 * head_dim]");
+                  pages.size(0) >= 1 && pages.size(1) >= 1 && pages.size(1) <= 65535,      // heads are a grid's second dimension
+              "kv4: pages must be a contiguous uint8 CUDA tensor [pages, kv_heads <= 65535, 72 * head_dim]");
   const Cache c{pages.size(0), pages.size(1), pages.size(2) / 72};
   TORCH_CHECK(pages.size(2) == 72 * c.D && (c.D == 64 || c.D == 128 || c.D == 256),
               "kv4: head_dim must be 64, 128 or 256");

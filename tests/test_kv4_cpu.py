@@ -108,3 +108,9 @@ def test_a_page_s_score_bounds_the_rounded_query():
         assert float(q @ k[0]) <= score + f / 2 * float(k[0].abs().sum())
         above += float(q @ k[0]) > score
     assert 0 < above < 60
+
+
+def test_more_heads_than_a_grid_has_rows_are_refused():
+    from vllm_moet_b200.ops.kv4 import KV4Cache
+    with pytest.raises(ValueError, match="65535"):
+        KV4Cache(1, 65536, 64)

@@ -1042,3 +1042,15 @@ def test_unwritten_bytes_against_64_bits(KV4Cache, D, dtype, max_q):
     out, lse = c.attend(*x.args(), 0.1, max_q=max_q, pages=pages.to(DEV), return_lse=True)
     check(out, lse, x.oracle(0.1, pages=pages), 128)
     c.check()
+
+
+def test_more_heads_than_a_grid_has_rows_are_refused(KV4Cache):
+    """Before anything is written: the bounds could not be recomputed."""
+    c = KV4Cache(1, 1, 64, device=DEV)
+    c.pages = torch.zeros(1, 65536, 72 * 64, dtype=torch.uint8, device=DEV)
+    c.bounds = torch.zeros(1, 65536, 2, 64, dtype=torch.int8, device=DEV)
+    c.unit = torch.ones(1, 65536, device=DEV)
+    k = torch.ones(1, 65536, 64, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(RuntimeError, match="65535"):
+        c.append(k, k, torch.zeros(1, dtype=torch.int64, device=DEV))
+    assert not c.pages.any()

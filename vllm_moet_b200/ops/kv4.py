@@ -49,6 +49,8 @@ class KV4Cache:
             raise ValueError(f"head_dim must be one of {HEAD_DIMS}, got {head_dim}")
         if num_pages < 1 or num_kv_heads < 1:
             raise ValueError("num_pages and num_kv_heads must be at least 1")
+        if num_kv_heads > 65535:
+            raise ValueError("num_kv_heads must be at most 65535 (a grid's second dimension)")
         if not (-14 <= k_exp <= 4 and -14 <= v_exp <= 4):
             raise ValueError("k_exp and v_exp must lie in [-14, 4] (what f16 holds exactly)")
         device = torch.device(device)
